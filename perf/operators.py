@@ -18,29 +18,29 @@ LR, BETAS, ADAM_EPS, DECAY, STEP0 = 1e-4, (0.9, 0.999), 1e-8, 1e-2, 1000
 def listed():
     return [
         # the bottleneck tokens of one half-second clip (55 tokens of width 64): latency
-        dict(name="norm forward, one clip", op="norm_fwd", rows=55, dim=64, dtype="fp32", pad=0),
+        dict(name="norm forward - one clip", op="norm_fwd", rows=55, dim=64, dtype="fp32", pad=0),
         # a long batch of wide half-precision tokens: bandwidth
-        dict(name="norm forward, wide tokens", op="norm_fwd", rows=65536, dim=2048, dtype="bf16", pad=0),
+        dict(name="norm forward - wide tokens", op="norm_fwd", rows=65536, dim=2048, dtype="bf16", pad=0),
         # the bottleneck tokens of a training batch of 1280 segments
-        dict(name="norm backward, train batch", op="norm_bwd", rows=70400, dim=64, dtype="fp32", pad=0),
+        dict(name="norm backward - train batch", op="norm_bwd", rows=70400, dim=64, dtype="fp32", pad=0),
         # one new token of one stream, the head sizes of the spectral model's bottleneck (6 heads of 10)
-        dict(name="decay token, one stream", op="decay_step", B=1, T=1, H=6, dk=10, dv=10, dtype="fp32", packed=False, ragged=False),
+        dict(name="decay token - one stream", op="decay_step", B=1, T=1, H=6, dk=10, dv=10, dtype="fp32", packed=False, ragged=False),
         # one new token of each of 1024 streams
-        dict(name="decay token, 1024 streams", op="decay_step", B=1024, T=1, H=8, dk=64, dv=64, dtype="bf16", packed=False, ragged=False),
+        dict(name="decay token - 1024 streams", op="decay_step", B=1024, T=1, H=8, dk=64, dv=64, dtype="bf16", packed=False, ragged=False),
         # a few clips of 55 tokens, q, k and v in one projection's output
-        dict(name="decay forward, clips", op="decay_fwd", B=8, T=55, H=6, dk=10, dv=10, dtype="fp32", packed=True, ragged=False),
+        dict(name="decay forward - clips", op="decay_fwd", B=8, T=55, H=6, dk=10, dv=10, dtype="fp32", packed=True, ragged=False),
         # a padded batch of clips of about ten seconds (100 tokens a second)
-        dict(name="decay forward, padded batch", op="decay_fwd", B=64, T=1001, H=8, dk=64, dv=64, dtype="bf16", packed=True, ragged=True),
+        dict(name="decay forward - padded batch", op="decay_fwd", B=64, T=1001, H=8, dk=64, dv=64, dtype="bf16", packed=True, ragged=True),
         # one recording of ten minutes: few rows, a long axis
-        dict(name="decay forward, recording", op="decay_fwd", B=1, T=60001, H=16, dk=128, dv=128, dtype="bf16", packed=False, ragged=False),
+        dict(name="decay forward - recording", op="decay_fwd", B=1, T=60001, H=16, dk=128, dv=128, dtype="bf16", packed=False, ragged=False),
         # forward and backward of a training batch in fp32, 8 heads of 16 (model width 128)
-        dict(name="decay training, fp32 heads", op="decay_train", B=64, T=1001, H=8, dk=16, dv=16, dtype="fp32", packed=True, ragged=True),
+        dict(name="decay training - fp32 heads", op="decay_train", B=64, T=1001, H=8, dk=16, dv=16, dtype="fp32", packed=True, ragged=True),
         # forward and backward with wide heads in half precision
-        dict(name="decay training, wide heads", op="decay_train", B=8, T=4096, H=16, dk=128, dv=128, dtype="bf16", packed=False, ragged=False),
+        dict(name="decay training - wide heads", op="decay_train", B=8, T=4096, H=16, dk=128, dv=128, dtype="bf16", packed=False, ragged=False),
         # the 76146 parameters of the spectral model
-        dict(name="adamw 32 bits, spectral model", op="adamw", tensors=128, numel=76146, bits=32, dtype="fp32", gdtype="fp32"),
+        dict(name="adamw 32 bits - spectral model", op="adamw", tensors=128, numel=76146, bits=32, dtype="fp32", gdtype="fp32"),
         # a large model with small states
-        dict(name="adamw 8 bits, large model", op="adamw", tensors=300, numel=150_000_000, bits=8, dtype="fp32", gdtype="bf16"),
+        dict(name="adamw 8 bits - large model", op="adamw", tensors=300, numel=150_000_000, bits=8, dtype="fp32", gdtype="bf16"),
     ]
 
 
