@@ -367,6 +367,30 @@ int noise_loss_finalize(const double* spec_partial, int n_spec, long spec_count,
 int noise_adamw_step(float* p, const float* g, float* m, float* v, long long* step, long n, float lr, float beta1,
                      float beta2, float eps, float weight_decay, float grad_scale, void* stream);
 
+/* The same update over `count` separate tensors, states in 32 or 8 bits.  p, g, numel, off, index and active are HOST arrays:
+ * tensor i has numel[i] values at device addresses p[i] / g[i], its states start at value off[i] (a multiple of 256) of the
+ * state buffers (every tensor's region padded to 256 values) and its coefficients are pair index[i] of coef.
+ * dtype codes: 0 fp32, 1 bf16, 2 fp16; gdtype == pdtype, or any with fp32 parameters.  bits 32: m, v fp32, scales unused;
+ * bits 8: m and v hold e4m3 bytes of the first moment and of the ROOT of the second, mscale / vscale one float per 256.
+ * noise_adamw_multi_begin first: step[i] += 1 and coef[i] for every i < n whose bit is set in active ((n + 63) / 64 words). */
+int noise_adamw_multi_begin(long long* step, float* coef, const unsigned long long* active, int n, double lr, double beta1,
+                            double beta2, void* stream);
+int noise_adamw_multi(const unsigned long long* p, const unsigned long long* g, const long* numel, const long* off,
+                      const int* index, int count, int pdtype, int gdtype, int bits, const float* coef, void* m, float* mscale,
+                      void* v, float* vscale, double lr, double beta1, double beta2, double eps, double weight_decay,
+                      double grad_scale, void* stream);
+
+/* ---- LayerNorm of token tensors, any width and type (train/models.py:90, :116, :214) ------------ */
+/* x [rows] x D with row stride ldx (elements), y [rows][D]; w, b [D] or NULL; mean, rstd [rows] fp32 or NULL.
+ * dtype: type of x, y; wdtype: type of w, b (fp32 or dtype) */
+int noise_layer_norm_fwd(const void* x, long ldx, const void* w, const void* b, float eps, void* y, float* mean, float* rstd,
+                         long rows, int D, int dtype, int wdtype, void* stream);
+/* dx [rows][D]; dw, db [D] in wdtype, or NULL; slab: noise_layer_norm_bwd_rows(rows, D) x 2D floats (NULL without dw, db) */
+int noise_layer_norm_bwd_rows(long rows, int D);
+int noise_layer_norm_bwd(const void* dy, long lddy, const void* x, long ldx, const float* mean, const float* rstd,
+                         const void* w, void* dx, void* dw, void* db, float* slab, long rows, int D, int dtype, int wdtype,
+                         void* stream);
+
 /* ---- once-for-all spectral U-Net forward (train/layers.py:496-668): every width, kernel size and depth is a run-time
  * choice, so these kernels are shape-generic (NHWC fp32, channel counts multiples of 4 up to any width).  Convolutions
  * write their raw output plus per-workgroup partial sums of y and y*y (`slab`: noise_ofa_max_rows() rows of 2C floats,

@@ -4,7 +4,8 @@ from . import _lib  # noqa: F401  (fails loudly when the kernel library is missi
 from .stft import STFT  # noqa: F401
 from .mixer import segmental_snr_mixer, activitydetector  # noqa: F401
 from .models import VADSpectralV2, VADMobileNetV2  # noqa: F401
-from .optim import FusedAdamW  # noqa: F401
+from .optim import FusedAdamW, MultiTensorAdamW  # noqa: F401
+from .layernorm import layer_norm, layer_norm_bwd, layer_norm_fwd  # noqa: F401
 from .data import VADNoiseDataModule  # noqa: F401
 from .streaming import StreamingDenoiser  # noqa: F401
 from .augment import AugmentPools, VADTrainAugment, add_pyreverb, impulse_response  # noqa: F401

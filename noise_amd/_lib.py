@@ -3,6 +3,7 @@
 The library is required: there is no fallback path.  Importing this module without the built
 library raises, and every wrapper raises RuntimeError(noise_last_error()) on a non-zero return.
 """
+import contextlib
 import ctypes
 import os
 
@@ -103,3 +104,17 @@ def require_cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("noise_amd kernels run on the GPU only: got a CPU tensor (no CPU fallback exists)")
+
+
+# element types of the token operators (codes of include/noise_hip.h)
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def on_device(*tensors):
+    """Context in which the launches and allocations of a call belong to the device its tensors live on, whichever device
+    is current in the caller; the tensors of one call must share a device."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors of one call live on different devices: {dev} and {t.device}")
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)

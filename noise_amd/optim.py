@@ -1,12 +1,21 @@
-"""Fused AdamW over the model's flat parameter buffer (one kernel launch per step).
+"""Fused AdamW: `FusedAdamW` over a model's flat parameter buffer (one kernel launch per step), `MultiTensorAdamW` over any
+list of separate tensors, with states in 32 or in 8 bits.
 
 Same update rule and defaults as the optimizer the reference wires through LightningCLI
 (train/main.py:13-14, train/configs/spectralv2.yaml:99-111): decoupled weight decay, no amsgrad.
 """
+import array
+import ctypes
+
 import torch
 
 from . import _lib
-from ._lib import ptr
+from ._lib import _D, _I, _P, ptr
+
+_lib.register({
+    "noise_adamw_multi_begin": [_P, _P, _P, _I, _D, _D, _D, _P],
+    "noise_adamw_multi": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _P, _P, _D, _D, _D, _D, _D, _D, _P],
+})
 
 
 class FusedAdamW:
@@ -45,4 +54,155 @@ class FusedAdamW:
         self._m.copy_(sd["exp_avg"])
         self._v.copy_(sd["exp_avg_sq"])
         self._step.copy_(sd["step"])
+        self.lr, self.betas, self.eps, self.weight_decay = sd["lr"], tuple(sd["betas"]), sd["eps"], sd["weight_decay"]
+
+
+class MultiTensorAdamW:
+    """AdamW over separate parameter tensors (fp32, bf16 or fp16, contiguous, on one GPU), a few launches per step for the
+    whole list.
+
+    Gradients have their parameter's type; an fp32 parameter also takes bf16 or fp16 gradients.  A parameter whose
+    gradient is None is left as it is and its step count does not advance.  The arithmetic is fp32 and a 16-bit parameter is
+    rounded once, to nearest: no fp32 master copy is kept.
+
+    `state_bits=32` keeps both moments in fp32 (8 bytes per value); `state_bits=8` keeps the first moment and the root of
+    the second as e4m3 values with one fp32 scale per 256 values of a tensor (2.03 bytes per value).  A block of 256 in
+    which a gradient is not finite gets NaN states.
+
+    `state` holds the flat state buffers (no copies): tensor i owns the values [offsets[i], offsets[i] + numel) of each,
+    every offset a multiple of 256, and scale [offsets[i] / 256 ...] of the scale buffers.
+    """
+    BLOCK = 256
+
+    def __init__(self, params, lr=1e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
+        self.params = list(params)
+        if not self.params:
+            raise ValueError("MultiTensorAdamW got an empty parameter list")
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits is 32 or 8, got {state_bits}")
+        if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and all(0 <= b < 1 for b in betas)):
+            raise ValueError(f"need lr, eps, weight_decay >= 0 and betas in [0, 1): got {lr}, {eps}, {weight_decay}, {betas}")
+        _lib.require_cuda(*self.params)
+        if len({id(p) for p in self.params}) < len(self.params):
+            raise ValueError("a parameter appears twice in the list")
+        dev = self.params[0].device
+        for i, p in enumerate(self.params):
+            if p.device != dev:
+                raise ValueError(f"parameters live on different devices: {dev} and {p.device}")
+            if p.dtype not in _lib.DTYPES:
+                raise TypeError(f"parameter {i} is {p.dtype}: float32, bfloat16 or float16 expected")
+            if not p.is_contiguous():
+                raise ValueError(f"parameter {i} of shape {tuple(p.shape)} is not contiguous")
+        self.lr, self.betas, self.eps, self.weight_decay = float(lr), (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
+        self.state_bits = state_bits
+        n = len(self.params)
+        self._numel = [p.numel() for p in self.params]
+        self.offsets, total = [], 0
+        for k in self._numel:
+            self.offsets.append(total)
+            total += (k + self.BLOCK - 1) // self.BLOCK * self.BLOCK
+        total = max(total, self.BLOCK)
+        z = dict(device=dev)
+        if state_bits == 8:
+            # the bytes of +0 are zero
+            small = lambda: torch.zeros(total, dtype=torch.uint8, **z).view(torch.float8_e4m3fn)
+            scales = lambda: torch.zeros(total // self.BLOCK, **z)
+            self.state = {"exp_avg": small(), "exp_avg_scale": scales(), "exp_avg_sq_root": small(), "exp_avg_sq_root_scale": scales()}
+        else:
+            self.state = {"exp_avg": torch.zeros(total, **z), "exp_avg_sq": torch.zeros(total, **z)}
+        self.step_count = torch.zeros(n, dtype=torch.int64, **z)
+        self._coef = torch.empty(n, 2, **z)
+
+    def zero_grad(self, set_to_none=True):
+        for p in self.params:
+            if set_to_none:
+                p.grad = None
+            elif p.grad is not None:
+                p.grad.zero_()
+
+    @torch.no_grad()
+    def step(self, grad_scale=1.0, grads=None):
+        """One update from `grads` (one tensor or None per parameter), the parameters' own `.grad` when omitted.
+        `grad_scale` multiplies every gradient (1 / world size of a summed data-parallel gradient)."""
+        params = self.params
+        grads = [p.grad for p in params] if grads is None else list(grads)
+        n = len(params)
+        if len(grads) != n:
+            raise ValueError(f"{len(grads)} gradients for {n} parameters")
+        live = [i for i in range(n) if grads[i] is not None]
+        if len(live) == 0:
+            return
+        self._check(live, grads)
+        if len(live) < n:
+            keep = list(live)
+            params, grads = [params[i] for i in keep], [grads[i] for i in keep]
+        groups = {}
+        kinds = list(zip((p.dtype for p in params), (g.dtype for g in grads)))
+        if len(set(kinds)) == 1:
+            groups[kinds[0]] = range(len(params))
+        else:
+            for j, kind in enumerate(kinds):
+                groups.setdefault(kind, []).append(j)
+        for pd, gd in groups:
+            if pd not in _lib.DTYPES or (gd != pd and not (pd == torch.float32 and gd in _lib.DTYPES)):
+                raise TypeError(f"a {pd} parameter cannot take a {gd} gradient")
+        index = array.array("i", live)
+        off = array.array("l", self.offsets if len(live) == n else [self.offsets[i] for i in live])
+        numel = array.array("l", self._numel if len(live) == n else [self._numel[i] for i in live])
+        pp = array.array("Q", map(torch.Tensor.data_ptr, params))
+        gp = array.array("Q", map(torch.Tensor.data_ptr, grads))
+        words = [0] * ((n + 63) // 64)
+        if len(live) == n:
+            words = [0xffffffffffffffff] * len(words)
+        else:
+            for i in live:
+                words[i >> 6] |= 1 << (i & 63)
+        mask = array.array("Q", words)
+        s = self.state
+        if self.state_bits == 8:
+            bufs = (s["exp_avg"], s["exp_avg_scale"], s["exp_avg_sq_root"], s["exp_avg_sq_root_scale"])
+        else:
+            bufs = (s["exp_avg"], None, s["exp_avg_sq"], None)
+        bufs = [ptr(b) for b in bufs]
+        addr = lambda a: ctypes.c_void_p(a.buffer_info()[0])
+        with _lib.on_device(self.step_count):
+            st = _lib.stream()
+            _lib.call("noise_adamw_multi_begin", ptr(self.step_count), ptr(self._coef), addr(mask), n, self.lr, *self.betas, st)
+            for (pd, gd), js in groups.items():
+                lists = [pp, gp, numel, off, index]
+                if len(js) < len(params):
+                    lists = [array.array(a.typecode, [a[j] for j in js]) for a in lists]
+                state_bytes = 4 if self.state_bits == 8 else 16
+                _lib.call("noise_adamw_multi", *map(addr, lists), len(js), _lib.DTYPES[pd], _lib.DTYPES[gd], self.state_bits,
+                          ptr(self._coef), *bufs, self.lr, *self.betas, self.eps, self.weight_decay, float(grad_scale), st,
+                          nbytes=sum(lists[2]) * (state_bytes + 2 * pd.itemsize + gd.itemsize) if _lib.PROFILE is not None else 0)
+        # the kernel wrote through raw pointers: autograd's and the models' stale-weight checks go by the version counters
+        torch.autograd.graph.increment_version(params)
+
+    def _check(self, live, grads):
+        dev = self.step_count.device
+        for i in live:
+            g, p = grads[i], self.params[i]
+            if g.shape != p.shape or g.device != dev:
+                raise ValueError(f"gradient {i} is {tuple(g.shape)} on {g.device}, its parameter {tuple(p.shape)} on {dev}")
+            if not g.is_contiguous():
+                grads[i] = g.contiguous()
+            if p.device != dev or p.numel() != self._numel[i] or not p.is_contiguous():
+                raise RuntimeError(f"parameter {i} was moved, resized or transposed after the optimizer was built")
+
+    def state_dict(self):
+        return {**{k: v.clone() for k, v in self.state.items()}, "step": self.step_count.clone(), "state_bits": self.state_bits,
+                "lr": self.lr, "betas": self.betas, "eps": self.eps, "weight_decay": self.weight_decay}
+
+    def load_state_dict(self, sd):
+        if sd.get("state_bits") != self.state_bits:
+            raise ValueError(f"a checkpoint with {sd.get('state_bits')}-bit states cannot be loaded into {self.state_bits}-bit ones")
+        for k, v in {**self.state, "step": self.step_count}.items():
+            if k not in sd or sd[k].shape != v.shape or sd[k].dtype != v.dtype:
+                raise ValueError(f"state {k!r} must be {v.dtype} {tuple(v.shape)}")
+        for k, v in self.state.items():
+            # bytes: 8-bit values are copied as they are
+            (v.view(torch.uint8) if self.state_bits == 8 and v.dtype == torch.float8_e4m3fn else v).copy_(
+                sd[k].view(torch.uint8) if v.dtype == torch.float8_e4m3fn else sd[k])
+        self.step_count.copy_(sd["step"])
         self.lr, self.betas, self.eps, self.weight_decay = sd["lr"], tuple(sd["betas"]), sd["eps"], sd["weight_decay"]

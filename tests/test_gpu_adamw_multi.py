@@ -1,0 +1,286 @@
+"""MultiTensorAdamW (csrc/adamw_multi.hip) against the update rule in 64 bits, the 8-bit states byte for byte."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+U = 2.0 ** -24
+SIZES = [1, 0, 3, 255, 256, 257, 1000, 4095, 4096, 4097, 9001, 16, 64]
+
+
+def tensors(sizes, pdtype, gdtype, seed, at=0):
+    """Parameters and gradients as views `at` values into their buffers (at % 4 != 0: no 16-byte alignment)."""
+    g = torch.Generator().manual_seed(seed)
+    ps, gs = [], []
+    for i, n in enumerate(sizes):
+        ps.append((0.1 * torch.randn(n + at, generator=g)).to(pdtype).to(DEV)[at:])
+        gs.append((torch.randn(n + at, generator=g) * 10.0 ** (i % 5 - 4) * torch.exp(2 * torch.randn(n + at, generator=g))).to(gdtype).to(DEV)[at:])
+    return [torch.nn.Parameter(p) for p in ps], gs
+
+
+# ---- the rule in 64 bits
+def e4m3_table():
+    c = torch.arange(127, dtype=torch.float64)
+    e, m = torch.div(c, 8, rounding_mode="floor"), c % 8
+    return torch.where(e > 0, (1 + m / 8) * 2.0 ** (e - 7), m / 8 * 2.0 ** -6)
+
+
+TABLE = e4m3_table()
+
+
+def small(t, lowest):
+    """64-bit values -> (codes 0..126 with a sign bit, scales): nearest, ties to even."""
+    n = t.numel()
+    pad = torch.zeros((n + 255) // 256 * 256, dtype=torch.float64)
+    pad[:n] = t
+    rows = pad.view(-1, 256)
+    scale = (rows.abs().amax(1) / 448.0).float()
+    a = torch.where(scale[:, None] > 0, rows.abs() / scale.double()[:, None], 0.0).clamp_max(448.0).reshape(-1)
+    mids = (TABLE[1:] + TABLE[:-1]) / 2
+    c = torch.searchsorted(mids, a)
+    tie = (c < 126) & (mids[c.clamp(max=125)] == a)
+    c = torch.where(tie & (c % 2 == 1), c + 1, c)
+    if lowest:
+        c = torch.where((pad > 0) & (c == 0), 1, c)
+    return (c + 128 * (torch.signbit(pad))).to(torch.uint8), scale
+
+
+def value(codes, scale, n):
+    v = TABLE[(codes.long() & 127)] * torch.where(codes >= 128, -1.0, 1.0)
+    return (v.view(-1, 256) * scale.double()[:, None]).reshape(-1)[:n]
+
+
+class Rule:
+    """AdamW of one tensor in 64 bits on the CPU; the states are rounded to their own type after every step."""
+
+    def __init__(self, p, bits):
+        self.p, self.bits, self.t, self.dtype = p.detach().double().cpu(), bits, 0, p.dtype
+        n = p.numel()
+        if bits == 8:
+            z = torch.zeros((n + 255) // 256 * 256, dtype=torch.uint8)
+            self.m = self.r = (z, torch.zeros(z.numel() // 256))
+        else:
+            self.m = self.v = torch.zeros(n, dtype=torch.float64)
+
+    def step(self, g, lr, b1, b2, eps, wd, scale=1.0):
+        """Returns (p before rounding, magnitude of the terms of p)."""
+        n = self.p.numel()
+        g = (g.detach().float().cpu() * scale).double()
+        self.t += 1
+        if self.bits == 8:
+            m, r = value(*self.m, n), value(*self.r, n)
+            m, v = b1 * m + (1 - b1) * g, b2 * r * r + (1 - b2) * g * g
+            self.m, self.r = small(m, False), small(v.sqrt(), True)
+        else:
+            m = self.m = b1 * self.m + (1 - b1) * g
+            v = self.v = b2 * self.v + (1 - b2) * g * g
+        u = lr / (1 - b1 ** self.t) * m / (v.sqrt() / math.sqrt(1 - b2 ** self.t) + eps)
+        self.p = self.p * (1 - lr * wd) - u
+        return self.p.abs() + 2 * u.abs()
+
+
+def close_p(got, rule, mag, steps):
+    """fp32 arithmetic: at most 12 roundings of the terms a step (moments, root, two divisions, the products and the sum),
+    then half a step of the parameter's type per update (none for fp32 beyond those)."""
+    tol = steps * 12 * U * mag + 1e-30
+    if got.dtype != torch.float32:
+        tol = tol + steps * torch.finfo(got.dtype).eps / 2 * mag * 1.01 + steps * torch.finfo(got.dtype).smallest_normal
+    d = (got.detach().double().cpu() - rule.p).abs()
+    assert (d <= tol).all(), (d / tol).max()
+
+
+def regions(opt, key, i):
+    o, n = opt.offsets[i], opt.params[i].numel()
+    if "scale" in key:
+        return opt.state[key][o // 256:o // 256 + (n + 255) // 256].cpu()
+    t = opt.state[key][o:o + (n + 255) // 256 * 256]
+    return (t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t).cpu()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("at", [0, 1])
+@pytest.mark.parametrize("pdtype,gdtype", [(torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.float32, torch.float16),
+                                           (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16)])
+def test_update_rule(pdtype, gdtype, at, bits):
+    import noise_amd as na
+    hyper = dict(lr=3e-3, betas=(0.8, 0.97), eps=1e-8, weight_decay=0.1)
+    params, grads = tensors(SIZES, pdtype, gdtype, 3, at)
+    rules = [Rule(p, bits) for p in params]
+    opt = na.MultiTensorAdamW(params, state_bits=bits, **hyper)
+    for step in range(1, 4):
+        gs = [(g.float() * (1 + 0.5 * step)).to(gdtype) for g in grads]
+        opt.step(grads=gs)
+        for i, (p, g, rule) in enumerate(zip(params, gs, rules)):
+            mag = rule.step(g, hyper["lr"], *hyper["betas"], hyper["eps"], hyper["weight_decay"])
+            if p.numel() == 0:
+                continue
+            close_p(p, rule, mag, 1)
+            rule.p = p.detach().double().cpu()           # each step's rounding is judged by itself
+            n = p.numel()
+            if bits == 8:
+                for key, (codes, scale) in (("exp_avg", rule.m), ("exp_avg_sq_root", rule.r)):
+                    assert torch.equal(regions(opt, key + "_scale", i), scale), (key, i)
+                    got = regions(opt, key, i)
+                    same = (got == codes) | ((got & 127 == 0) & (codes & 127 == 0))      # -0 and +0
+                    assert same.all(), (key, i, (~same).nonzero()[:4])
+            else:
+                m, v = regions(opt, "exp_avg", i), regions(opt, "exp_avg_sq", i)
+                assert not m[n:].any() and not v[n:].any()
+                # two products and a sum a step on states that started equal: 3 roundings of the terms' magnitudes
+                gm = g.double().cpu().abs()
+                assert ((m[:n].double() - rule.m).abs() <= 8 * U * (rule.m.abs() + gm) + 1e-38).all()
+                assert ((v[:n].double() - rule.v).abs() <= 12 * U * rule.v + 1e-38).all()
+                rule.m, rule.v = m[:n].double(), v[:n].double()
+    assert (opt.step_count == 3).all()
+
+
+def test_matches_the_flat_optimizer():
+    """The same numbers through FusedAdamW's kernel: the two differ by the rounding of a few products."""
+    import noise_amd as na
+    from noise_amd import _lib
+    n = 5000
+    g = torch.Generator().manual_seed(1)
+    p0, gr = torch.randn(n, generator=g).to(DEV), torch.randn(n, generator=g).to(DEV)
+    q = torch.nn.Parameter(p0.clone())
+    opt = na.MultiTensorAdamW([q], lr=1e-2)
+    p, m, v, step = p0.clone(), torch.zeros(n, device=DEV), torch.zeros(n, device=DEV), torch.zeros((), dtype=torch.int64, device=DEV)
+    for _ in range(4):
+        opt.step(grads=[gr])
+        _lib.call("noise_adamw_step", *(_lib.ptr(t) for t in (p, gr, m, v, step)), n, 1e-2, 0.9, 0.999, 1e-8, 1e-2, 1.0, _lib.stream())
+    assert ((p - q.detach()).abs() <= 4 * 24 * U * (p.abs() + 0.02)).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_tensors_missing_gradients_and_mixed_types(bits):
+    """More tensors than one launch holds, of two types in one list, some without a gradient: those keep their values, states
+    and step count."""
+    import noise_amd as na
+    sizes = [(i * 37) % 700 for i in range(230)]
+    params, grads = tensors(sizes, torch.float32, torch.float32, 11)
+    for i in range(0, 230, 3):
+        params[i] = torch.nn.Parameter(params[i].detach().bfloat16())
+        grads[i] = grads[i].bfloat16()
+    before = [p.detach().clone() for p in params]
+    rules = [Rule(p, bits) for p in params]
+    opt = na.MultiTensorAdamW(params, lr=1e-2, state_bits=bits)
+    for step in range(2):
+        gs = [None if (i + step) % 5 == 0 else g for i, g in enumerate(grads)]
+        for p, g in zip(params, gs):
+            p.grad = g
+        opt.step()
+        for i, (p, g) in enumerate(zip(params, gs)):
+            if g is None:
+                if step == 0:
+                    assert torch.equal(p.detach(), before[i]) and not regions(opt, "exp_avg", i).any()
+            elif p.numel():
+                close_p(p, rules[i], rules[i].step(g, 1e-2, 0.9, 0.999, 1e-8, 1e-2), 1)
+                rules[i].p = p.detach().double().cpu()
+    want = torch.tensor([sum((i + s) % 5 != 0 for s in range(2)) for i in range(230)])
+    assert torch.equal(opt.step_count.cpu(), want)
+    opt.zero_grad()
+    assert all(p.grad is None for p in params)
+    opt.step()                                          # nothing to do
+    assert torch.equal(opt.step_count.cpu(), want)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_grad_scale_checkpoint_and_versions(bits):
+    import noise_amd as na
+    params, grads = tensors([300, 1000], torch.float32, torch.float32, 5)
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    opt = na.MultiTensorAdamW(params, lr=1e-2, state_bits=bits)
+    version = params[0]._version
+    opt.step(grad_scale=0.25, grads=[4 * g for g in grads])     # powers of two: exact
+    assert params[0]._version > version
+    other = na.MultiTensorAdamW(twin, lr=1e-2, state_bits=bits)
+    other.step(grads=grads)
+    assert all(torch.equal(a, b) for a, b in zip(params, twin))
+    third = na.MultiTensorAdamW([torch.nn.Parameter(p.detach().clone()) for p in params], state_bits=bits)
+    sd = {k: (v.cpu() if torch.is_tensor(v) else v) for k, v in opt.state_dict().items()}
+    third.load_state_dict(sd)
+    assert third.lr == 1e-2
+    for o in (opt, third):
+        o.step(grads=grads)
+    assert all(torch.equal(a, b) for a, b in zip(opt.params, third.params))
+    assert all(torch.equal(opt.state[k].view(torch.uint8), third.state[k].view(torch.uint8)) for k in opt.state)
+    with pytest.raises(ValueError, match="-bit states"):
+        na.MultiTensorAdamW(twin, state_bits=40 - bits).load_state_dict(sd)
+    with pytest.raises(ValueError, match="state 'exp_avg'"):
+        na.MultiTensorAdamW(twin[:1], state_bits=bits).load_state_dict(sd)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_extreme_gradients(bits):
+    """Zeros, tiny and huge gradients; a NaN reaches only its own value (32 bits) or its block of 256 (8 bits)."""
+    import noise_amd as na
+    n = 1024
+    p = torch.nn.Parameter(torch.ones(n, device=DEV))
+    g = torch.zeros(n, device=DEV)
+    g[256:512] = torch.logspace(-18, 18, 256, device=DEV)
+    g[512] = float("nan")
+    g[768:] = 1e-20
+    opt = na.MultiTensorAdamW([p], lr=1e-3, weight_decay=0.0, state_bits=bits)
+    opt.step(grads=[g])
+    assert (p[:256] == 1).all() and torch.isfinite(p[:512]).all() and torch.isnan(p[512]) and torch.isfinite(p[513:]).all()
+    # first step: every update is lr * g / (|g| + eps sqrt(1 - b2) ...), never more than lr
+    assert ((p[256:512] - 1).abs() <= 1e-3 * (1 + 1e-4)).all()
+    opt.step(grads=[torch.zeros_like(g)])
+    bad = torch.isnan(p.detach()).cpu()
+    assert bad[512] and not bad[:512].any() and not bad[768:].any()
+    assert bad.sum() == (1 if bits == 32 else 256)
+    # a positive second moment is never stored as zero: no step of a later small gradient exceeds a few lr
+    assert ((p[256:512] - 1).abs() < 5e-3).all()
+
+
+def test_refusals():
+    import noise_amd as na
+    p, g = tensors([8, 12], torch.float32, torch.float32, 1)
+    with pytest.raises(ValueError, match="twice"):
+        na.MultiTensorAdamW([p[0], p[0]])
+    with pytest.raises(TypeError, match="float64"):
+        na.MultiTensorAdamW([torch.nn.Parameter(torch.zeros(3, device=DEV, dtype=torch.float64))])
+    with pytest.raises(ValueError, match="contiguous"):
+        na.MultiTensorAdamW([torch.nn.Parameter(torch.zeros(4, 6, device=DEV).t())])
+    opt = na.MultiTensorAdamW(p)
+    with pytest.raises(ValueError, match="gradients for"):
+        opt.step(grads=g[:1])
+    with pytest.raises(ValueError, match="gradient 1"):
+        opt.step(grads=[g[0], g[0]])
+    with pytest.raises(TypeError, match="cannot take"):
+        opt.step(grads=[g[0].double(), g[1]])
+    with pytest.raises(ValueError, match="gradient 0"):
+        opt.step(grads=[g[0].cpu(), g[1]])
+    assert not opt.step_count.any()
+    half = na.MultiTensorAdamW([torch.nn.Parameter(torch.zeros(8, device=DEV, dtype=torch.bfloat16))])
+    with pytest.raises(TypeError, match="cannot take"):
+        half.step(grads=[g[0]])
+    # a transposed gradient is read through a packed copy
+    q = torch.nn.Parameter(torch.zeros(4, 6, device=DEV))
+    gt = torch.randn(6, 4, device=DEV).t()
+    a, b = na.MultiTensorAdamW([q]), na.MultiTensorAdamW([torch.nn.Parameter(torch.zeros(4, 6, device=DEV))])
+    a.step(grads=[gt])
+    b.step(grads=[gt.contiguous()])
+    assert torch.equal(q, b.params[0])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_step_replays(bits):
+    import noise_amd as na
+    params, grads = tensors([100, 5000, 7], torch.float32, torch.float32, 21)
+    twin = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    a, b = na.MultiTensorAdamW(params, lr=1e-2, state_bits=bits), na.MultiTensorAdamW(twin, lr=1e-2, state_bits=bits)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        a.step(grads=grads)
+    assert not a.step_count.any()
+    for k in range(4):
+        for g in grads:
+            g.mul_(1.0 - 0.1 * k)
+        graph.replay()
+        b.step(grads=grads)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(params, twin)) and (a.step_count == k + 1).all()

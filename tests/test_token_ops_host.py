@@ -1,0 +1,61 @@
+"""Argument checks of the token operators that need no GPU: what they refuse, before any launch."""
+import ctypes
+
+import pytest
+import torch
+
+
+def test_cpu_tensors_are_refused():
+    import noise_amd as na
+    x = torch.zeros(2, 8)
+    with pytest.raises(RuntimeError, match="GPU"):
+        na.layer_norm(x, torch.ones(8), torch.zeros(8))
+    with pytest.raises(RuntimeError, match="GPU"):
+        na.layer_norm_bwd(x, x, torch.zeros(2), torch.ones(2))
+    with pytest.raises(RuntimeError, match="GPU"):
+        na.MultiTensorAdamW([torch.nn.Parameter(x)])
+
+
+def test_optimizer_arguments():
+    import noise_amd as na
+    p = [torch.nn.Parameter(torch.zeros(3))]
+    with pytest.raises(ValueError, match="empty"):
+        na.MultiTensorAdamW([])
+    with pytest.raises(ValueError, match="state_bits"):
+        na.MultiTensorAdamW(p, state_bits=16)
+    for kw in (dict(lr=-1), dict(eps=-1e-8), dict(betas=(0.9, 1.0)), dict(betas=(-0.1, 0.9)), dict(weight_decay=-1), dict(lr=float("nan"))):
+        with pytest.raises(ValueError, match="need lr"):
+            na.MultiTensorAdamW(p, **kw)
+
+
+def test_c_entry_points_refuse_bad_arguments():
+    """Bad sizes, types and null pointers come back as errors: nothing is launched."""
+    from noise_amd import _lib
+    one = ctypes.c_void_p(16)
+    for args, text in (((None, 8, None, None, 1e-6, one, None, None, 1, 8, 0, 0, None), "null"),
+                       ((one, 8, None, None, 1e-6, one, None, None, 0, 8, 0, 0, None), "rows"),
+                       ((one, 8, None, None, 1e-6, one, None, None, 1, 0, 0, 0, None), "rows"),
+                       ((one, -8, None, None, 1e-6, one, None, None, 1, 8, 0, 0, None), "stride"),
+                       ((one, 8, None, None, 1e-6, one, None, None, 1, 8, 3, 0, None), "type"),
+                       ((one, 8, None, None, 1e-6, one, None, None, 1, 8, 1, 2, None), "type")):
+        with pytest.raises(RuntimeError, match=text):
+            _lib.call("noise_layer_norm_fwd", *args)
+    with pytest.raises(RuntimeError, match="null"):
+        _lib.call("noise_layer_norm_bwd", one, 8, one, 8, None, one, None, one, None, None, None, 1, 8, 0, 0, None)
+    with pytest.raises(RuntimeError, match="slab"):
+        _lib.call("noise_layer_norm_bwd", one, 8, one, 8, one, one, None, one, one, None, None, 1, 8, 0, 0, None)
+    assert _lib.lib.noise_layer_norm_bwd_rows(10 ** 6, 64) == 1024 and _lib.lib.noise_layer_norm_bwd_rows(5, 64) == 5
+    assert _lib.lib.noise_layer_norm_bwd_rows(10 ** 6, 1 << 20) == 64
+    with pytest.raises(RuntimeError, match="bad argument"):
+        _lib.call("noise_adamw_multi_begin", None, None, None, 1, 1e-3, 0.9, 0.99, None)
+    import array
+    q, l, i = array.array("Q", [64]), array.array("l", [4]), array.array("i", [0])
+    a = lambda x: ctypes.c_void_p(x.buffer_info()[0])
+    off = array.array("l", [0])
+    tail = (one, one, None, one, None, 1e-3, 0.9, 0.99, 1e-8, 0.0, 1.0, None)
+    for pd, gd, bits, text in ((0, 0, 16, "32 bits"), (0, 0, 8, "32 bits"), (1, 2, 32, "type"), (3, 3, 32, "type"), (1, 0, 32, "type")):
+        with pytest.raises(RuntimeError, match=text):
+            _lib.call("noise_adamw_multi", a(q), a(q), a(l), a(off), a(i), 1, pd, gd, bits, *tail)
+    for bad in (dict(off=array.array("l", [100])), dict(l=array.array("l", [-1])), dict(q=array.array("Q", [0]))):
+        with pytest.raises(RuntimeError, match="tensor 0"):
+            _lib.call("noise_adamw_multi", a(bad.get("q", q)), a(q), a(bad.get("l", l)), a(bad.get("off", off)), a(i), 1, 0, 0, 32, *tail)
