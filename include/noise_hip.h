@@ -391,6 +391,21 @@ int noise_layer_norm_bwd(const void* dy, long lddy, const void* x, long ldx, con
                          const void* w, void* dx, void* dw, void* db, float* slab, long rows, int D, int dtype, int wdtype,
                          void* stream);
 
+/* ---- decay attention: causal linear attention with one decay per head ---------------------------- */
+/* X_p = e^g X_{p-1} + s_kv k_p (x) v_p, o_p = s_o a_p X_p over p < length; a, k [B][T][H][dk], v, o [B][T][H][dv] by strides
+ * (elements between clips, tokens, heads of a, k, v, o: 12 values on the HOST; unit stride on the last axis); rows of o at
+ * and behind the length are zero.  log_decay g [H] <= 0; lengths [B] or NULL (all T); x0, x_end [B][H][dk][dv] fp32 or NULL
+ * (x0_transposed: x0 is [B][H][dv][dk]).  reverse != 0: last token first, x0 meets the last token undecayed and x_end gets
+ * one more decay (the gradient of the state before the first token).  1 <= dk, dv <= 128.
+ * workspace: noise_decay_attn_workspace() floats (0: may be NULL) */
+long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv);
+int noise_decay_attn_walk(const void* a, const void* k, const void* v, void* o, const long* strides, const float* log_decay,
+                          const int* lengths, const float* x0, int x0_transposed, float* x_end, float* workspace, float s_o,
+                          float s_kv, int reverse, int B, int T, int H, int dk, int dv, int dtype, void* stream);
+/* one token per clip: state [B][H][dk][dv] updated in place, o [B][H][dv]; strides: (clip, head) of q, k, v on the HOST */
+int noise_decay_attn_step(const void* q, const void* k, const void* v, const long* strides, const float* log_decay, float* state,
+                          void* o, float scale, int B, int H, int dk, int dv, int dtype, void* stream);
+
 /* ---- once-for-all spectral U-Net forward (train/layers.py:496-668): every width, kernel size and depth is a run-time
  * choice, so these kernels are shape-generic (NHWC fp32, channel counts multiples of 4 up to any width).  Convolutions
  * write their raw output plus per-workgroup partial sums of y and y*y (`slab`: noise_ofa_max_rows() rows of 2C floats,

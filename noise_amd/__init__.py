@@ -5,6 +5,7 @@ from .stft import STFT  # noqa: F401
 from .mixer import segmental_snr_mixer, activitydetector  # noqa: F401
 from .models import VADSpectralV2, VADMobileNetV2  # noqa: F401
 from .optim import FusedAdamW, MultiTensorAdamW  # noqa: F401
+from .decay_attn import decay_attention, decay_attention_bwd, decay_attention_fwd, decay_attention_step  # noqa: F401
 from .layernorm import layer_norm, layer_norm_bwd, layer_norm_fwd  # noqa: F401
 from .data import VADNoiseDataModule  # noqa: F401
 from .streaming import StreamingDenoiser  # noqa: F401

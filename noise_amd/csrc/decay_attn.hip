@@ -1,0 +1,424 @@
+// Decay attention: causal linear attention with one decay per head and a state a stream can carry,
+//   S_t = exp(g) S_{t-1} + k_t (x) v_t,   o_t = scale q_t S_t,
+// over clips in chunks, backwards, and for single tokens.
+//
+// Everything but the single token is ONE operator ("walk") on three token tensors a, k (width dk) and v (width dv),
+//   X_p = lam X_{p-1} + s_kv k_p (x) v_p,   o_p = s_o a_p X_p,
+// read in either direction of time:
+//   forward  o   (a, k, v) = (q, k, v)   first token first, X = S,    s_o = scale
+//   backward dq  (a, k, v) = (do, v, k)  first token first, X = S^T,  s_o = scale
+//            dv  (a, k, v) = (k, q, do)  last token first,  X = dS,   s_kv = scale
+//            dk  (a, k, v) = (v, do, q)  last token first,  X = dS^T, s_kv = scale
+// The gradient of the final state meets the last token without a decay (`shift`).
+//
+// Chunks of C tokens with the state X before them:
+//   o_i = s_o [ s_kv sum_{j<=i} lam^{i-j} (a_i . k_j) v_j + lam^{i+1} a_i X ],   X <- lam^C X + s_kv sum_j lam^{C-1-j} k_j (x) v_j
+// i.e. four small matrix products per chunk.  A workgroup owns one (clip, head, segment of the token axis) and walks its
+// chunks with X in registers.  Where clips and heads alone do not fill the GPU the token axis is cut into segments: one pass
+// sums each segment's own contribution to the state, a scan turns them into the state before each segment, and the walk
+// starts from those.
+#include "token.h"
+
+namespace {
+
+constexpr int DA_C = 32;   // tokens per chunk
+
+struct Strides {
+  long b, t, h;   // elements between clips, tokens and heads; the last axis has unit stride
+};
+
+struct WalkArgs {
+  const void *a, *k, *v;
+  void* o;
+  Strides sa, sk, sv, so;
+  const float* log_decay;   // [H]
+  const int* lengths;       // [B] or null: T
+  const float* x0;          // state before the first token, [B][H][dk][dv] (x0_tr: [dv][dk]) or null: zero
+  float* x_end;             // state behind the last token, [B][H][dk][dv], or null
+  float* seg;               // [B][H][nseg][dk][dv] workspace: sums of the segments, then the states before them
+  float s_o, s_kv;
+  int B, T, H, dk, dv, nseg, seg_len;
+  int reverse, shift, end_decay, x0_tr;
+  int va, vk, vv;           // rows allow 4-element accesses
+};
+
+__device__ __forceinline__ float decay_pow(float g2, int n) { return n <= 0 ? 1.f : exp2f(g2 * (float)n); }
+
+// Four elements of a token row, zero outside the row's width or behind the clip's end.
+template <typename T>
+__device__ __forceinline__ f32x4 row4(const T* base, bool live, int c, int width, bool vec) {
+  f32x4 r = {0.f, 0.f, 0.f, 0.f};
+  if (!live) return r;
+  if (vec && c + 4 <= width) {
+    float t[4];
+    load_vec<T, 4>(base + c, t);
+    r = f32x4{t[0], t[1], t[2], t[3]};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < width) r[i] = (float)base[c + i];
+  }
+  return r;
+}
+
+// fp32 arithmetic throughout (v_mfma_f32_16x16x4_f32).  P: dk and dv padded to 16, 32, 64 or 128; P / 16 waves up to four,
+// each owning 16 NT of the P state columns.  The contraction index of an MFMA may be permuted as long as both operands agree:
+// lane quarter q takes elements 4q..4q+3 of a 16-wide block over four consecutive instructions, so row-major operands are
+// 16-byte LDS reads and an accumulator tile (row 4q + r in register r) is the next product's operand as it lies: the state
+// never leaves its registers.  Only the C x C weights pass through LDS (each wave computes a share of them).
+template <typename T, int P, bool STATE_ONLY>
+__global__ __launch_bounds__(P >= 64 ? 256 : P * 4) void walk_f32_kernel(WalkArgs w) {
+  constexpr int NW = P >= 64 ? 4 : P / 16, NT = P / 16 / NW, KT = P / 16, NTHR = NW * 64;
+  constexpr int LD = P + 4, LDP = DA_C + 4, SLOTS = DA_C * P / 4 / NTHR;
+  __shared__ float sa[STATE_ONLY ? 4 : DA_C * LD];
+  __shared__ float sk[DA_C * LD], sv[DA_C * LD];
+  __shared__ float sp[STATE_ONLY ? 4 : DA_C * LDP];
+  __shared__ float pw[DA_C + 1];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, q = lane >> 4, l16 = lane & 15;
+  const int bh = blockIdx.x % (w.B * w.H), seg = blockIdx.x / (w.B * w.H);
+  const int b = bh / w.H, h = bh % w.H;
+  const int len = w.lengths ? min(max(w.lengths[b], 0), w.T) : w.T;
+  const int p0 = seg * w.seg_len, p1 = min(p0 + w.seg_len, len);
+  const int last_seg = len > 0 ? (len - 1) / w.seg_len : 0;
+  T* ob = (T*)w.o + (size_t)b * w.so.b + (size_t)h * w.so.h;
+  if (!STATE_ONLY) {
+    // rows behind the clip's end are zero
+    const int t0 = max(len, p0), t1 = min(p0 + w.seg_len, w.T);
+    for (long i = (long)tid; i < (long)(t1 - t0) * w.dv; i += NTHR) ob[(t0 + i / w.dv) * w.so.t + i % w.dv] = (T)0.f;
+  }
+  if (STATE_ONLY ? seg >= last_seg : seg > last_seg) return;
+  const float g2 = w.log_decay[h] * 1.44269504088896341f;
+  if (tid <= DA_C) pw[tid] = decay_pow(g2, tid);
+  const T* ab = (const T*)w.a + (size_t)b * w.sa.b + (size_t)h * w.sa.h;
+  const T* kb = (const T*)w.k + (size_t)b * w.sk.b + (size_t)h * w.sk.h;
+  const T* vb = (const T*)w.v + (size_t)b * w.sv.b + (size_t)h * w.sv.h;
+
+  // ---- state before the segment
+  f32x4 X[KT][NT];
+  const size_t mat = (size_t)w.dk * w.dv;
+  {
+    const bool from_seg = !STATE_ONLY && seg > 0;
+    const float* src = STATE_ONLY ? nullptr : from_seg ? w.seg + ((size_t)bh * w.nseg + seg) * mat : w.x0 ? w.x0 + (size_t)bh * mat : nullptr;
+    const int sr = !from_seg && w.x0_tr ? 1 : w.dv, sc = !from_seg && w.x0_tr ? w.dk : 1;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = kt * 16 + 4 * q + r, col = (wave * NT + nt) * 16 + l16;
+          X[kt][nt][r] = src && row < w.dk && col < w.dv ? src[(size_t)row * sr + (size_t)col * sc] : 0.f;
+        }
+  }
+
+  f32x4 ra[STATE_ONLY ? 1 : SLOTS], rk[SLOTS], rv[SLOTS];
+  auto fetch = [&](int c0) {
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      const int i = (s * NTHR + tid) / (P / 4), c = (s * NTHR + tid) % (P / 4) * 4;
+      const int p = c0 + i;
+      const bool live = p < p1;
+      const long t = live ? (w.reverse ? len - 1 - p : p) : 0;
+      if (!STATE_ONLY) ra[s] = row4(ab + t * w.sa.t, live, c, w.dk, w.va);
+      rk[s] = row4(kb + t * w.sk.t, live, c, w.dk, w.vk);
+      rv[s] = row4(vb + t * w.sv.t, live, c, w.dv, w.vv);
+    }
+  };
+  fetch(p0);
+  for (int c0 = p0; c0 < p1; c0 += DA_C) {
+    const int n = min(DA_C, p1 - c0);                       // tokens in this chunk
+    const int shift = w.shift && c0 == 0 ? 1 : 0;
+    __syncthreads();                                        // the previous chunk's readers are done
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      const int i = (s * NTHR + tid) / (P / 4), c = (s * NTHR + tid) % (P / 4) * 4;
+      if (!STATE_ONLY) *(f32x4*)(sa + i * LD + c) = ra[s];
+      *(f32x4*)(sk + i * LD + c) = rk[s];
+      *(f32x4*)(sv + i * LD + c) = rv[s];
+    }
+    __syncthreads();
+    if (c0 + DA_C < p1) fetch(c0 + DA_C);
+    f32x4 O[2][NT];
+    if (!STATE_ONLY) {
+      // ---- weights lam^{i-j} (a_i . k_j), one 16 x 16 tile per wave; the tile above the diagonal is never read
+      for (int tile = wave; tile < 4; tile += NW) {
+        const int mt = tile >> 1, jt = tile & 1;
+        if (jt > mt) continue;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          const f32x4 x = *(const f32x4*)(sa + (mt * 16 + l16) * LD + kt * 16 + 4 * q);
+          const f32x4 y = *(const f32x4*)(sk + (jt * 16 + l16) * LD + kt * 16 + 4 * q);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], y[r], acc, 0, 0, 0);
+        }
+        const float s = w.s_o * w.s_kv;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = mt * 16 + 4 * q + r, j = jt * 16 + l16;
+          sp[i * LDP + j] = i >= j ? acc[r] * (s * pw[max(i - j, 0)]) : 0.f;
+        }
+      }
+      // ---- what the state contributes
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) O[mt][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          const f32x4 x = *(const f32x4*)(sa + (mt * 16 + l16) * LD + kt * 16 + 4 * q);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) O[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], X[kt][nt][r], O[mt][nt], 0, 0, 0);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float f = w.s_o * pw[mt * 16 + 4 * q + r + 1 - shift];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) O[mt][nt][r] *= f;
+        }
+      }
+      __syncthreads();
+    }
+    // ---- this chunk's values: O += P V and X = lam^n X + K^T V'
+    const float f = pw[n - shift];
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) X[kt][nt][r] *= f;
+#pragma unroll
+    for (int jt = 0; jt < 2; ++jt) {
+      f32x4 V[NT];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) V[nt][r] = sv[(jt * 16 + 4 * q + r) * LD + (wave * NT + nt) * 16 + l16];
+      if (!STATE_ONLY) {
+#pragma unroll
+        for (int mt = jt; mt < 2; ++mt) {
+          const f32x4 x = *(const f32x4*)(sp + (mt * 16 + l16) * LDP + jt * 16 + 4 * q);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) O[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], V[nt][r], O[mt][nt], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float f = w.s_kv * pw[max(n - 1 - (jt * 16 + 4 * q + r), 0)];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) V[nt][r] *= f;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          const float x = sk[(jt * 16 + 4 * q + r) * LD + kt * 16 + l16];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) X[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, V[nt][r], X[kt][nt], 0, 0, 0);
+        }
+      }
+    }
+    if (!STATE_ONLY) {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = mt * 16 + 4 * q + r;
+          if (i >= n) continue;
+          const long t = w.reverse ? len - 1 - (c0 + i) : c0 + i;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const int col = (wave * NT + nt) * 16 + l16;
+            if (col < w.dv) ob[t * w.so.t + col] = (T)O[mt][nt][r];
+          }
+        }
+    }
+  }
+  // ---- state behind the segment
+  float* dst = STATE_ONLY ? w.seg + ((size_t)bh * w.nseg + seg) * mat : seg == last_seg && w.x_end ? w.x_end + (size_t)bh * mat : nullptr;
+  if (!dst) return;
+  const float f = !STATE_ONLY && w.end_decay && len > 0 ? pw[1] : 1.f;
+#pragma unroll
+  for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = kt * 16 + 4 * q + r, col = (wave * NT + nt) * 16 + l16;
+        if (row < w.dk && col < w.dv) dst[(size_t)row * w.dv + col] = X[kt][nt][r] * f;
+      }
+}
+
+// Sums of the segments -> states before the segments, in place: seg[s] = lam^{seg_len} seg[s-1] + sum[s-1], seg[0] = x0.  The
+// shifted first decay of a reversed walk is that of segment 0.
+__global__ __launch_bounds__(256) void walk_scan_kernel(WalkArgs w) {
+  const int mat = w.dk * w.dv;
+  const int e = blockIdx.x * 256 + threadIdx.x;
+  const int bh = blockIdx.y;
+  if (e >= mat) return;
+  const int b = bh / w.H, h = bh % w.H;
+  const int len = w.lengths ? min(max(w.lengths[b], 0), w.T) : w.T;
+  const int nseg = len > 0 ? (len - 1) / w.seg_len : 0;
+  const float g2 = w.log_decay[h] * 1.44269504088896341f;
+  const float f = decay_pow(g2, w.seg_len), f0 = w.shift ? decay_pow(g2, w.seg_len - 1) : f;
+  float x = 0.f;
+  if (w.x0) x = w.x0[(size_t)bh * mat + (w.x0_tr ? (size_t)(e % w.dv) * w.dk + e / w.dv : (size_t)e)];
+  float* p = w.seg + (size_t)bh * w.nseg * mat + e;
+  float sum = nseg > 0 ? p[0] : 0.f;
+  for (int s = 1; s <= nseg; ++s) {
+    const float next = s < nseg ? p[(size_t)s * mat] : 0.f;
+    x = x * (s == 1 ? f0 : f) + sum;
+    p[(size_t)s * mat] = x;
+    sum = next;
+  }
+}
+
+// One token per clip: the state is read and written once.  A workgroup owns one (clip, head); a thread owns four (or one)
+// neighbouring columns of every RG-th row, the row groups meet in LDS for o.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void step_kernel(const T* __restrict__ q, Strides sq, const T* __restrict__ k, Strides sk,
+                                                   const T* __restrict__ v, Strides sv, const float* __restrict__ log_decay,
+                                                   float* __restrict__ state, T* __restrict__ o, int H, int dk, int dv,
+                                                   float scale) {
+  __shared__ float red[256 * V];
+  const int b = blockIdx.x / H, h = blockIdx.x % H;
+  const int cols = (dv + V - 1) / V, groups = 256 / cols;     // dv <= 128 V
+  const int c = threadIdx.x % cols * V, grp = threadIdx.x / cols;
+  const float lam = decay_pow(log_decay[h] * 1.44269504088896341f, 1);
+  const T* qp = q + (size_t)b * sq.b + (size_t)h * sq.h;
+  const T* kp = k + (size_t)b * sk.b + (size_t)h * sk.h;
+  const T* vp = v + (size_t)b * sv.b + (size_t)h * sv.h;
+  float* sp = state + ((size_t)b * H + h) * dk * dv;
+  float acc[V], vv[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    acc[i] = 0.f;
+    vv[i] = (float)vp[c + i];
+  }
+  if (grp < groups) {
+    for (int r = grp; r < dk; r += groups) {
+      const float kr = (float)kp[r], qr = (float)qp[r];
+      float x[V];
+      load_vec<float, V>(sp + (size_t)r * dv + c, x);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        x[i] = x[i] * lam + kr * vv[i];
+        acc[i] += qr * x[i];
+      }
+      store_vec<float, V>(sp + (size_t)r * dv + c, x);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) red[threadIdx.x * V + i] = acc[i];
+  __syncthreads();
+  if (grp == 0) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      float t = 0.f;
+      for (int j = 0; j < groups; ++j) t += red[(j * cols + threadIdx.x) * V + i];
+      o[((size_t)b * H + h) * dv + c + i] = (T)(t * scale);
+    }
+  }
+}
+
+bool rows_vec4(const void* p, const Strides& s, int width, int esize) {
+  return ((uintptr_t)p % (4 * esize)) == 0 && s.b % 4 == 0 && s.t % 4 == 0 && s.h % 4 == 0 && width >= 4;
+}
+
+template <typename T>
+void walk_launch(const WalkArgs& w, hipStream_t st) {
+  const int d = w.dk > w.dv ? w.dk : w.dv;
+  const unsigned grid = (unsigned)w.B * w.H * w.nseg;
+#define GO(P, ONLY) hipLaunchKernelGGL((walk_f32_kernel<T, P, ONLY>), dim3(grid), dim3(P >= 64 ? 256 : P * 4), 0, st, w)
+#define PICK(ONLY)             \
+  do {                         \
+    if (d <= 16) GO(16, ONLY); \
+    else if (d <= 32) GO(32, ONLY); \
+    else if (d <= 64) GO(64, ONLY); \
+    else GO(128, ONLY);        \
+  } while (0)
+  if (w.nseg > 1) {
+    PICK(true);
+    hipLaunchKernelGGL(walk_scan_kernel, dim3(noise_cdiv((long)w.dk * w.dv, 256), w.B * w.H), dim3(256), 0, st, w);
+  }
+  PICK(false);
+#undef PICK
+#undef GO
+}
+
+// Segments of the token axis: as many as it takes to give every CU two workgroups, none shorter than 8 chunks (the state of a
+// segment is written, scanned and read again: dk dv values each against 4 x 8 C tokens' rows).
+int walk_segments(long bh, int T) {
+  const long want = (2L * 256 + bh - 1) / bh, most = T / (8 * DA_C);
+  const long n = want < most ? want : most;
+  return n < 1 ? 1 : (int)n;
+}
+
+const char* walk_check(int B, int T, int H, int dk, int dv, int dtype) {
+  if (B < 1 || T < 1 || H < 1) return "empty shape";
+  if (dk < 1 || dk > 128 || dv < 1 || dv > 128) return "head sizes are 1..128";
+  if ((long)B * H > (1L << 23)) return "more than 2^23 (clip, head) pairs in one call";
+  if (dtype < NOISE_F32 || dtype > NOISE_F16) return "unknown element type";
+  return nullptr;
+}
+
+}  // namespace
+
+// Floats of workspace a walk of this shape needs.
+NOISE_EXPORT long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv) {
+  if (walk_check(B, T, H, dk, dv, NOISE_F32)) return 0;
+  const int n = walk_segments((long)B * H, T);
+  return n > 1 ? (long)B * H * n * dk * dv : 0;
+}
+
+// strides: (clip, token, head) of a, k, v and o; reverse: last token first, with the undecayed first step and the decayed end
+NOISE_EXPORT int noise_decay_attn_walk(const void* a, const void* k, const void* v, void* o, const long* strides,
+                                       const float* log_decay, const int* lengths, const float* x0, int x0_transposed,
+                                       float* x_end, float* workspace, float s_o, float s_kv, int reverse, int B, int T, int H,
+                                       int dk, int dv, int dtype, void* stream) {
+  const char* why = walk_check(B, T, H, dk, dv, dtype);
+  NOISE_REQUIRE(!why, "noise_decay_attn_walk: %s (B %d, T %d, H %d, head sizes %d and %d)", why, B, T, H, dk, dv);
+  NOISE_REQUIRE(a && k && v && o && strides && log_decay, "noise_decay_attn_walk: null pointer");
+  WalkArgs w;
+  w.a = a, w.k = k, w.v = v, w.o = o;
+  w.sa = {strides[0], strides[1], strides[2]};
+  w.sk = {strides[3], strides[4], strides[5]};
+  w.sv = {strides[6], strides[7], strides[8]};
+  w.so = {strides[9], strides[10], strides[11]};
+  w.log_decay = log_decay, w.lengths = lengths, w.x0 = x0, w.x0_tr = x0_transposed, w.x_end = x_end, w.seg = workspace;
+  w.s_o = s_o, w.s_kv = s_kv;
+  w.B = B, w.T = T, w.H = H, w.dk = dk, w.dv = dv;
+  w.reverse = reverse, w.shift = reverse, w.end_decay = reverse;
+  w.nseg = walk_segments((long)B * H, T);
+  w.seg_len = (noise_cdiv(T, w.nseg) + DA_C - 1) / DA_C * DA_C;
+  w.nseg = noise_cdiv(T, w.seg_len);
+  NOISE_REQUIRE(w.nseg == 1 || workspace, "noise_decay_attn_walk: this shape needs a workspace");
+  const int es = dtype == NOISE_F32 ? 4 : 2;
+  w.va = rows_vec4(a, w.sa, dk, es), w.vk = rows_vec4(k, w.sk, dk, es), w.vv = rows_vec4(v, w.sv, dv, es);
+  hipStream_t st = (hipStream_t)stream;
+  if (dtype == NOISE_F32) walk_launch<float>(w, st);
+  else if (dtype == NOISE_BF16) walk_launch<bf16_t>(w, st);
+  else walk_launch<f16_t>(w, st);
+  NOISE_CHECK_LAUNCH("noise_decay_attn_walk");
+  return 0;
+}
+
+NOISE_EXPORT int noise_decay_attn_step(const void* q, const void* k, const void* v, const long* strides, const float* log_decay,
+                                       float* state, void* o, float scale, int B, int H, int dk, int dv, int dtype,
+                                       void* stream) {
+  NOISE_REQUIRE(q && k && v && strides && log_decay && state && o, "noise_decay_attn_step: null pointer");
+  NOISE_REQUIRE(B > 0 && H > 0 && dk > 0 && dk <= 128 && dv > 0 && dv <= 128 && (long)B * H <= (1L << 23),
+                "noise_decay_attn_step: head sizes are 1..128 and at most 2^23 (stream, head) pairs (B %d, H %d, %d and %d)", B, H, dk, dv);
+  NOISE_REQUIRE(dtype >= NOISE_F32 && dtype <= NOISE_F16, "noise_decay_attn_step: unknown element type");
+  const Strides sq = {strides[0], 0, strides[1]}, sk = {strides[2], 0, strides[3]}, sv = {strides[4], 0, strides[5]};
+  const bool vec = dv % 4 == 0 && ((uintptr_t)state & 15) == 0;
+  hipStream_t st = (hipStream_t)stream;
+#define GO(T, V) hipLaunchKernelGGL((step_kernel<T, V>), dim3(B * H), dim3(256), 0, st, (const T*)q, sq, (const T*)k, sk, (const T*)v, sv, log_decay, state, (T*)o, H, dk, dv, scale)
+  if (dtype == NOISE_F32) { if (vec) GO(float, 4); else GO(float, 1); }
+  else if (dtype == NOISE_BF16) { if (vec) GO(bf16_t, 4); else GO(bf16_t, 1); }
+  else { if (vec) GO(f16_t, 4); else GO(f16_t, 1); }
+#undef GO
+  NOISE_CHECK_LAUNCH("noise_decay_attn_step");
+  return 0;
+}

@@ -1,0 +1,171 @@
+"""Decay attention: causal linear attention with a decay for each head, on the kernels of csrc/decay_attn.hip.
+
+    S_t = exp(log_decay) S_{t-1} + k_t (x) v_t          o_t = scale * q_t S_t
+
+Next to the softmax attention of the models' bottleneck (train/models.py:14-36), which needs every token of a clip at
+once, this one carries a state of fixed size: whole clips run in chunks, a stream runs token by token from the same state.
+
+    o, state = decay_attention(q, k, v, log_decay)                            # clips; differentiable in q, k, v and state
+    o, state = decay_attention(q, k, v, log_decay, state, lengths=lengths)    # the next piece of a padded batch
+    o = decay_attention_step(q, k, v, log_decay, state)                       # one token per stream, state updated in place
+    o, end = decay_attention_fwd(...)                                         # explicit passes
+    dq, dk, dv, d_state = decay_attention_bwd(do, q, k, v, log_decay, state, lengths, d_state=d_end)
+
+q and k are (B, T, H, Dk), v is (B, T, H, Dv) with head sizes of 1 to 128, all fp32, bf16 or fp16 with any strides (views of one
+packed projection are read in place; a last axis without unit stride is copied first).  `log_decay` is (H,) fp32, at most 0
+(-inf: no memory), and takes no gradient.  States are (B, H, Dk, Dv) fp32.  `lengths` (B,) integers on the GPU: the tokens of
+clip b at and behind lengths[b] are neither read nor added to the state, their rows of o and of the gradients are zero, and the
+state returned is the one behind the last real token.  `scale` defaults to Dk ** -0.5.
+"""
+import ctypes
+
+import torch
+
+from . import _lib
+from ._lib import _F, _I, _L, _P, ptr
+
+_lib.register({
+    "noise_decay_attn_walk": [_P] * 8 + [_I, _P, _P, _F, _F] + [_I] * 7 + [_P],
+    "noise_decay_attn_step": [_P] * 7 + [_F] + [_I] * 5 + [_P],
+    "noise_decay_attn_workspace": [_I] * 5,
+})
+_lib.lib.noise_decay_attn_workspace.restype = _L
+
+MAX_HEAD = 128
+
+
+def _unit(t):
+    """t itself when its last axis has unit stride, a packed copy otherwise."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _check(q, k, v, log_decay, state, tokens):
+    _lib.require_cuda(q, k, v, log_decay, state)
+    dims = 4 if tokens else 3
+    if q.dim() != dims or k.shape != q.shape or v.dim() != dims or v.shape[:-1] != q.shape[:-1]:
+        raise ValueError(f"q, k must be {'(B, T, H, Dk)' if tokens else '(B, H, Dk)'} and v the same with Dv: got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    if q.dtype not in _lib.DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"q, k, v must share one of float32, bfloat16, float16: got {q.dtype}, {k.dtype}, {v.dtype}")
+    B, H, dk, dv = q.shape[0], q.shape[-2], q.shape[-1], v.shape[-1]
+    if not (1 <= dk <= MAX_HEAD and 1 <= dv <= MAX_HEAD):
+        raise ValueError(f"head sizes of 1 to {MAX_HEAD} are supported, got {dk} and {dv}")
+    if log_decay.shape != (H,) or log_decay.dtype != torch.float32:
+        raise ValueError(f"log_decay must be float32 ({H},), got {log_decay.dtype} {tuple(log_decay.shape)}")
+    _check_state("state", state, (B, H, dk, dv))
+    return B, H, dk, dv
+
+
+def _check_state(name, state, shape):
+    if state is not None and (tuple(state.shape) != shape or state.dtype != torch.float32):
+        raise ValueError(f"{name} must be float32 {shape}, got {state.dtype} {tuple(state.shape)}")
+
+
+def _check_lengths(lengths, B):
+    if lengths is None:
+        return None
+    _lib.require_cuda(lengths)
+    if tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"lengths must be ({B},) integers, got {lengths.dtype} {tuple(lengths.shape)}")
+    return lengths.to(torch.int32).contiguous()
+
+
+def _walk(a, k, v, log_decay, lengths, x0, x0_transposed, x_end, s_o, s_kv, reverse):
+    B, T, H, dk = a.shape
+    dv = v.shape[-1]
+    a, k, v = _unit(a), _unit(k), _unit(v)
+    o = torch.empty(B, T, H, dv, device=a.device, dtype=a.dtype)
+    n = _lib.lib.noise_decay_attn_workspace(B, T, H, dk, dv)
+    ws = torch.empty(n, device=a.device, dtype=torch.float32) if n else None
+    strides = (_L * 12)(*a.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3])
+    _lib.call("noise_decay_attn_walk", ptr(a), ptr(k), ptr(v), ptr(o), strides, ptr(log_decay), ptr(lengths), ptr(x0),
+              int(x0_transposed), ptr(x_end), ptr(ws), s_o, s_kv, int(reverse), B, T, H, dk, dv, _lib.DTYPES[a.dtype], _lib.stream(),
+              nbytes=a.element_size() * 2 * (a.numel() + v.numel()))
+    return o
+
+
+def decay_attention_fwd(q, k, v, log_decay, state=None, lengths=None, scale=None):
+    """(o, state behind the last token): o (B, T, H, Dv) in q's type, the state a new fp32 tensor."""
+    B, H, dk, dv = _check(q, k, v, log_decay, state, True)
+    lengths = _check_lengths(lengths, B)
+    scale = dk ** -0.5 if scale is None else float(scale)
+    with _lib.on_device(q, k, v, log_decay, state, lengths):
+        if q.numel() == 0:      # no token: the state as it was
+            end = torch.zeros(B, H, dk, dv, device=q.device) if state is None else state.clone()
+            return torch.empty(v.shape, device=v.device, dtype=v.dtype), end
+        end = torch.empty(B, H, dk, dv, device=q.device, dtype=torch.float32)
+        x0 = state.contiguous() if state is not None else None
+        o = _walk(q, k, v, log_decay.contiguous(), lengths, x0, False, end, scale, 1.0, False)
+        return o, end
+
+
+def decay_attention_bwd(do, q, k, v, log_decay, state=None, lengths=None, scale=None, d_state=None):
+    """(dq, dk, dv, gradient of `state`) for the gradients `do` of o and `d_state` of the returned state (None: zero)."""
+    B, H, dk, dv = _check(q, k, v, log_decay, state, True)
+    lengths = _check_lengths(lengths, B)
+    _lib.require_cuda(do, d_state)
+    if do.shape != v.shape or do.dtype != v.dtype:
+        raise ValueError(f"do must be {tuple(v.shape)} in {v.dtype}, got {tuple(do.shape)} in {do.dtype}")
+    _check_state("d_state", d_state, (B, H, dk, dv))
+    scale = dk ** -0.5 if scale is None else float(scale)
+    with _lib.on_device(q, do, k, v, log_decay, state, lengths, d_state):
+        d0 = torch.empty(B, H, dk, dv, device=q.device, dtype=torch.float32)
+        if q.numel() == 0:
+            d0.copy_(d_state) if d_state is not None else d0.zero_()
+            return torch.empty_like(q), torch.empty_like(k), torch.empty_like(v), d0
+        g = log_decay.contiguous()
+        x0 = state.contiguous() if state is not None else None
+        x1 = d_state.contiguous() if d_state is not None else None
+        do = _unit(do)
+        dq = _walk(do, v, k, g, lengths, x0, True, None, scale, 1.0, False)
+        dvv = _walk(k, q, do, g, lengths, x1, False, d0, 1.0, scale, True)
+        dkk = _walk(v, do, q, g, lengths, x1, True, None, 1.0, scale, True)
+        return dq, dkk, dvv, d0
+
+
+class _DecayAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state, lengths, scale):
+        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
+        ctx.scale = scale
+        return decay_attention_fwd(q, k, v, log_decay, state, lengths, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, d_end):
+        q, k, v, log_decay, state, lengths = ctx.saved_tensors
+        dq, dk, dv, d_state = decay_attention_bwd(do, q, k, v, log_decay, state, lengths, ctx.scale, d_end)
+        return dq, dk, dv, None, d_state if state is not None else None, None, None
+
+
+def decay_attention(q, k, v, log_decay, state=None, lengths=None, scale=None):
+    """(o, state behind the last token); back-propagates into q, k, v and state."""
+    if log_decay.requires_grad:
+        raise ValueError("log_decay takes no gradient: detach it")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
+        return _DecayAttention.apply(q, k, v, log_decay, state, lengths, scale)
+    return decay_attention_fwd(q, k, v, log_decay, state, lengths, scale)
+
+
+def decay_attention_step(q, k, v, log_decay, state, scale=None, out=None):
+    """One token per stream: q, k (B, H, Dk), v (B, H, Dv); `state` (B, H, Dk, Dv) fp32, packed, is updated in place.  Returns
+    o (B, H, Dv) (`out` when given).  No gradient."""
+    if state is None:
+        raise ValueError("decay_attention_step needs the streams' state")
+    B, H, dk, dv = _check(q, k, v, log_decay, state, False)
+    if not state.is_contiguous():
+        raise ValueError("state must be packed: it is updated in place")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
+        raise RuntimeError("decay_attention_step has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if out is None:
+        out = torch.empty(B, H, dv, device=q.device, dtype=q.dtype)
+    elif tuple(out.shape) != (B, H, dv) or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError(f"out must be a packed {q.dtype} {(B, H, dv)}, got {out.dtype} {tuple(out.shape)}")
+    scale = dk ** -0.5 if scale is None else float(scale)
+    with _lib.on_device(q, k, v, log_decay, state, out):
+        if B * H:
+            q, k, v = _unit(q), _unit(k), _unit(v)
+            strides = (_L * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
+            _lib.call("noise_decay_attn_step", ptr(q), ptr(k), ptr(v), strides, ptr(log_decay.contiguous()), ptr(state), ptr(out),
+                      scale, B, H, dk, dv, _lib.DTYPES[q.dtype], _lib.stream(), nbytes=8 * state.numel())
+    return out
