@@ -39,7 +39,7 @@ struct WalkArgs {
   float s_o, s_kv;
   int B, T, H, dk, dv, nseg, seg_len;
   int reverse, shift, end_decay, x0_tr;
-  int va, vk, vv;           // rows allow 4-element accesses
+  int va, vk, vv, vo;       // rows allow 16-byte accesses (fp32 arithmetic: 4-element ones)
 };
 
 __device__ __forceinline__ float decay_pow(float g2, int n) { return n <= 0 ? 1.f : exp2f(g2 * (float)n); }
@@ -250,6 +250,256 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4) void walk_f32_kernel(WalkArg
       }
 }
 
+// bf16 tokens on the bf16 matrix cores (v_mfma_f32_16x16x32_bf16), 64 tokens per chunk, P / 32 waves that own 32 state
+// columns each.  What is rounded to bf16 on its way into a product, and what is not:
+//   * the weights lam^{i-j} (a_i . k_j) and the state as it meets a_i: once each, like the output they lead to;
+//   * lam^{n-1-j} v_j on its way into the state is split into three bf16 terms (24 bits), since the state is fp32, carried
+//     over any number of chunks and returned: X keeps fp32 accuracy at three products per term.
+// Operands: lane (q = lane / 16, l = lane % 16) of an MFMA takes eight contraction indices 8q..8q+7 of row l, and an
+// accumulator tile holds rows 4q + r of column l.  Two state tiles whose rows are dealt as 8q + 4s + r (s = tile) together
+// are the eight indices the next product wants, so the state stays in registers; the same deal on the columns makes a lane's
+// outputs eight neighbours (one 16-byte store).  Contractions over tokens read K and V through ds_read_b64_tr_b16, which
+// hands a lane four tokens of one column.  Rows are padded by 32 bytes: a transposing read of four rows then touches every
+// bank once.
+constexpr int DB_C = 64;
+
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using bf16x4 = __attribute__((ext_vector_type(4))) __bf16;
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
+
+__device__ __forceinline__ u32x4 row8(const bf16_t* base, bool live, int c, int width, bool vec) {
+  u32x4 r = {0u, 0u, 0u, 0u};
+  if (!live) return r;
+  if (vec && c + 8 <= width) return *reinterpret_cast<const u32x4*>(base + c);
+  bf16x8 t;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = c + i < width ? base[c + i] : (bf16_t)0.f;
+  return __builtin_bit_cast(u32x4, t);
+}
+
+// Eight tokens (rows row0 + 8q .. + 7) of the column that lane l stands for when tile columns are dealt as 8 (l / 4) + l % 4:
+// `tile` points at (row0, first column + 4 * tile number).
+template <int LD>
+__device__ __forceinline__ bf16x8 read_tokens(const bf16_t* tile, int q, int l16) {
+  using lds4 = __attribute__((address_space(3))) s16x4;
+  const bf16_t* p = tile + (8 * q + l16 / 4) * LD + l16 % 4 * 8;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * LD));
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+template <int P, bool STATE_ONLY>
+__global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
+  constexpr int NTHR = P * 2, NW = P / 32, KP = P / 32;      // KP: pairs of state row tiles
+  constexpr int LD = P + 16, LDP = DB_C + 8, SLOTS = DB_C * P / 8 / NTHR;
+  __shared__ __attribute__((aligned(16))) bf16_t sa[STATE_ONLY ? 8 : DB_C * LD];
+  __shared__ __attribute__((aligned(16))) bf16_t sk[DB_C * LD], sv[DB_C * LD];
+  __shared__ __attribute__((aligned(16))) bf16_t sp[STATE_ONLY ? 8 : DB_C * LDP];
+  __shared__ float pw[DB_C + 1];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, q = lane >> 4, l16 = lane & 15;
+  const int bh = blockIdx.x % (w.B * w.H), seg = blockIdx.x / (w.B * w.H);
+  const int b = bh / w.H, h = bh % w.H;
+  const int len = w.lengths ? min(max(w.lengths[b], 0), w.T) : w.T;
+  const int p0 = seg * w.seg_len, p1 = min(p0 + w.seg_len, len);
+  const int last_seg = len > 0 ? (len - 1) / w.seg_len : 0;
+  bf16_t* ob = (bf16_t*)w.o + (size_t)b * w.so.b + (size_t)h * w.so.h;
+  if (!STATE_ONLY) {
+    // rows behind the clip's end are zero
+    const int t0 = max(len, p0), t1 = min(p0 + w.seg_len, w.T);
+    for (long i = (long)tid; i < (long)(t1 - t0) * w.dv; i += NTHR) ob[(t0 + i / w.dv) * w.so.t + i % w.dv] = (bf16_t)0.f;
+  }
+  if (STATE_ONLY ? seg >= last_seg : seg > last_seg) return;
+  const float g2 = w.log_decay[h] * 1.44269504088896341f;
+  for (int i = tid; i <= DB_C; i += NTHR) pw[i] = decay_pow(g2, i);
+  const bf16_t* ab = (const bf16_t*)w.a + (size_t)b * w.sa.b + (size_t)h * w.sa.h;
+  const bf16_t* kb = (const bf16_t*)w.k + (size_t)b * w.sk.b + (size_t)h * w.sk.h;
+  const bf16_t* vb = (const bf16_t*)w.v + (size_t)b * w.sv.b + (size_t)h * w.sv.h;
+  const int col0 = wave * 32;                                // the wave's state columns
+
+  // X[kp][s][nt][r]: row kp 32 + 8q + 4s + r, column col0 + 8 (l / 4) + 4 nt + l % 4
+  f32x4 X[KP][2][2];
+  const size_t mat = (size_t)w.dk * w.dv;
+  const int xcol = col0 + 8 * (l16 >> 2) + (l16 & 3);
+  {
+    const bool from_seg = !STATE_ONLY && seg > 0;
+    const float* src = STATE_ONLY ? nullptr : from_seg ? w.seg + ((size_t)bh * w.nseg + seg) * mat : w.x0 ? w.x0 + (size_t)bh * mat : nullptr;
+    const int sr = !from_seg && w.x0_tr ? 1 : w.dv, sc = !from_seg && w.x0_tr ? w.dk : 1;
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = kp * 32 + 8 * q + 4 * s + r, col = xcol + 4 * nt;
+            X[kp][s][nt][r] = src && row < w.dk && col < w.dv ? src[(size_t)row * sr + (size_t)col * sc] : 0.f;
+          }
+  }
+
+  u32x4 ra[STATE_ONLY ? 1 : SLOTS], rk[SLOTS], rv[SLOTS];
+  auto fetch = [&](int c0) {
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      const int i = (s * NTHR + tid) / (P / 8), c = (s * NTHR + tid) % (P / 8) * 8;
+      const int p = c0 + i;
+      const bool live = p < p1;
+      const long t = live ? (w.reverse ? len - 1 - p : p) : 0;
+      if (!STATE_ONLY) ra[s] = row8(ab + t * w.sa.t, live, c, w.dk, w.va);
+      rk[s] = row8(kb + t * w.sk.t, live, c, w.dk, w.vk);
+      rv[s] = row8(vb + t * w.sv.t, live, c, w.dv, w.vv);
+    }
+  };
+  fetch(p0);
+  for (int c0 = p0; c0 < p1; c0 += DB_C) {
+    const int n = min(DB_C, p1 - c0);                       // tokens in this chunk
+    const int shift = w.shift && c0 == 0 ? 1 : 0;
+    __syncthreads();                                        // the previous chunk's readers are done
+#pragma unroll
+    for (int s = 0; s < SLOTS; ++s) {
+      const int i = (s * NTHR + tid) / (P / 8), c = (s * NTHR + tid) % (P / 8) * 8;
+      if (!STATE_ONLY) *(u32x4*)(sa + i * LD + c) = ra[s];
+      *(u32x4*)(sk + i * LD + c) = rk[s];
+      *(u32x4*)(sv + i * LD + c) = rv[s];
+    }
+    __syncthreads();
+    if (c0 + DB_C < p1) fetch(c0 + DB_C);
+    f32x4 O[STATE_ONLY ? 1 : 4][2];
+    if (!STATE_ONLY) {
+      // ---- weights, transposed tile by tile (rows j, columns i) so that a lane holds four neighbouring j of one i: the ten
+      // 16 x 16 tiles on and below the diagonal are dealt over the waves; the other tiles of a pair of 16 that is read are zero
+      for (int tile = wave; tile < 12; tile += NW) {
+        // 0..9: (it, jt) with jt <= it in order; 10, 11: the zero tiles (0, 1) and (2, 3)
+        const int it = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : tile < 10 ? 3 : tile == 10 ? 0 : 2;
+        const int jt = tile < 10 ? tile - it * (it + 1) / 2 : it + 1;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        if (tile < 10) {
+#pragma unroll
+          for (int kp = 0; kp < KP; ++kp) {
+            const bf16x8 x = *(const bf16x8*)(sk + (jt * 16 + l16) * LD + kp * 32 + 8 * q);
+            const bf16x8 y = *(const bf16x8*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
+            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0);
+          }
+        }
+        const float s = w.s_o * w.s_kv;
+        const int i = it * 16 + l16, j = jt * 16 + 4 * q;
+        bf16x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = (bf16_t)(i >= j + r ? acc[r] * (s * pw[max(i - j - r, 0)]) : 0.f);
+        *(bf16x4*)(sp + i * LDP + j) = v;
+      }
+      // ---- what the state contributes, transposed: rows are the wave's columns, columns the tokens
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) O[it][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kp = 0; kp < KP; ++kp) {
+        bf16x8 x[2];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[nt][e] = (bf16_t)X[kp][e >> 2][nt][e & 3];
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const bf16x8 y = *(const bf16x8*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) O[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[nt], y, O[it][nt], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const float f = w.s_o * pw[it * 16 + l16 + 1 - shift];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) O[it][nt] *= f;
+      }
+      __syncthreads();
+    }
+    // ---- this chunk's values: O += P V and X = lam^n X + K^T V'
+    const float f = pw[n - shift];
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) X[kp][s][nt] *= f;
+#pragma unroll
+    for (int jj = 0; jj < 2; ++jj) {
+      bf16x8 v[2];
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) v[nt] = read_tokens<LD>(sv + jj * 32 * LD + col0 + 4 * nt, q, l16);
+      if (!STATE_ONLY) {
+#pragma unroll
+        for (int it = 2 * jj; it < 4; ++it) {
+          const bf16x8 y = *(const bf16x8*)(sp + (it * 16 + l16) * LDP + jj * 32 + 8 * q);
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) O[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[nt], y, O[it][nt], 0, 0, 0);
+        }
+      }
+      bf16x8 t[2][3];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float f = w.s_kv * pw[max(n - 1 - (jj * 32 + 8 * q + e), 0)];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+          float y = (float)v[nt][e] * f;
+#pragma unroll
+          for (int u = 0; u < 3; ++u) {
+            t[nt][u][e] = (bf16_t)y;
+            y -= (float)t[nt][u][e];
+          }
+        }
+      }
+#pragma unroll
+      for (int kp = 0; kp < KP; ++kp)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const bf16x8 x = read_tokens<LD>(sk + jj * 32 * LD + kp * 32 + 4 * s, q, l16);
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+            for (int u = 2; u >= 0; --u) X[kp][s][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, t[nt][u], X[kp][s][nt], 0, 0, 0);
+        }
+    }
+    if (!STATE_ONLY) {
+#pragma unroll
+      for (int it = 0; it < 4; ++it) {
+        const int i = it * 16 + l16;
+        if (i >= n) continue;
+        const long t = w.reverse ? len - 1 - (c0 + i) : c0 + i;
+        const int col = col0 + 8 * q;
+        bf16_t* op = ob + t * w.so.t + col;
+        bf16x8 y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = (bf16_t)O[it][e >> 2][e & 3];
+        if (w.vo && col + 8 <= w.dv) {
+          *(bf16x8*)op = y;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (col + e < w.dv) op[e] = y[e];
+        }
+      }
+    }
+  }
+  // ---- state behind the segment
+  float* dst = STATE_ONLY ? w.seg + ((size_t)bh * w.nseg + seg) * mat : seg == last_seg && w.x_end ? w.x_end + (size_t)bh * mat : nullptr;
+  if (!dst) return;
+  const float f = !STATE_ONLY && w.end_decay && len > 0 ? pw[1] : 1.f;
+#pragma unroll
+  for (int kp = 0; kp < KP; ++kp)
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = kp * 32 + 8 * q + 4 * s + r, col = xcol + 4 * nt;
+          if (row < w.dk && col < w.dv) dst[(size_t)row * w.dv + col] = X[kp][s][nt][r] * f;
+        }
+}
+
 // Sums of the segments -> states before the segments, in place: seg[s] = lam^{seg_len} seg[s-1] + sum[s-1], seg[0] = x0.  The
 // shifted first decay of a reversed walk is that of segment 0.
 __global__ __launch_bounds__(256) void walk_scan_kernel(WalkArgs w) {
@@ -322,8 +572,32 @@ __global__ __launch_bounds__(256) void step_kernel(const T* __restrict__ q, Stri
   }
 }
 
-bool rows_vec4(const void* p, const Strides& s, int width, int esize) {
-  return ((uintptr_t)p % (4 * esize)) == 0 && s.b % 4 == 0 && s.t % 4 == 0 && s.h % 4 == 0 && width >= 4;
+// Whether `v` neighbouring elements of a row may be accessed as one.
+bool rows_vec(const void* p, const Strides& s, int v, int esize) {
+  return ((uintptr_t)p % (v * esize)) == 0 && s.b % v == 0 && s.t % v == 0 && s.h % v == 0;
+}
+
+void scan_launch(const WalkArgs& w, hipStream_t st) {
+  hipLaunchKernelGGL(walk_scan_kernel, dim3(noise_cdiv((long)w.dk * w.dv, 256), w.B * w.H), dim3(256), 0, st, w);
+}
+
+void walk_launch_bf16(const WalkArgs& w, hipStream_t st) {
+  const int d = w.dk > w.dv ? w.dk : w.dv;
+  const unsigned grid = (unsigned)w.B * w.H * w.nseg;
+#define GO(P, ONLY) hipLaunchKernelGGL((walk_bf16_kernel<P, ONLY>), dim3(grid), dim3(P * 2), 0, st, w)
+#define PICK(ONLY)             \
+  do {                         \
+    if (d <= 32) GO(32, ONLY); \
+    else if (d <= 64) GO(64, ONLY); \
+    else GO(128, ONLY);        \
+  } while (0)
+  if (w.nseg > 1) {
+    PICK(true);
+    scan_launch(w, st);
+  }
+  PICK(false);
+#undef PICK
+#undef GO
 }
 
 template <typename T>
@@ -340,17 +614,17 @@ void walk_launch(const WalkArgs& w, hipStream_t st) {
   } while (0)
   if (w.nseg > 1) {
     PICK(true);
-    hipLaunchKernelGGL(walk_scan_kernel, dim3(noise_cdiv((long)w.dk * w.dv, 256), w.B * w.H), dim3(256), 0, st, w);
+    scan_launch(w, st);
   }
   PICK(false);
 #undef PICK
 #undef GO
 }
 
-// Segments of the token axis: as many as it takes to give every CU two workgroups, none shorter than 8 chunks (the state of a
-// segment is written, scanned and read again: dk dv values each against 4 x 8 C tokens' rows).
+// Segments of the token axis: as many as it takes to give every CU two workgroups, none shorter than 256 tokens (the state of a
+// segment is written, scanned and read again: dk dv values each against 256 tokens' rows).
 int walk_segments(long bh, int T) {
-  const long want = (2L * 256 + bh - 1) / bh, most = T / (8 * DA_C);
+  const long want = (2L * 256 + bh - 1) / bh, most = T / (4 * DB_C);
   const long n = want < most ? want : most;
   return n < 1 ? 1 : (int)n;
 }
@@ -391,14 +665,14 @@ NOISE_EXPORT int noise_decay_attn_walk(const void* a, const void* k, const void*
   w.B = B, w.T = T, w.H = H, w.dk = dk, w.dv = dv;
   w.reverse = reverse, w.shift = reverse, w.end_decay = reverse;
   w.nseg = walk_segments((long)B * H, T);
-  w.seg_len = (noise_cdiv(T, w.nseg) + DA_C - 1) / DA_C * DA_C;
+  w.seg_len = (noise_cdiv(T, w.nseg) + DB_C - 1) / DB_C * DB_C;
   w.nseg = noise_cdiv(T, w.seg_len);
   NOISE_REQUIRE(w.nseg == 1 || workspace, "noise_decay_attn_walk: this shape needs a workspace");
-  const int es = dtype == NOISE_F32 ? 4 : 2;
-  w.va = rows_vec4(a, w.sa, dk, es), w.vk = rows_vec4(k, w.sk, dk, es), w.vv = rows_vec4(v, w.sv, dv, es);
+  const int es = dtype == NOISE_F32 ? 4 : 2, nv = dtype == NOISE_BF16 ? 8 : 4;
+  w.va = rows_vec(a, w.sa, nv, es), w.vk = rows_vec(k, w.sk, nv, es), w.vv = rows_vec(v, w.sv, nv, es), w.vo = rows_vec(o, w.so, nv, es);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == NOISE_F32) walk_launch<float>(w, st);
-  else if (dtype == NOISE_BF16) walk_launch<bf16_t>(w, st);
+  else if (dtype == NOISE_BF16) walk_launch_bf16(w, st);
   else walk_launch<f16_t>(w, st);
   NOISE_CHECK_LAUNCH("noise_decay_attn_walk");
   return 0;
