@@ -39,7 +39,7 @@ struct WalkArgs {
   float s_o, s_kv;
   int B, T, H, dk, dv, nseg, seg_len;
   int reverse, shift, end_decay, x0_tr;
-  int va, vk, vv, vo;       // rows allow 16-byte accesses (fp32 arithmetic: 4-element ones)
+  int va, vk, vv, vo;       // rows allow wide accesses: rows_buffer for bf16, four elements at a time otherwise
 };
 
 __device__ __forceinline__ float decay_pow(float g2, int n) { return n <= 0 ? 1.f : exp2f(g2 * (float)n); }
@@ -289,14 +289,32 @@ __device__ __forceinline__ bf16x8 read_tokens(const bf16_t* tile, int q, int l16
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-template <int P, bool STATE_ONLY>
+__device__ __forceinline__ float low_bf16(unsigned u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high_bf16(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
+  const __attribute__((ext_vector_type(2))) __bf16 v = {(bf16_t)a, (bf16_t)b};
+  return __builtin_bit_cast(unsigned, v);
+}
+
+// Rows of a chunk as a buffer: accesses behind its end read zero and store nothing, so that neither the clip's last chunk nor
+// columns behind the head need a branch.  `rows` of them, `stride` elements apart, `width` elements each.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_rows(const bf16_t* first, int rows, long stride, int width) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)first, 0, (int)(((rows - 1) * stride + width) * 2), 0x00020000);
+}
+// A byte offset into such a buffer; one before its start, or of a column that does not exist, lands far behind its end.
+__device__ __forceinline__ int chunk_offset(int off, bool exists) { return (int)min((unsigned)(exists ? off : -1), 0x80000000u); }
+
+// VEC: every row of a, k, v and o starts on a 16-byte boundary, rows do not overlap and a chunk spans less than 2 GB.
+template <int P, bool STATE_ONLY, bool VEC>
 __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
   constexpr int NTHR = P * 2, NW = P / 32, KP = P / 32;      // KP: pairs of state row tiles
   constexpr int LD = P + 16, LDP = DB_C + 8, SLOTS = DB_C * P / 8 / NTHR;
   __shared__ __attribute__((aligned(16))) bf16_t sa[STATE_ONLY ? 8 : DB_C * LD];
   __shared__ __attribute__((aligned(16))) bf16_t sk[DB_C * LD], sv[DB_C * LD];
   __shared__ __attribute__((aligned(16))) bf16_t sp[STATE_ONLY ? 8 : DB_C * LDP];
-  __shared__ float pw[DB_C + 1];
+  __shared__ float pw[DB_C + 1];                             // lam^i
+  __shared__ float pv[2 * DB_C];                             // s_kv lam^{63-i}; a chunk of n tokens starts at 64 - n
+  __shared__ float pp[DB_C + 16];                            // [15 + i - j]: s_o s_kv lam^{i-j}
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, q = lane >> 4, l16 = lane & 15;
   const int bh = blockIdx.x % (w.B * w.H), seg = blockIdx.x / (w.B * w.H);
   const int b = bh / w.H, h = bh % w.H;
@@ -311,7 +329,11 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
   }
   if (STATE_ONLY ? seg >= last_seg : seg > last_seg) return;
   const float g2 = w.log_decay[h] * 1.44269504088896341f;
-  for (int i = tid; i <= DB_C; i += NTHR) pw[i] = decay_pow(g2, i);
+  for (int i = tid; i < 2 * DB_C; i += NTHR) {
+    if (i <= DB_C) pw[i] = decay_pow(g2, i);
+    if (i < DB_C + 16) pp[i] = w.s_o * w.s_kv * decay_pow(g2, i - 15);
+    pv[i] = w.s_kv * decay_pow(g2, DB_C - 1 - i);
+  }
   const bf16_t* ab = (const bf16_t*)w.a + (size_t)b * w.sa.b + (size_t)h * w.sa.h;
   const bf16_t* kb = (const bf16_t*)w.k + (size_t)b * w.sk.b + (size_t)h * w.sk.h;
   const bf16_t* vb = (const bf16_t*)w.v + (size_t)b * w.sv.b + (size_t)h * w.sv.h;
@@ -338,30 +360,45 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
           }
   }
 
+  // a thread's SLOTS pieces of a tile are RS rows apart, in the same column
+  constexpr int RS = NTHR / (P / 8);
+  const int i0 = tid / (P / 8), cc = tid % (P / 8) * 8;
+  const int dir = w.reverse ? -1 : 1;
   u32x4 ra[STATE_ONLY ? 1 : SLOTS], rk[SLOTS], rv[SLOTS];
-  auto fetch = [&](int c0) {
+  auto rows8 = [&](const bf16_t* base, const Strides& st, int width, bool vec, int c0, u32x4 (&out)[SLOTS]) {
+    const int n = min(DB_C, p1 - c0);
+    if (VEC) {
+      const auto rs = chunk_rows(base + (w.reverse ? len - c0 - n : c0) * st.t, n, st.t, width);
+      const int step = dir * RS * 2 * (int)st.t;
+      int off = (w.reverse ? n - 1 - i0 : i0) * 2 * (int)st.t + 2 * cc;
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s) {
-      const int i = (s * NTHR + tid) / (P / 8), c = (s * NTHR + tid) % (P / 8) * 8;
-      const int p = c0 + i;
-      const bool live = p < p1;
-      const long t = live ? (w.reverse ? len - 1 - p : p) : 0;
-      if (!STATE_ONLY) ra[s] = row8(ab + t * w.sa.t, live, c, w.dk, w.va);
-      rk[s] = row8(kb + t * w.sk.t, live, c, w.dk, w.vk);
-      rv[s] = row8(vb + t * w.sv.t, live, c, w.dv, w.vv);
+      for (int s = 0; s < SLOTS; ++s, off += step)
+        out[s] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, chunk_offset(off, cc < width), 0, 0));
+    } else {
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s) {
+        const int p = c0 + i0 + s * RS;
+        const bool live = p < p1;
+        out[s] = row8(base + (live ? (w.reverse ? len - 1 - p : p) : 0) * st.t, live, cc, width, vec);
+      }
     }
   };
-  fetch(p0);
+  auto fetch = [&](int c0) {
+    if constexpr (!STATE_ONLY) rows8(ab, w.sa, w.dk, w.va, c0, ra);
+    rows8(kb, w.sk, w.dk, w.vk, c0, rk);
+    rows8(vb, w.sv, w.dv, w.vv, c0, rv);
+  };
+  if (p0 < p1) fetch(p0);
   for (int c0 = p0; c0 < p1; c0 += DB_C) {
     const int n = min(DB_C, p1 - c0);                       // tokens in this chunk
     const int shift = w.shift && c0 == 0 ? 1 : 0;
     __syncthreads();                                        // the previous chunk's readers are done
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-      const int i = (s * NTHR + tid) / (P / 8), c = (s * NTHR + tid) % (P / 8) * 8;
-      if (!STATE_ONLY) *(u32x4*)(sa + i * LD + c) = ra[s];
-      *(u32x4*)(sk + i * LD + c) = rk[s];
-      *(u32x4*)(sv + i * LD + c) = rv[s];
+      const int at = (i0 + s * RS) * LD + cc;
+      if (!STATE_ONLY) *(u32x4*)(sa + at) = ra[s];
+      *(u32x4*)(sk + at) = rk[s];
+      *(u32x4*)(sv + at) = rv[s];
     }
     __syncthreads();
     if (c0 + DB_C < p1) fetch(c0 + DB_C);
@@ -382,12 +419,15 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
             acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0);
           }
         }
-        const float s = w.s_o * w.s_kv;
         const int i = it * 16 + l16, j = jt * 16 + 4 * q;
-        bf16x4 v;
+        if (it == jt) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = (bf16_t)(i >= j + r ? acc[r] * (s * pw[max(i - j - r, 0)]) : 0.f);
-        *(bf16x4*)(sp + i * LDP + j) = v;
+          for (int r = 0; r < 4; ++r) acc[r] = l16 >= 4 * q + r ? acc[r] * pp[15 + i - j - r] : 0.f;
+        } else if (tile < 10) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[r] *= pp[15 + i - j - r];
+        }
+        *(uint2*)(sp + i * LDP + j) = make_uint2(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]));
       }
       // ---- what the state contributes, transposed: rows are the wave's columns, columns the tokens
 #pragma unroll
@@ -398,9 +438,12 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
       for (int kp = 0; kp < KP; ++kp) {
         bf16x8 x[2];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int nt = 0; nt < 2; ++nt) {
+          u32x4 u;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[nt][e] = (bf16_t)X[kp][e >> 2][nt][e & 3];
+          for (int e = 0; e < 4; ++e) u[e] = pack_bf16(X[kp][e >> 1][nt][2 * (e & 1)], X[kp][e >> 1][nt][2 * (e & 1) + 1]);
+          x[nt] = __builtin_bit_cast(bf16x8, u);
+        }
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
           const bf16x8 y = *(const bf16x8*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
@@ -437,17 +480,21 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
           for (int nt = 0; nt < 2; ++nt) O[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[nt], y, O[it][nt], 0, 0, 0);
         }
       }
-      bf16x8 t[2][3];
+      u32x4 t[2][3];
+      const float* f8 = pv + DB_C - n + jj * 32 + 8 * q;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float f = w.s_kv * pw[max(n - 1 - (jj * 32 + 8 * q + e), 0)];
+      for (int e = 0; e < 4; ++e) {
+        const float f0 = f8[2 * e], f1 = f8[2 * e + 1];
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt) {
-          float y = (float)v[nt][e] * f;
+          const unsigned u = __builtin_bit_cast(u32x4, v[nt])[e];
+          float y0 = low_bf16(u) * f0, y1 = high_bf16(u) * f1;
 #pragma unroll
-          for (int u = 0; u < 3; ++u) {
-            t[nt][u][e] = (bf16_t)y;
-            y -= (float)t[nt][u][e];
+          for (int z = 0; z < 3; ++z) {
+            const unsigned c = pack_bf16(y0, y1);
+            t[nt][z][e] = c;
+            y0 -= low_bf16(c);
+            y1 -= high_bf16(c);
           }
         }
       }
@@ -459,26 +506,28 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
-            for (int u = 2; u >= 0; --u) X[kp][s][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, t[nt][u], X[kp][s][nt], 0, 0, 0);
+            for (int z = 2; z >= 0; --z)
+              X[kp][s][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, t[nt][z]), X[kp][s][nt], 0, 0, 0);
         }
     }
     if (!STATE_ONLY) {
+      const int col = col0 + 8 * q;
+      const auto rs = chunk_rows(ob + (w.reverse ? len - c0 - n : c0) * w.so.t, n, w.so.t, w.dv);
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
         const int i = it * 16 + l16;
-        if (i >= n) continue;
-        const long t = w.reverse ? len - 1 - (c0 + i) : c0 + i;
-        const int col = col0 + 8 * q;
-        bf16_t* op = ob + t * w.so.t + col;
-        bf16x8 y;
+        u32x4 y;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = (bf16_t)O[it][e >> 2][e & 3];
-        if (w.vo && col + 8 <= w.dv) {
-          *(bf16x8*)op = y;
-        } else {
+        for (int e = 0; e < 4; ++e) y[e] = pack_bf16(O[it][e >> 1][2 * (e & 1)], O[it][e >> 1][2 * (e & 1) + 1]);
+        const int row = w.reverse ? n - 1 - i : i;
+        if (VEC) {
+          __builtin_amdgcn_raw_buffer_store_b128(y, rs, chunk_offset(row * 2 * (int)w.so.t + 2 * col, col < w.dv), 0, 0);
+        } else if (i < n) {
+          bf16_t* op = ob + ((w.reverse ? len - c0 - n : c0) + row) * w.so.t + col;
+          const bf16x8 z = __builtin_bit_cast(bf16x8, y);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (col + e < w.dv) op[e] = y[e];
+            if (col + e < w.dv) op[e] = z[e];
         }
       }
     }
@@ -576,6 +625,10 @@ __global__ __launch_bounds__(256) void step_kernel(const T* __restrict__ q, Stri
 bool rows_vec(const void* p, const Strides& s, int v, int esize) {
   return ((uintptr_t)p % (v * esize)) == 0 && s.b % v == 0 && s.t % v == 0 && s.h % v == 0;
 }
+// ... and as a piece of a chunk's buffer (bf16 kernels): whole pieces, rows apart, offsets below 2^31 bytes.
+bool rows_buffer(const void* p, const Strides& s, int width) {
+  return rows_vec(p, s, 8, 2) && width % 8 == 0 && s.t >= width && s.t < (1L << 23);
+}
 
 void scan_launch(const WalkArgs& w, hipStream_t st) {
   hipLaunchKernelGGL(walk_scan_kernel, dim3(noise_cdiv((long)w.dk * w.dv, 256), w.B * w.H), dim3(256), 0, st, w);
@@ -584,7 +637,12 @@ void scan_launch(const WalkArgs& w, hipStream_t st) {
 void walk_launch_bf16(const WalkArgs& w, hipStream_t st) {
   const int d = w.dk > w.dv ? w.dk : w.dv;
   const unsigned grid = (unsigned)w.B * w.H * w.nseg;
-#define GO(P, ONLY) hipLaunchKernelGGL((walk_bf16_kernel<P, ONLY>), dim3(grid), dim3(P * 2), 0, st, w)
+  const bool vec = w.va && w.vk && w.vv && w.vo;
+#define GO(P, ONLY)                                                                                        \
+  do {                                                                                                     \
+    if (vec) hipLaunchKernelGGL((walk_bf16_kernel<P, ONLY, true>), dim3(grid), dim3(P * 2), 0, st, w);     \
+    else hipLaunchKernelGGL((walk_bf16_kernel<P, ONLY, false>), dim3(grid), dim3(P * 2), 0, st, w);        \
+  } while (0)
 #define PICK(ONLY)             \
   do {                         \
     if (d <= 32) GO(32, ONLY); \
@@ -668,8 +726,12 @@ NOISE_EXPORT int noise_decay_attn_walk(const void* a, const void* k, const void*
   w.seg_len = (noise_cdiv(T, w.nseg) + DB_C - 1) / DB_C * DB_C;
   w.nseg = noise_cdiv(T, w.seg_len);
   NOISE_REQUIRE(w.nseg == 1 || workspace, "noise_decay_attn_walk: this shape needs a workspace");
-  const int es = dtype == NOISE_F32 ? 4 : 2, nv = dtype == NOISE_BF16 ? 8 : 4;
-  w.va = rows_vec(a, w.sa, nv, es), w.vk = rows_vec(k, w.sk, nv, es), w.vv = rows_vec(v, w.sv, nv, es), w.vo = rows_vec(o, w.so, nv, es);
+  if (dtype == NOISE_BF16) {
+    w.va = rows_buffer(a, w.sa, dk), w.vk = rows_buffer(k, w.sk, dk), w.vv = rows_buffer(v, w.sv, dv), w.vo = rows_buffer(o, w.so, dv);
+  } else {
+    const int es = dtype == NOISE_F32 ? 4 : 2;
+    w.va = rows_vec(a, w.sa, 4, es), w.vk = rows_vec(k, w.sk, 4, es), w.vv = rows_vec(v, w.sv, 4, es), w.vo = 0;
+  }
   hipStream_t st = (hipStream_t)stream;
   if (dtype == NOISE_F32) walk_launch<float>(w, st);
   else if (dtype == NOISE_BF16) walk_launch_bf16(w, st);
