@@ -392,7 +392,6 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
   for (int c0 = p0; c0 < p1; c0 += DB_C) {
     const int n = min(DB_C, p1 - c0);                       // tokens in this chunk
     const int shift = w.shift && c0 == 0 ? 1 : 0;
-    __syncthreads();                                        // the previous chunk's readers are done
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
       const int at = (i0 + s * RS) * LD + cc;
@@ -457,9 +456,9 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt) O[it][nt] *= f;
       }
-      __syncthreads();
     }
-    // ---- this chunk's values: O += P V and X = lam^n X + K^T V'
+    // ---- X = lam^n X + K^T V'
+    bf16x8 v[2][2];
     const float f = pw[n - shift];
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp)
@@ -469,17 +468,8 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
         for (int nt = 0; nt < 2; ++nt) X[kp][s][nt] *= f;
 #pragma unroll
     for (int jj = 0; jj < 2; ++jj) {
-      bf16x8 v[2];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) v[nt] = read_tokens<LD>(sv + jj * 32 * LD + col0 + 4 * nt, q, l16);
-      if (!STATE_ONLY) {
-#pragma unroll
-        for (int it = 2 * jj; it < 4; ++it) {
-          const bf16x8 y = *(const bf16x8*)(sp + (it * 16 + l16) * LDP + jj * 32 + 8 * q);
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt) O[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[nt], y, O[it][nt], 0, 0, 0);
-        }
-      }
+      for (int nt = 0; nt < 2; ++nt) v[jj][nt] = read_tokens<LD>(sv + jj * 32 * LD + col0 + 4 * nt, q, l16);
       u32x4 t[2][3];
       const float* f8 = pv + DB_C - n + jj * 32 + 8 * q;
 #pragma unroll
@@ -487,7 +477,7 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
         const float f0 = f8[2 * e], f1 = f8[2 * e + 1];
 #pragma unroll
         for (int nt = 0; nt < 2; ++nt) {
-          const unsigned u = __builtin_bit_cast(u32x4, v[nt])[e];
+          const unsigned u = __builtin_bit_cast(u32x4, v[jj][nt])[e];
           float y0 = low_bf16(u) * f0, y1 = high_bf16(u) * f1;
 #pragma unroll
           for (int z = 0; z < 3; ++z) {
@@ -510,7 +500,19 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
               X[kp][s][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, t[nt][z]), X[kp][s][nt], 0, 0, 0);
         }
     }
+    // every wave is done with the tiles and has left its weights: the next chunk's tiles may be written from here on, its
+    // weights only behind the next barrier, i.e. when all have read these
+    __syncthreads();
     if (!STATE_ONLY) {
+      // ---- O += P V
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj)
+#pragma unroll
+        for (int it = 2 * jj; it < 4; ++it) {
+          const bf16x8 y = *(const bf16x8*)(sp + (it * 16 + l16) * LDP + jj * 32 + 8 * q);
+#pragma unroll
+          for (int nt = 0; nt < 2; ++nt) O[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[jj][nt], y, O[it][nt], 0, 0, 0);
+        }
       const int col = col0 + 8 * q;
       const auto rs = chunk_rows(ob + (w.reverse ? len - c0 - n : c0) * w.so.t, n, w.so.t, w.dv);
 #pragma unroll
