@@ -250,23 +250,26 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4) void walk_f32_kernel(WalkArg
       }
 }
 
-// bf16 tokens on the bf16 matrix cores (v_mfma_f32_16x16x32_bf16), 64 tokens per chunk, P / 32 waves that own 32 state
+// bf16 tokens on the bf16 matrix cores (v_mfma_f32_16x16x32_bf16), 64 tokens per chunk, P / 16 waves that own 16 state
 // columns each.  What is rounded to bf16 on its way into a product, and what is not:
 //   * the weights lam^{i-j} (a_i . k_j) and the state as it meets a_i: once each, like the output they lead to;
 //   * lam^{n-1-j} v_j on its way into the state is split into three bf16 terms (24 bits), since the state is fp32, carried
 //     over any number of chunks and returned: X keeps fp32 accuracy at three products per term.
 // Operands: lane (q = lane / 16, l = lane % 16) of an MFMA takes eight contraction indices 8q..8q+7 of row l, and an
 // accumulator tile holds rows 4q + r of column l.  Two state tiles whose rows are dealt as 8q + 4s + r (s = tile) together
-// are the eight indices the next product wants, so the state stays in registers; the same deal on the columns makes a lane's
-// outputs eight neighbours (one 16-byte store).  Contractions over tokens read K and V through ds_read_b64_tr_b16, which
-// hands a lane four tokens of one column.  Rows are padded by 32 bytes: a transposing read of four rows then touches every
-// bank once.
+// are the eight indices the next product wants, so the state stays in registers.  Contractions over tokens read K and V
+// through ds_read_b64_tr_b16, which hands a lane four tokens of one column; K's columns lie in LDS as those tiles want
+// them (of every 32, the 4-element halves s = 0 first), so that a transposing read takes 32 contiguous bytes of four rows, and
+// rows are padded by 32 bytes, so that it touches every bank once.
+// Bound: HBM in the end, but first the latency of the chain load - weights - products of a chunk: 16 columns per wave (not
+// 32) halve the registers of a wave and put four waves on a SIMD, at twice the LDS reads of a and K.
 constexpr int DB_C = 64;
 
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using bf16x4 = __attribute__((ext_vector_type(4))) __bf16;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
+using u32x2 = __attribute__((ext_vector_type(2))) unsigned;
 
 __device__ __forceinline__ u32x4 row8(const bf16_t* base, bool live, int c, int width, bool vec) {
   u32x4 r = {0u, 0u, 0u, 0u};
@@ -278,12 +281,11 @@ __device__ __forceinline__ u32x4 row8(const bf16_t* base, bool live, int c, int 
   return __builtin_bit_cast(u32x4, t);
 }
 
-// Eight tokens (rows row0 + 8q .. + 7) of the column that lane l stands for when tile columns are dealt as 8 (l / 4) + l % 4:
-// `tile` points at (row0, first column + 4 * tile number).
+// Eight tokens (rows 8q .. 8q + 7 behind `tile`) of column l of the 16 columns that start there.
 template <int LD>
 __device__ __forceinline__ bf16x8 read_tokens(const bf16_t* tile, int q, int l16) {
   using lds4 = __attribute__((address_space(3))) s16x4;
-  const bf16_t* p = tile + (8 * q + l16 / 4) * LD + l16 % 4 * 8;
+  const bf16_t* p = tile + (8 * q + l16 / 4) * LD + l16 % 4 * 4;
   const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
   const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * LD));
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -306,8 +308,8 @@ __device__ __forceinline__ int chunk_offset(int off, bool exists) { return (int)
 
 // VEC: every row of a, k, v and o starts on a 16-byte boundary, rows do not overlap and a chunk spans less than 2 GB.
 template <int P, bool STATE_ONLY, bool VEC>
-__global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
-  constexpr int NTHR = P * 2, NW = P / 32, KP = P / 32;      // KP: pairs of state row tiles
+__global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_bf16_kernel(WalkArgs w) {
+  constexpr int NTHR = P * 4, NW = P / 16, KP = P / 32;      // KP: pairs of state row tiles
   constexpr int LD = P + 16, LDP = DB_C + 8, SLOTS = DB_C * P / 8 / NTHR;
   __shared__ __attribute__((aligned(16))) bf16_t sa[STATE_ONLY ? 8 : DB_C * LD];
   __shared__ __attribute__((aligned(16))) bf16_t sk[DB_C * LD], sv[DB_C * LD];
@@ -337,12 +339,12 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
   const bf16_t* ab = (const bf16_t*)w.a + (size_t)b * w.sa.b + (size_t)h * w.sa.h;
   const bf16_t* kb = (const bf16_t*)w.k + (size_t)b * w.sk.b + (size_t)h * w.sk.h;
   const bf16_t* vb = (const bf16_t*)w.v + (size_t)b * w.sv.b + (size_t)h * w.sv.h;
-  const int col0 = wave * 32;                                // the wave's state columns
+  const int col0 = wave * 16;                                // the wave's state columns
 
-  // X[kp][s][nt][r]: row kp 32 + 8q + 4s + r, column col0 + 8 (l / 4) + 4 nt + l % 4
-  f32x4 X[KP][2][2];
+  // X[kp][s][r]: row kp 32 + 8q + 4s + r, column col0 + l
+  f32x4 X[KP][2];
   const size_t mat = (size_t)w.dk * w.dv;
-  const int xcol = col0 + 8 * (l16 >> 2) + (l16 & 3);
+  const int xcol = col0 + l16;
   {
     const bool from_seg = !STATE_ONLY && seg > 0;
     const float* src = STATE_ONLY ? nullptr : from_seg ? w.seg + ((size_t)bh * w.nseg + seg) * mat : w.x0 ? w.x0 + (size_t)bh * mat : nullptr;
@@ -352,12 +354,10 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int row = kp * 32 + 8 * q + 4 * s + r, col = xcol + 4 * nt;
-            X[kp][s][nt][r] = src && row < w.dk && col < w.dv ? src[(size_t)row * sr + (size_t)col * sc] : 0.f;
-          }
+        for (int r = 0; r < 4; ++r) {
+          const int row = kp * 32 + 8 * q + 4 * s + r;
+          X[kp][s][r] = src && row < w.dk && xcol < w.dv ? src[(size_t)row * sr + (size_t)xcol * sc] : 0.f;
+        }
   }
 
   // a thread's SLOTS pieces of a tile are RS rows apart, in the same column
@@ -396,12 +396,14 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
     for (int s = 0; s < SLOTS; ++s) {
       const int at = (i0 + s * RS) * LD + cc;
       if (!STATE_ONLY) *(u32x4*)(sa + at) = ra[s];
-      *(u32x4*)(sk + at) = rk[s];
+      bf16_t* kd = sk + (i0 + s * RS) * LD + cc / 32 * 32 + cc % 32 / 2;
+      *(uint2*)kd = make_uint2(rk[s][0], rk[s][1]);
+      *(uint2*)(kd + 16) = make_uint2(rk[s][2], rk[s][3]);
       *(u32x4*)(sv + at) = rv[s];
     }
     __syncthreads();
     if (c0 + DB_C < p1) fetch(c0 + DB_C);
-    f32x4 O[STATE_ONLY ? 1 : 4][2];
+    f32x4 O[STATE_ONLY ? 1 : 4];
     if (!STATE_ONLY) {
       // ---- weights, transposed tile by tile (rows j, columns i) so that a lane holds four neighbouring j of one i: the ten
       // 16 x 16 tiles on and below the diagonal are dealt over the waves; the other tiles of a pair of 16 that is read are zero
@@ -413,7 +415,9 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
         if (tile < 10) {
 #pragma unroll
           for (int kp = 0; kp < KP; ++kp) {
-            const bf16x8 x = *(const bf16x8*)(sk + (jt * 16 + l16) * LD + kp * 32 + 8 * q);
+            const bf16_t* kr = sk + (jt * 16 + l16) * LD + kp * 32 + 4 * q;
+            const uint2 k0 = *(const uint2*)kr, k1 = *(const uint2*)(kr + 16);
+            const bf16x8 x = __builtin_bit_cast(bf16x8, u32x4{k0.x, k0.y, k1.x, k1.y});
             const bf16x8 y = *(const bf16x8*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
             acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0);
           }
@@ -430,74 +434,54 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
       }
       // ---- what the state contributes, transposed: rows are the wave's columns, columns the tokens
 #pragma unroll
-      for (int it = 0; it < 4; ++it)
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) O[it][nt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int it = 0; it < 4; ++it) O[it] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kp = 0; kp < KP; ++kp) {
-        bf16x8 x[2];
+        u32x4 u;
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          u32x4 u;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) u[e] = pack_bf16(X[kp][e >> 1][nt][2 * (e & 1)], X[kp][e >> 1][nt][2 * (e & 1) + 1]);
-          x[nt] = __builtin_bit_cast(bf16x8, u);
-        }
+        for (int e = 0; e < 4; ++e) u[e] = pack_bf16(X[kp][e >> 1][2 * (e & 1)], X[kp][e >> 1][2 * (e & 1) + 1]);
+        const bf16x8 x = __builtin_bit_cast(bf16x8, u);
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
           const bf16x8 y = *(const bf16x8*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt) O[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[nt], y, O[it][nt], 0, 0, 0);
+          O[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, O[it], 0, 0, 0);
         }
       }
 #pragma unroll
-      for (int it = 0; it < 4; ++it) {
-        const float f = w.s_o * pw[it * 16 + l16 + 1 - shift];
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) O[it][nt] *= f;
-      }
+      for (int it = 0; it < 4; ++it) O[it] *= w.s_o * pw[it * 16 + l16 + 1 - shift];
     }
     // ---- X = lam^n X + K^T V'
-    bf16x8 v[2][2];
+    bf16x8 v[2];
     const float f = pw[n - shift];
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp)
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) X[kp][s][nt] *= f;
+      for (int s = 0; s < 2; ++s) X[kp][s] *= f;
 #pragma unroll
     for (int jj = 0; jj < 2; ++jj) {
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) v[jj][nt] = read_tokens<LD>(sv + jj * 32 * LD + col0 + 4 * nt, q, l16);
-      u32x4 t[2][3];
+      v[jj] = read_tokens<LD>(sv + jj * 32 * LD + col0, q, l16);
+      u32x4 t[3];
       const float* f8 = pv + DB_C - n + jj * 32 + 8 * q;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float f0 = f8[2 * e], f1 = f8[2 * e + 1];
+        const unsigned u = __builtin_bit_cast(u32x4, v[jj])[e];
+        float y0 = low_bf16(u) * f8[2 * e], y1 = high_bf16(u) * f8[2 * e + 1];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          const unsigned u = __builtin_bit_cast(u32x4, v[jj][nt])[e];
-          float y0 = low_bf16(u) * f0, y1 = high_bf16(u) * f1;
-#pragma unroll
-          for (int z = 0; z < 3; ++z) {
-            const unsigned c = pack_bf16(y0, y1);
-            t[nt][z][e] = c;
-            y0 -= low_bf16(c);
-            y1 -= high_bf16(c);
-          }
+        for (int z = 0; z < 3; ++z) {
+          const unsigned c = pack_bf16(y0, y1);
+          t[z][e] = c;
+          y0 -= low_bf16(c);
+          y1 -= high_bf16(c);
         }
       }
 #pragma unroll
       for (int kp = 0; kp < KP; ++kp)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const bf16x8 x = read_tokens<LD>(sk + jj * 32 * LD + kp * 32 + 4 * s, q, l16);
+          const bf16x8 x = read_tokens<LD>(sk + jj * 32 * LD + kp * 32 + 16 * s, q, l16);
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int z = 2; z >= 0; --z)
-              X[kp][s][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, t[nt][z]), X[kp][s][nt], 0, 0, 0);
+          for (int z = 2; z >= 0; --z)
+            X[kp][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, t[z]), X[kp][s], 0, 0, 0);
         }
     }
     // every wave is done with the tiles and has left its weights: the next chunk's tiles may be written from here on, its
@@ -510,25 +494,22 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
 #pragma unroll
         for (int it = 2 * jj; it < 4; ++it) {
           const bf16x8 y = *(const bf16x8*)(sp + (it * 16 + l16) * LDP + jj * 32 + 8 * q);
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt) O[it][nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[jj][nt], y, O[it][nt], 0, 0, 0);
+          O[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[jj], y, O[it], 0, 0, 0);
         }
-      const int col = col0 + 8 * q;
+      const int col = col0 + 4 * q;
       const auto rs = chunk_rows(ob + (w.reverse ? len - c0 - n : c0) * w.so.t, n, w.so.t, w.dv);
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
         const int i = it * 16 + l16;
-        u32x4 y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[e] = pack_bf16(O[it][e >> 1][2 * (e & 1)], O[it][e >> 1][2 * (e & 1) + 1]);
+        const u32x2 y = {pack_bf16(O[it][0], O[it][1]), pack_bf16(O[it][2], O[it][3])};
         const int row = w.reverse ? n - 1 - i : i;
         if (VEC) {
-          __builtin_amdgcn_raw_buffer_store_b128(y, rs, chunk_offset(row * 2 * (int)w.so.t + 2 * col, col < w.dv), 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b64(y, rs, chunk_offset(row * 2 * (int)w.so.t + 2 * col, col < w.dv), 0, 0);
         } else if (i < n) {
           bf16_t* op = ob + ((w.reverse ? len - c0 - n : c0) + row) * w.so.t + col;
-          const bf16x8 z = __builtin_bit_cast(bf16x8, y);
+          const bf16x4 z = __builtin_bit_cast(bf16x4, y);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
+          for (int e = 0; e < 4; ++e)
             if (col + e < w.dv) op[e] = z[e];
         }
       }
@@ -543,12 +524,10 @@ __global__ __launch_bounds__(P * 2, 2) void walk_bf16_kernel(WalkArgs w) {
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int row = kp * 32 + 8 * q + 4 * s + r, col = xcol + 4 * nt;
-          if (row < w.dk && col < w.dv) dst[(size_t)row * w.dv + col] = X[kp][s][nt][r] * f;
-        }
+      for (int r = 0; r < 4; ++r) {
+        const int row = kp * 32 + 8 * q + 4 * s + r;
+        if (row < w.dk && xcol < w.dv) dst[(size_t)row * w.dv + xcol] = X[kp][s][r] * f;
+      }
 }
 
 // Sums of the segments -> states before the segments, in place: seg[s] = lam^{seg_len} seg[s-1] + sum[s-1], seg[0] = x0.  The
@@ -642,8 +621,8 @@ void walk_launch_bf16(const WalkArgs& w, hipStream_t st) {
   const bool vec = w.va && w.vk && w.vv && w.vo;
 #define GO(P, ONLY)                                                                                        \
   do {                                                                                                     \
-    if (vec) hipLaunchKernelGGL((walk_bf16_kernel<P, ONLY, true>), dim3(grid), dim3(P * 2), 0, st, w);     \
-    else hipLaunchKernelGGL((walk_bf16_kernel<P, ONLY, false>), dim3(grid), dim3(P * 2), 0, st, w);        \
+    if (vec) hipLaunchKernelGGL((walk_bf16_kernel<P, ONLY, true>), dim3(grid), dim3(P * 4), 0, st, w);     \
+    else hipLaunchKernelGGL((walk_bf16_kernel<P, ONLY, false>), dim3(grid), dim3(P * 4), 0, st, w);        \
   } while (0)
 #define PICK(ONLY)             \
   do {                         \
