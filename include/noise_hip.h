@@ -397,11 +397,12 @@ int noise_layer_norm_bwd(const void* dy, long lddy, const void* x, long ldx, con
  * and behind the length are zero.  log_decay g [H] <= 0; lengths [B] or NULL (all T); x0, x_end [B][H][dk][dv] fp32 or NULL
  * (x0_transposed: x0 is [B][H][dv][dk]).  reverse != 0: last token first, x0 meets the last token undecayed and x_end gets
  * one more decay (the gradient of the state before the first token).  1 <= dk, dv <= 128.
- * workspace: noise_decay_attn_workspace() floats (0: may be NULL) */
+ * workspace: noise_decay_attn_workspace() floats (0: may be NULL); reuse != 0: it is as a walk with k and v swapped, x0
+ * transposed and all else equal has just left it */
 long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv);
 int noise_decay_attn_walk(const void* a, const void* k, const void* v, void* o, const long* strides, const float* log_decay,
                           const int* lengths, const float* x0, int x0_transposed, float* x_end, float* workspace, float s_o,
-                          float s_kv, int reverse, int B, int T, int H, int dk, int dv, int dtype, void* stream);
+                          float s_kv, int reverse, int reuse, int B, int T, int H, int dk, int dv, int dtype, void* stream);
 /* one token per clip: state [B][H][dk][dv] updated in place, o [B][H][dv]; strides: (clip, head) of q, k, v on the HOST */
 int noise_decay_attn_step(const void* q, const void* k, const void* v, const long* strides, const float* log_decay, float* state,
                           void* o, float scale, int B, int H, int dk, int dv, int dtype, void* stream);

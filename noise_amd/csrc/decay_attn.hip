@@ -39,6 +39,7 @@ struct WalkArgs {
   float s_o, s_kv;
   int B, T, H, dk, dv, nseg, seg_len;
   int reverse, shift, end_decay, x0_tr;
+  int seg_tr;               // seg holds the states of the walk with k and v swapped, [dv][dk] each: nothing to sum
   int va, vk, vv, vo;       // rows allow wide accesses: rows_buffer for bf16, four elements at a time otherwise
 };
 
@@ -99,7 +100,8 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4) void walk_f32_kernel(WalkArg
   {
     const bool from_seg = !STATE_ONLY && seg > 0;
     const float* src = STATE_ONLY ? nullptr : from_seg ? w.seg + ((size_t)bh * w.nseg + seg) * mat : w.x0 ? w.x0 + (size_t)bh * mat : nullptr;
-    const int sr = !from_seg && w.x0_tr ? 1 : w.dv, sc = !from_seg && w.x0_tr ? w.dk : 1;
+    const bool tr = from_seg ? w.seg_tr : w.x0_tr;
+    const int sr = tr ? 1 : w.dv, sc = tr ? w.dk : 1;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -348,7 +350,8 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_bf16_kernel(Walk
   {
     const bool from_seg = !STATE_ONLY && seg > 0;
     const float* src = STATE_ONLY ? nullptr : from_seg ? w.seg + ((size_t)bh * w.nseg + seg) * mat : w.x0 ? w.x0 + (size_t)bh * mat : nullptr;
-    const int sr = !from_seg && w.x0_tr ? 1 : w.dv, sc = !from_seg && w.x0_tr ? w.dk : 1;
+    const bool tr = from_seg ? w.seg_tr : w.x0_tr;
+    const int sr = tr ? 1 : w.dv, sc = tr ? w.dk : 1;
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp)
 #pragma unroll
@@ -630,7 +633,7 @@ void walk_launch_bf16(const WalkArgs& w, hipStream_t st) {
     else if (d <= 64) GO(64, ONLY); \
     else GO(128, ONLY);        \
   } while (0)
-  if (w.nseg > 1) {
+  if (w.nseg > 1 && !w.seg_tr) {
     PICK(true);
     scan_launch(w, st);
   }
@@ -651,7 +654,7 @@ void walk_launch(const WalkArgs& w, hipStream_t st) {
     else if (d <= 64) GO(64, ONLY); \
     else GO(128, ONLY);        \
   } while (0)
-  if (w.nseg > 1) {
+  if (w.nseg > 1 && !w.seg_tr) {
     PICK(true);
     scan_launch(w, st);
   }
@@ -660,10 +663,14 @@ void walk_launch(const WalkArgs& w, hipStream_t st) {
 #undef GO
 }
 
-// Segments of the token axis: as many as it takes to give every CU two workgroups, none shorter than 256 tokens (the state of a
-// segment is written, scanned and read again: dk dv values each against 256 tokens' rows).
-int walk_segments(long bh, int T) {
-  const long want = (2L * 256 + bh - 1) / bh, most = T / (4 * DB_C);
+// Segments of the token axis: as many as it takes to fill every CU with the workgroups it holds (a workgroup has one wave per
+// 16 columns, so narrow heads need more of them), none shorter than 64 tokens or than twice the head (a segment's state is
+// written, scanned and read again: 4 dk dv values against its tokens' 4 rows).  DA_PER_CU: workgroups per CU for heads of at
+// most 16, 32, 64 and 128.
+constexpr int DA_PER_CU[4] = {8, 5, 3, 2};
+int walk_segments(long bh, int T, int d) {
+  const int size = d <= 16 ? 0 : d <= 32 ? 1 : d <= 64 ? 2 : 3;
+  const long want = (256L * DA_PER_CU[size] + bh - 1) / bh, most = T / (d <= 32 ? 64 : 2 * d);
   const long n = want < most ? want : most;
   return n < 1 ? 1 : (int)n;
 }
@@ -681,14 +688,15 @@ const char* walk_check(int B, int T, int H, int dk, int dv, int dtype) {
 // Floats of workspace a walk of this shape needs.
 NOISE_EXPORT long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv) {
   if (walk_check(B, T, H, dk, dv, NOISE_F32)) return 0;
-  const int n = walk_segments((long)B * H, T);
+  const int n = walk_segments((long)B * H, T, dk > dv ? dk : dv);
   return n > 1 ? (long)B * H * n * dk * dv : 0;
 }
 
-// strides: (clip, token, head) of a, k, v and o; reverse: last token first, with the undecayed first step and the decayed end
+// strides: (clip, token, head) of a, k, v and o; reverse: last token first, with the undecayed first step and the decayed end;
+// reuse: the workspace is as the walk with k and v (and x0 with its transpose) swapped left it
 NOISE_EXPORT int noise_decay_attn_walk(const void* a, const void* k, const void* v, void* o, const long* strides,
                                        const float* log_decay, const int* lengths, const float* x0, int x0_transposed,
-                                       float* x_end, float* workspace, float s_o, float s_kv, int reverse, int B, int T, int H,
+                                       float* x_end, float* workspace, float s_o, float s_kv, int reverse, int reuse, int B, int T, int H,
                                        int dk, int dv, int dtype, void* stream) {
   const char* why = walk_check(B, T, H, dk, dv, dtype);
   NOISE_REQUIRE(!why, "noise_decay_attn_walk: %s (B %d, T %d, H %d, head sizes %d and %d)", why, B, T, H, dk, dv);
@@ -702,8 +710,8 @@ NOISE_EXPORT int noise_decay_attn_walk(const void* a, const void* k, const void*
   w.log_decay = log_decay, w.lengths = lengths, w.x0 = x0, w.x0_tr = x0_transposed, w.x_end = x_end, w.seg = workspace;
   w.s_o = s_o, w.s_kv = s_kv;
   w.B = B, w.T = T, w.H = H, w.dk = dk, w.dv = dv;
-  w.reverse = reverse, w.shift = reverse, w.end_decay = reverse;
-  w.nseg = walk_segments((long)B * H, T);
+  w.reverse = reverse, w.shift = reverse, w.end_decay = reverse, w.seg_tr = reuse;
+  w.nseg = walk_segments((long)B * H, T, dk > dv ? dk : dv);
   w.seg_len = (noise_cdiv(T, w.nseg) + DB_C - 1) / DB_C * DB_C;
   w.nseg = noise_cdiv(T, w.seg_len);
   NOISE_REQUIRE(w.nseg == 1 || workspace, "noise_decay_attn_walk: this shape needs a workspace");

@@ -25,7 +25,7 @@ from . import _lib
 from ._lib import _F, _I, _L, _P, ptr
 
 _lib.register({
-    "noise_decay_attn_walk": [_P] * 8 + [_I, _P, _P, _F, _F] + [_I] * 7 + [_P],
+    "noise_decay_attn_walk": [_P] * 8 + [_I, _P, _P, _F, _F] + [_I] * 8 + [_P],
     "noise_decay_attn_step": [_P] * 7 + [_F] + [_I] * 5 + [_P],
     "noise_decay_attn_workspace": [_I] * 5,
 })
@@ -70,18 +70,20 @@ def _check_lengths(lengths, B):
     return lengths.to(torch.int32).contiguous()
 
 
-def _walk(a, k, v, log_decay, lengths, x0, x0_transposed, x_end, s_o, s_kv, reverse):
+def _walk(a, k, v, log_decay, lengths, x0, x0_transposed, x_end, s_o, s_kv, reverse, swapped=None):
+    """One pass of the operator at the top of csrc/decay_attn.hip: (o, workspace).  `swapped`: the workspace that the pass with
+    k and v swapped returned."""
     B, T, H, dk = a.shape
     dv = v.shape[-1]
     a, k, v = _unit(a), _unit(k), _unit(v)
     o = torch.empty(B, T, H, dv, device=a.device, dtype=a.dtype)
     n = _lib.lib.noise_decay_attn_workspace(B, T, H, dk, dv)
-    ws = torch.empty(n, device=a.device, dtype=torch.float32) if n else None
+    ws = swapped if swapped is not None else torch.empty(n, device=a.device, dtype=torch.float32) if n else None
     strides = (_L * 12)(*a.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3])
     _lib.call("noise_decay_attn_walk", ptr(a), ptr(k), ptr(v), ptr(o), strides, ptr(log_decay), ptr(lengths), ptr(x0),
-              int(x0_transposed), ptr(x_end), ptr(ws), s_o, s_kv, int(reverse), B, T, H, dk, dv, _lib.DTYPES[a.dtype], _lib.stream(),
+              int(x0_transposed), ptr(x_end), ptr(ws), s_o, s_kv, int(reverse), int(swapped is not None), B, T, H, dk, dv, _lib.DTYPES[a.dtype], _lib.stream(),
               nbytes=a.element_size() * 2 * (a.numel() + v.numel()))
-    return o
+    return o, ws
 
 
 def decay_attention_fwd(q, k, v, log_decay, state=None, lengths=None, scale=None):
@@ -95,7 +97,7 @@ def decay_attention_fwd(q, k, v, log_decay, state=None, lengths=None, scale=None
             return torch.empty(v.shape, device=v.device, dtype=v.dtype), end
         end = torch.empty(B, H, dk, dv, device=q.device, dtype=torch.float32)
         x0 = state.contiguous() if state is not None else None
-        o = _walk(q, k, v, log_decay.contiguous(), lengths, x0, False, end, scale, 1.0, False)
+        o, _ = _walk(q, k, v, log_decay.contiguous(), lengths, x0, False, end, scale, 1.0, False)
         return o, end
 
 
@@ -117,9 +119,9 @@ def decay_attention_bwd(do, q, k, v, log_decay, state=None, lengths=None, scale=
         x0 = state.contiguous() if state is not None else None
         x1 = d_state.contiguous() if d_state is not None else None
         do = _unit(do)
-        dq = _walk(do, v, k, g, lengths, x0, True, None, scale, 1.0, False)
-        dvv = _walk(k, q, do, g, lengths, x1, False, d0, 1.0, scale, True)
-        dkk = _walk(v, do, q, g, lengths, x1, True, None, 1.0, scale, True)
+        dq, _ = _walk(do, v, k, g, lengths, x0, True, None, scale, 1.0, False)
+        dvv, ws = _walk(k, q, do, g, lengths, x1, False, d0, 1.0, scale, True)
+        dkk, _ = _walk(v, do, q, g, lengths, x1, True, None, 1.0, scale, True, swapped=ws)
         return dq, dkk, dvv, d0
 
 
