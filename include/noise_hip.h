@@ -399,7 +399,7 @@ int noise_layer_norm_bwd(const void* dy, long lddy, const void* x, long ldx, con
  * one more decay (the gradient of the state before the first token).  1 <= dk, dv <= 128.
  * workspace: noise_decay_attn_workspace() floats (0: may be NULL); reuse != 0: it is as a walk with k and v swapped, x0
  * transposed and all else equal has just left it */
-long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv);
+long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv, int dtype);
 int noise_decay_attn_walk(const void* a, const void* k, const void* v, void* o, const long* strides, const float* log_decay,
                           const int* lengths, const float* x0, int x0_transposed, float* x_end, float* workspace, float s_o,
                           float s_kv, int reverse, int reuse, int B, int T, int H, int dk, int dv, int dtype, void* stream);

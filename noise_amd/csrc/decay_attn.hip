@@ -68,7 +68,7 @@ __device__ __forceinline__ f32x4 row4(const T* base, bool live, int c, int width
 // 16-byte LDS reads and an accumulator tile (row 4q + r in register r) is the next product's operand as it lies: the state
 // never leaves its registers.  Only the C x C weights pass through LDS (each wave computes a share of them).
 template <typename T, int P, bool STATE_ONLY>
-__global__ __launch_bounds__(P >= 64 ? 256 : P * 4) void walk_f32_kernel(WalkArgs w) {
+__global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_f32_kernel(WalkArgs w) {
   constexpr int NW = P >= 64 ? 4 : P / 16, NT = P / 16 / NW, KT = P / 16, NTHR = NW * 64;
   constexpr int LD = P + 4, LDP = DA_C + 4, SLOTS = DA_C * P / 4 / NTHR;
   __shared__ float sa[STATE_ONLY ? 4 : DA_C * LD];
@@ -143,8 +143,9 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4) void walk_f32_kernel(WalkArg
     f32x4 O[2][NT];
     if (!STATE_ONLY) {
       // ---- weights lam^{i-j} (a_i . k_j), one 16 x 16 tile per wave; the tile above the diagonal is never read
-      for (int tile = wave; tile < 4; tile += NW) {
-        const int mt = tile >> 1, jt = tile & 1;
+#pragma unroll
+      for (int u = 0; u < 4 / NW; ++u) {
+        const int mt = (u * NW + wave) >> 1, jt = (u * NW + wave) & 1;
         if (jt > mt) continue;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -338,6 +339,13 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_bf16_kernel(Walk
     if (i < DB_C + 16) pp[i] = w.s_o * w.s_kv * decay_pow(g2, i - 15);
     pv[i] = w.s_kv * decay_pow(g2, DB_C - 1 - i);
   }
+  if (!STATE_ONLY) {
+    // the weight tiles (0, 1) and (2, 3) lie above the diagonal but in a pair that is read: they stay zero
+    for (int i = tid; i < 32 * 16; i += NTHR) {
+      const int half = i >> 8, r = i >> 4 & 15, c = i & 15;
+      sp[(half * 32 + r) * LDP + half * 32 + 16 + c] = (bf16_t)0.f;
+    }
+  }
   const bf16_t* ab = (const bf16_t*)w.a + (size_t)b * w.sa.b + (size_t)h * w.sa.h;
   const bf16_t* kb = (const bf16_t*)w.k + (size_t)b * w.sk.b + (size_t)h * w.sk.h;
   const bf16_t* vb = (const bf16_t*)w.v + (size_t)b * w.sv.b + (size_t)h * w.sv.h;
@@ -409,30 +417,25 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_bf16_kernel(Walk
     f32x4 O[STATE_ONLY ? 1 : 4];
     if (!STATE_ONLY) {
       // ---- weights, transposed tile by tile (rows j, columns i) so that a lane holds four neighbouring j of one i: the ten
-      // 16 x 16 tiles on and below the diagonal are dealt over the waves; the other tiles of a pair of 16 that is read are zero
-      for (int tile = wave; tile < 12; tile += NW) {
-        // 0..9: (it, jt) with jt <= it in order; 10, 11: the zero tiles (0, 1) and (2, 3)
-        const int it = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : tile < 10 ? 3 : tile == 10 ? 0 : 2;
-        const int jt = tile < 10 ? tile - it * (it + 1) / 2 : it + 1;
+      // 16 x 16 tiles on and below the diagonal, in the order (0,0) (1,0) (1,1) (2,0) ..., are dealt over the waves
+#pragma unroll(P == 128 ? 1 : 5)   // eight waves have two tiles at most, and no registers for both at once
+      for (int u = 0; u * NW < 10; ++u) {
+        const int tile = u * NW + wave;
+        if ((u + 1) * NW > 10 && tile >= 10) break;
+        const int it = 0xffa94 >> (2 * tile) & 3, jt = tile - it * (it + 1) / 2;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        if (tile < 10) {
 #pragma unroll
-          for (int kp = 0; kp < KP; ++kp) {
-            const bf16_t* kr = sk + (jt * 16 + l16) * LD + kp * 32 + 4 * q;
-            const uint2 k0 = *(const uint2*)kr, k1 = *(const uint2*)(kr + 16);
-            const bf16x8 x = __builtin_bit_cast(bf16x8, u32x4{k0.x, k0.y, k1.x, k1.y});
-            const bf16x8 y = *(const bf16x8*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0);
-          }
+        for (int kp = 0; kp < KP; ++kp) {
+          const bf16_t* kr = sk + (jt * 16 + l16) * LD + kp * 32 + 4 * q;
+          const uint2 k0 = *(const uint2*)kr, k1 = *(const uint2*)(kr + 16);
+          const bf16x8 x = __builtin_bit_cast(bf16x8, u32x4{k0.x, k0.y, k1.x, k1.y});
+          const bf16x8 y = *(const bf16x8*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0);
         }
         const int i = it * 16 + l16, j = jt * 16 + 4 * q;
-        if (it == jt) {
+        const bool diag = it == jt;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc[r] = l16 >= 4 * q + r ? acc[r] * pp[15 + i - j - r] : 0.f;
-        } else if (tile < 10) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[r] *= pp[15 + i - j - r];
-        }
+        for (int r = 0; r < 4; ++r) acc[r] = diag && l16 < 4 * q + r ? 0.f : acc[r] * pp[15 + i - j - r];
         *(uint2*)(sp + i * LDP + j) = make_uint2(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]));
       }
       // ---- what the state contributes, transposed: rows are the wave's columns, columns the tokens
@@ -663,14 +666,19 @@ void walk_launch(const WalkArgs& w, hipStream_t st) {
 #undef GO
 }
 
-// Segments of the token axis: as many as it takes to fill every CU with the workgroups it holds (a workgroup has one wave per
-// 16 columns, so narrow heads need more of them), none shorter than 64 tokens or than twice the head (a segment's state is
-// written, scanned and read again: 4 dk dv values against its tokens' 4 rows).  DA_PER_CU: workgroups per CU for heads of at
-// most 16, 32, 64 and 128.
-constexpr int DA_PER_CU[4] = {8, 5, 3, 2};
-int walk_segments(long bh, int T, int d) {
-  const int size = d <= 16 ? 0 : d <= 32 ? 1 : d <= 64 ? 2 : 3;
-  const long want = (256L * DA_PER_CU[size] + bh - 1) / bh, most = T / (d <= 32 ? 64 : 2 * d);
+// Segments of the token axis.  From `full` (clip, head) pairs on, clips and heads fill the GPU well enough that the second
+// read of k and v costs more than it gives; below, the axis is cut until there are `target` workgroups.  A workgroup has one wave
+// per 16 columns (fp32: at most four), so narrow heads need more of them.  Measured on 2048 tokens, us per forward pass with
+// 1 / 2 / 4 / 8 segments: bf16, heads of 128: 256 pairs 176 / 197 / 236 / 297, 128 pairs 152 / 132 / 127 / 159; heads of 64: 512
+// pairs 133 / 186 / 198 / 234, 128 pairs 92 / 73 / 60 / 61; heads of 32: 512 pairs 93 / 106 / 122 / 130, 128 pairs 82 / 62 / 44 /
+// 42; fp32, heads of 128: 256 pairs 489 / 554 / 568 / 641, heads of 16: 1024 pairs 183 / 205 / 239 / 246, 256 pairs 159 / 112 / 69 / 70.
+// No segment is shorter than 64 tokens or than twice the head: its state is written, scanned and read again.
+int walk_segments(long bh, int T, int d, bool bf16) {
+  static const int fill[2][4][2] = {{{1024, 2048}, {1024, 2048}, {256, 1024}, {256, 512}},
+                                    {{512, 1024}, {512, 1024}, {512, 512}, {256, 512}}};
+  const int* f = fill[bf16][d <= 16 ? 0 : d <= 32 ? 1 : d <= 64 ? 2 : 3];
+  if (bh >= f[0]) return 1;
+  const long want = (f[1] + bh - 1) / bh, most = T / (d <= 32 ? 64 : 2 * d);
   const long n = want < most ? want : most;
   return n < 1 ? 1 : (int)n;
 }
@@ -686,9 +694,9 @@ const char* walk_check(int B, int T, int H, int dk, int dv, int dtype) {
 }  // namespace
 
 // Floats of workspace a walk of this shape needs.
-NOISE_EXPORT long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv) {
-  if (walk_check(B, T, H, dk, dv, NOISE_F32)) return 0;
-  const int n = walk_segments((long)B * H, T, dk > dv ? dk : dv);
+NOISE_EXPORT long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv, int dtype) {
+  if (walk_check(B, T, H, dk, dv, dtype)) return 0;
+  const int n = walk_segments((long)B * H, T, dk > dv ? dk : dv, dtype == NOISE_BF16);
   return n > 1 ? (long)B * H * n * dk * dv : 0;
 }
 
@@ -711,7 +719,7 @@ NOISE_EXPORT int noise_decay_attn_walk(const void* a, const void* k, const void*
   w.s_o = s_o, w.s_kv = s_kv;
   w.B = B, w.T = T, w.H = H, w.dk = dk, w.dv = dv;
   w.reverse = reverse, w.shift = reverse, w.end_decay = reverse, w.seg_tr = reuse;
-  w.nseg = walk_segments((long)B * H, T, dk > dv ? dk : dv);
+  w.nseg = walk_segments((long)B * H, T, dk > dv ? dk : dv, dtype == NOISE_BF16);
   w.seg_len = (noise_cdiv(T, w.nseg) + DB_C - 1) / DB_C * DB_C;
   w.nseg = noise_cdiv(T, w.seg_len);
   NOISE_REQUIRE(w.nseg == 1 || workspace, "noise_decay_attn_walk: this shape needs a workspace");

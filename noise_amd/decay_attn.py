@@ -27,7 +27,7 @@ from ._lib import _F, _I, _L, _P, ptr
 _lib.register({
     "noise_decay_attn_walk": [_P] * 8 + [_I, _P, _P, _F, _F] + [_I] * 8 + [_P],
     "noise_decay_attn_step": [_P] * 7 + [_F] + [_I] * 5 + [_P],
-    "noise_decay_attn_workspace": [_I] * 5,
+    "noise_decay_attn_workspace": [_I] * 6,
 })
 _lib.lib.noise_decay_attn_workspace.restype = _L
 
@@ -77,7 +77,7 @@ def _walk(a, k, v, log_decay, lengths, x0, x0_transposed, x_end, s_o, s_kv, reve
     dv = v.shape[-1]
     a, k, v = _unit(a), _unit(k), _unit(v)
     o = torch.empty(B, T, H, dv, device=a.device, dtype=a.dtype)
-    n = _lib.lib.noise_decay_attn_workspace(B, T, H, dk, dv)
+    n = _lib.lib.noise_decay_attn_workspace(B, T, H, dk, dv, _lib.DTYPES[a.dtype])
     ws = swapped if swapped is not None else torch.empty(n, device=a.device, dtype=torch.float32) if n else None
     strides = (_L * 12)(*a.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3])
     _lib.call("noise_decay_attn_walk", ptr(a), ptr(k), ptr(v), ptr(o), strides, ptr(log_decay), ptr(lengths), ptr(x0),
