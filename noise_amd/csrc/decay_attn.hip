@@ -40,24 +40,21 @@ struct WalkArgs {
   int B, T, H, dk, dv, nseg, seg_len;
   int reverse, shift, end_decay, x0_tr;
   int seg_tr;               // seg holds the states of the walk with k and v swapped, [dv][dk] each: nothing to sum
-  int va, vk, vv, vo;       // rows allow wide accesses: rows_buffer for bf16, four elements at a time otherwise
+  int va, vk, vv, vo;       // rows allow wide accesses: rows_buffer for 16-bit types, four elements at a time for fp32
 };
 
 __device__ __forceinline__ float decay_pow(float g2, int n) { return n <= 0 ? 1.f : exp2f(g2 * (float)n); }
 
 // Four elements of a token row, zero outside the row's width or behind the clip's end.
-template <typename T>
-__device__ __forceinline__ f32x4 row4(const T* base, bool live, int c, int width, bool vec) {
+__device__ __forceinline__ f32x4 row4(const float* base, bool live, int c, int width, bool vec) {
   f32x4 r = {0.f, 0.f, 0.f, 0.f};
   if (!live) return r;
   if (vec && c + 4 <= width) {
-    float t[4];
-    load_vec<T, 4>(base + c, t);
-    r = f32x4{t[0], t[1], t[2], t[3]};
+    r = *reinterpret_cast<const f32x4*>(base + c);
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (c + i < width) r[i] = (float)base[c + i];
+      if (c + i < width) r[i] = base[c + i];
   }
   return r;
 }
@@ -67,7 +64,7 @@ __device__ __forceinline__ f32x4 row4(const T* base, bool live, int c, int width
 // lane quarter q takes elements 4q..4q+3 of a 16-wide block over four consecutive instructions, so row-major operands are
 // 16-byte LDS reads and an accumulator tile (row 4q + r in register r) is the next product's operand as it lies: the state
 // never leaves its registers.  Only the C x C weights pass through LDS (each wave computes a share of them).
-template <typename T, int P, bool STATE_ONLY>
+template <int P, bool STATE_ONLY>
 __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_f32_kernel(WalkArgs w) {
   constexpr int NW = P >= 64 ? 4 : P / 16, NT = P / 16 / NW, KT = P / 16, NTHR = NW * 64;
   constexpr int LD = P + 4, LDP = DA_C + 4, SLOTS = DA_C * P / 4 / NTHR;
@@ -81,18 +78,18 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
   const int len = w.lengths ? min(max(w.lengths[b], 0), w.T) : w.T;
   const int p0 = seg * w.seg_len, p1 = min(p0 + w.seg_len, len);
   const int last_seg = len > 0 ? (len - 1) / w.seg_len : 0;
-  T* ob = (T*)w.o + (size_t)b * w.so.b + (size_t)h * w.so.h;
+  float* ob = (float*)w.o + (size_t)b * w.so.b + (size_t)h * w.so.h;
   if (!STATE_ONLY) {
     // rows behind the clip's end are zero
     const int t0 = max(len, p0), t1 = min(p0 + w.seg_len, w.T);
-    for (long i = (long)tid; i < (long)(t1 - t0) * w.dv; i += NTHR) ob[(t0 + i / w.dv) * w.so.t + i % w.dv] = (T)0.f;
+    for (long i = (long)tid; i < (long)(t1 - t0) * w.dv; i += NTHR) ob[(t0 + i / w.dv) * w.so.t + i % w.dv] = 0.f;
   }
   if (STATE_ONLY ? seg >= last_seg : seg > last_seg) return;
   const float g2 = w.log_decay[h] * 1.44269504088896341f;
   if (tid <= DA_C) pw[tid] = decay_pow(g2, tid);
-  const T* ab = (const T*)w.a + (size_t)b * w.sa.b + (size_t)h * w.sa.h;
-  const T* kb = (const T*)w.k + (size_t)b * w.sk.b + (size_t)h * w.sk.h;
-  const T* vb = (const T*)w.v + (size_t)b * w.sv.b + (size_t)h * w.sv.h;
+  const float* ab = (const float*)w.a + (size_t)b * w.sa.b + (size_t)h * w.sa.h;
+  const float* kb = (const float*)w.k + (size_t)b * w.sk.b + (size_t)h * w.sk.h;
+  const float* vb = (const float*)w.v + (size_t)b * w.sv.b + (size_t)h * w.sv.h;
 
   // ---- state before the segment
   f32x4 X[KT][NT];
@@ -233,7 +230,7 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const int col = (wave * NT + nt) * 16 + l16;
-            if (col < w.dv) ob[t * w.so.t + col] = (T)O[mt][nt][r];
+            if (col < w.dv) ob[t * w.so.t + col] = O[mt][nt][r];
           }
         }
     }
@@ -253,11 +250,14 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
       }
 }
 
-// bf16 tokens on the bf16 matrix cores (v_mfma_f32_16x16x32_bf16), 64 tokens per chunk, P / 16 waves that own 16 state
-// columns each.  What is rounded to bf16 on its way into a product, and what is not:
+// 16-bit tokens on the 16-bit matrix cores (v_mfma_f32_16x16x32_bf16 / _f16), 64 tokens per chunk, P / 16 waves that own 16
+// state columns each.  What is rounded to 16 bits on its way into a product, and what is not:
 //   * the weights lam^{i-j} (a_i . k_j) and the state as it meets a_i: once each, like the output they lead to;
-//   * lam^{n-1-j} v_j on its way into the state is split into three bf16 terms (24 bits), since the state is fp32, carried
-//     over any number of chunks and returned: X keeps fp32 accuracy at three products per term.
+//   * lam^{n-1-j} v_j on its way into the state is split into three terms of the type (24 bits), since the state is fp32,
+//     carried over any number of chunks and returned: X keeps fp32 accuracy at three products per term.
+// fp16 has the fraction for that but not the range, so those three operands go in scaled by powers of two that bounds give
+// (dk max|a| max|k| for the weights, max|v| for the split values, and for the state the recurrence of the bound itself); X is
+// kept in the units of the last chunk's values.  The bounds may be far too large: fp16 stays normal over 2^29.
 // Operands: lane (q = lane / 16, l = lane % 16) of an MFMA takes eight contraction indices 8q..8q+7 of row l, and an
 // accumulator tile holds rows 4q + r of column l.  Two state tiles whose rows are dealt as 8q + 4s + r (s = tile) together
 // are the eight indices the next product wants, so the state stays in registers.  Contractions over tokens read K and V
@@ -268,69 +268,93 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
 // 32) halve the registers of a wave and put four waves on a SIMD, at twice the LDS reads of a and K.
 constexpr int DB_C = 64;
 
-using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
-using bf16x4 = __attribute__((ext_vector_type(4))) __bf16;
+template <typename T>
+using x8 = __attribute__((ext_vector_type(8))) T;
+template <typename T>
+using x2 = __attribute__((ext_vector_type(2))) T;
+using u16x2 = __attribute__((ext_vector_type(2))) unsigned short;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
 using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
 using u32x2 = __attribute__((ext_vector_type(2))) unsigned;
 
-__device__ __forceinline__ u32x4 row8(const bf16_t* base, bool live, int c, int width, bool vec) {
+template <typename T>
+__device__ __forceinline__ u32x4 row8(const T* base, bool live, int c, int width, bool vec) {
   u32x4 r = {0u, 0u, 0u, 0u};
   if (!live) return r;
   if (vec && c + 8 <= width) return *reinterpret_cast<const u32x4*>(base + c);
-  bf16x8 t;
+  x8<T> t;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = c + i < width ? base[c + i] : (bf16_t)0.f;
+  for (int i = 0; i < 8; ++i) t[i] = c + i < width ? base[c + i] : (T)0.f;
   return __builtin_bit_cast(u32x4, t);
 }
 
 // Eight tokens (rows 8q .. 8q + 7 behind `tile`) of column l of the 16 columns that start there.
-template <int LD>
-__device__ __forceinline__ bf16x8 read_tokens(const bf16_t* tile, int q, int l16) {
+template <int LD, typename T>
+__device__ __forceinline__ x8<T> read_tokens(const T* tile, int q, int l16) {
   using lds4 = __attribute__((address_space(3))) s16x4;
-  const bf16_t* p = tile + (8 * q + l16 / 4) * LD + l16 % 4 * 4;
+  const T* p = tile + (8 * q + l16 / 4) * LD + l16 % 4 * 4;
   const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
   const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * LD));
-  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+  return __builtin_bit_cast(x8<T>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-__device__ __forceinline__ float low_bf16(unsigned u) { return __uint_as_float(u << 16); }
-__device__ __forceinline__ float high_bf16(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
-__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
-  const __attribute__((ext_vector_type(2))) __bf16 v = {(bf16_t)a, (bf16_t)b};
+// The two halves of a register as floats, two floats rounded into one, and the product.
+template <typename T>
+__device__ __forceinline__ float low16(unsigned u) {
+  if constexpr (__is_same(T, bf16_t)) return __uint_as_float(u << 16);
+  else return (float)__builtin_bit_cast(x2<f16_t>, u)[0];
+}
+template <typename T>
+__device__ __forceinline__ float high16(unsigned u) {
+  if constexpr (__is_same(T, bf16_t)) return __uint_as_float(u & 0xffff0000u);
+  else return (float)__builtin_bit_cast(x2<f16_t>, u)[1];
+}
+template <typename T>
+__device__ __forceinline__ unsigned pack16(float a, float b) {
+  const x2<T> v = {(T)a, (T)b};
   return __builtin_bit_cast(unsigned, v);
 }
+__device__ __forceinline__ f32x4 mfma16(x8<bf16_t> a, x8<bf16_t> b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mfma16(x8<f16_t> a, x8<f16_t> b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// Largest magnitude among the fp16 values of a register, as bits (their order is the integers').
+__device__ __forceinline__ u16x2 abs_max16(u16x2 m, unsigned u) { return __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, u & 0x7fff7fffu)); }
+__device__ __forceinline__ float pow2(int e) { return ldexpf(1.f, e); }
+// The exponent that brings a bound below 2^top; a bound of zero, infinity or NaN gives a harmless one.
+__device__ __forceinline__ int scale_for(float bound, int top) { return max(min(top - __builtin_amdgcn_frexp_expf(bound), 60), -60); }
 
 // Rows of a chunk as a buffer: accesses behind its end read zero and store nothing, so that neither the clip's last chunk nor
 // columns behind the head need a branch.  `rows` of them, `stride` elements apart, `width` elements each.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_rows(const bf16_t* first, int rows, long stride, int width) {
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_rows(const void* first, int rows, long stride, int width) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)first, 0, (int)(((rows - 1) * stride + width) * 2), 0x00020000);
 }
 // A byte offset into such a buffer; one before its start, or of a column that does not exist, lands far behind its end.
 __device__ __forceinline__ int chunk_offset(int off, bool exists) { return (int)min((unsigned)(exists ? off : -1), 0x80000000u); }
 
 // VEC: every row of a, k, v and o starts on a 16-byte boundary, rows do not overlap and a chunk spans less than 2 GB.
-template <int P, bool STATE_ONLY, bool VEC>
-__global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_bf16_kernel(WalkArgs w) {
+template <typename T, int P, bool STATE_ONLY, bool VEC>
+__global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkArgs w) {
+  constexpr bool F16 = __is_same(T, f16_t);
   constexpr int NTHR = P * 4, NW = P / 16, KP = P / 32;      // KP: pairs of state row tiles
   constexpr int LD = P + 16, LDP = DB_C + 8, SLOTS = DB_C * P / 8 / NTHR;
-  __shared__ __attribute__((aligned(16))) bf16_t sa[STATE_ONLY ? 8 : DB_C * LD];
-  __shared__ __attribute__((aligned(16))) bf16_t sk[DB_C * LD], sv[DB_C * LD];
-  __shared__ __attribute__((aligned(16))) bf16_t sp[STATE_ONLY ? 8 : DB_C * LDP];
+  __shared__ __attribute__((aligned(16))) T sa[STATE_ONLY ? 8 : DB_C * LD];
+  __shared__ __attribute__((aligned(16))) T sk[DB_C * LD], sv[DB_C * LD];
+  __shared__ __attribute__((aligned(16))) T sp[STATE_ONLY ? 8 : DB_C * LDP];
   __shared__ float pw[DB_C + 1];                             // lam^i
   __shared__ float pv[2 * DB_C];                             // s_kv lam^{63-i}; a chunk of n tokens starts at 64 - n
   __shared__ float pp[DB_C + 16];                            // [15 + i - j]: s_o s_kv lam^{i-j}
+  __shared__ unsigned top[F16 ? 3 * NW : 1];                 // largest a, k, v of the waves' pieces, as bits
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, q = lane >> 4, l16 = lane & 15;
   const int bh = blockIdx.x % (w.B * w.H), seg = blockIdx.x / (w.B * w.H);
   const int b = bh / w.H, h = bh % w.H;
   const int len = w.lengths ? min(max(w.lengths[b], 0), w.T) : w.T;
   const int p0 = seg * w.seg_len, p1 = min(p0 + w.seg_len, len);
   const int last_seg = len > 0 ? (len - 1) / w.seg_len : 0;
-  bf16_t* ob = (bf16_t*)w.o + (size_t)b * w.so.b + (size_t)h * w.so.h;
+  T* ob = (T*)w.o + (size_t)b * w.so.b + (size_t)h * w.so.h;
   if (!STATE_ONLY) {
     // rows behind the clip's end are zero
     const int t0 = max(len, p0), t1 = min(p0 + w.seg_len, w.T);
-    for (long i = (long)tid; i < (long)(t1 - t0) * w.dv; i += NTHR) ob[(t0 + i / w.dv) * w.so.t + i % w.dv] = (bf16_t)0.f;
+    for (long i = (long)tid; i < (long)(t1 - t0) * w.dv; i += NTHR) ob[(t0 + i / w.dv) * w.so.t + i % w.dv] = (T)0.f;
   }
   if (STATE_ONLY ? seg >= last_seg : seg > last_seg) return;
   const float g2 = w.log_decay[h] * 1.44269504088896341f;
@@ -343,12 +367,12 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_bf16_kernel(Walk
     // the weight tiles (0, 1) and (2, 3) lie above the diagonal but in a pair that is read: they stay zero
     for (int i = tid; i < 32 * 16; i += NTHR) {
       const int half = i >> 8, r = i >> 4 & 15, c = i & 15;
-      sp[(half * 32 + r) * LDP + half * 32 + 16 + c] = (bf16_t)0.f;
+      sp[(half * 32 + r) * LDP + half * 32 + 16 + c] = (T)0.f;
     }
   }
-  const bf16_t* ab = (const bf16_t*)w.a + (size_t)b * w.sa.b + (size_t)h * w.sa.h;
-  const bf16_t* kb = (const bf16_t*)w.k + (size_t)b * w.sk.b + (size_t)h * w.sk.h;
-  const bf16_t* vb = (const bf16_t*)w.v + (size_t)b * w.sv.b + (size_t)h * w.sv.h;
+  const T* ab = (const T*)w.a + (size_t)b * w.sa.b + (size_t)h * w.sa.h;
+  const T* kb = (const T*)w.k + (size_t)b * w.sk.b + (size_t)h * w.sk.h;
+  const T* vb = (const T*)w.v + (size_t)b * w.sv.b + (size_t)h * w.sv.h;
   const int col0 = wave * 16;                                // the wave's state columns
 
   // X[kp][s][r]: row kp 32 + 8q + 4s + r, column col0 + l
@@ -371,12 +395,24 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_bf16_kernel(Walk
         }
   }
 
+  int E = 0;            // fp16: X is held times 2^E
+  float bound = 0.f;    // fp16: no element of X is larger
+  if constexpr (F16) {
+#pragma unroll
+    for (int kp = 0; kp < KP; ++kp)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) bound = fmaxf(bound, fabsf(X[kp][s][r]));
+    bound = wave_reduce_max(bound);
+  }
+
   // a thread's SLOTS pieces of a tile are RS rows apart, in the same column
   constexpr int RS = NTHR / (P / 8);
   const int i0 = tid / (P / 8), cc = tid % (P / 8) * 8;
   const int dir = w.reverse ? -1 : 1;
   u32x4 ra[STATE_ONLY ? 1 : SLOTS], rk[SLOTS], rv[SLOTS];
-  auto rows8 = [&](const bf16_t* base, const Strides& st, int width, bool vec, int c0, u32x4 (&out)[SLOTS]) {
+  auto rows8 = [&](const T* base, const Strides& st, int width, bool vec, int c0, u32x4 (&out)[SLOTS]) {
     const int n = min(DB_C, p1 - c0);
     if (VEC) {
       const auto rs = chunk_rows(base + (w.reverse ? len - c0 - n : c0) * st.t, n, st.t, width);
@@ -407,18 +443,56 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_bf16_kernel(Walk
     for (int s = 0; s < SLOTS; ++s) {
       const int at = (i0 + s * RS) * LD + cc;
       if (!STATE_ONLY) *(u32x4*)(sa + at) = ra[s];
-      bf16_t* kd = sk + (i0 + s * RS) * LD + cc / 32 * 32 + cc % 32 / 2;
+      T* kd = sk + (i0 + s * RS) * LD + cc / 32 * 32 + cc % 32 / 2;
       *(uint2*)kd = make_uint2(rk[s][0], rk[s][1]);
       *(uint2*)(kd + 16) = make_uint2(rk[s][2], rk[s][3]);
       *(u32x4*)(sv + at) = rv[s];
     }
+    if constexpr (F16) {
+      u16x2 m[3] = {};
+#pragma unroll
+      for (int s = 0; s < SLOTS; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (!STATE_ONLY) m[0] = abs_max16(m[0], ra[s][e]);
+          m[1] = abs_max16(m[1], rk[s][e]);
+          m[2] = abs_max16(m[2], rv[s][e]);
+        }
+#pragma unroll
+      for (int z = STATE_ONLY ? 1 : 0; z < 3; ++z) {
+        unsigned u = max(m[z][0], m[z][1]);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) u = max(u, (unsigned)__shfl_xor((int)u, o, 64));
+        if (lane == 0) top[z * NW + wave] = u;
+      }
+    }
     __syncthreads();
     if (c0 + DB_C < p1) fetch(c0 + DB_C);
+    float unit_p = 1.f, unit_x = 1.f, back = 1.f, unit_v = 1.f, carry = 1.f, largest = 0.f;
+    if constexpr (F16) {
+      float big[3];
+#pragma unroll
+      for (int z = 0; z < 3; ++z) {
+        unsigned u = 0;
+#pragma unroll
+        for (int i = 0; i < NW; ++i) u = max(u, STATE_ONLY && z == 0 ? 0u : top[z * NW + i]);
+        big[z] = (float)__builtin_bit_cast(f16_t, (unsigned short)u);
+      }
+      const int ep = scale_for((float)P * fabsf(w.s_o * w.s_kv) * big[0] * big[1], 15), ev = scale_for(fabsf(w.s_kv) * big[2], 15);
+      const int ex = scale_for(bound, 14);
+      unit_p = pow2(ep);                // weights
+      unit_x = pow2(ex - E);            // X as an operand
+      back = pow2(ep - ex);             // its product, in the weights' units
+      unit_v = pow2(ev);                // values on their way into X
+      carry = pow2(ev - E);
+      E = ev;
+      largest = fabsf(w.s_kv) * big[1] * big[2] * (float)n;
+    }
     f32x4 O[STATE_ONLY ? 1 : 4];
     if (!STATE_ONLY) {
       // ---- weights, transposed tile by tile (rows j, columns i) so that a lane holds four neighbouring j of one i: the ten
       // 16 x 16 tiles on and below the diagonal, in the order (0,0) (1,0) (1,1) (2,0) ..., are dealt over the waves
-#pragma unroll(P == 128 ? 1 : 5)   // eight waves have two tiles at most, and no registers for both at once
+#pragma unroll P == 128 ? 1 : 5   // eight waves have two tiles at most, and no registers for both at once
       for (int u = 0; u * NW < 10; ++u) {
         const int tile = u * NW + wave;
         if ((u + 1) * NW > 10 && tile >= 10) break;
@@ -426,17 +500,17 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_bf16_kernel(Walk
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kp = 0; kp < KP; ++kp) {
-          const bf16_t* kr = sk + (jt * 16 + l16) * LD + kp * 32 + 4 * q;
+          const T* kr = sk + (jt * 16 + l16) * LD + kp * 32 + 4 * q;
           const uint2 k0 = *(const uint2*)kr, k1 = *(const uint2*)(kr + 16);
-          const bf16x8 x = __builtin_bit_cast(bf16x8, u32x4{k0.x, k0.y, k1.x, k1.y});
-          const bf16x8 y = *(const bf16x8*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
-          acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0);
+          const x8<T> x = __builtin_bit_cast(x8<T>, u32x4{k0.x, k0.y, k1.x, k1.y});
+          const x8<T> y = *(const x8<T>*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
+          acc = mfma16(x, y, acc);
         }
         const int i = it * 16 + l16, j = jt * 16 + 4 * q;
         const bool diag = it == jt;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[r] = diag && l16 < 4 * q + r ? 0.f : acc[r] * pp[15 + i - j - r];
-        *(uint2*)(sp + i * LDP + j) = make_uint2(pack_bf16(acc[0], acc[1]), pack_bf16(acc[2], acc[3]));
+        for (int r = 0; r < 4; ++r) acc[r] = diag && l16 < 4 * q + r ? 0.f : acc[r] * (F16 ? unit_p * pp[15 + i - j - r] : pp[15 + i - j - r]);
+        *(uint2*)(sp + i * LDP + j) = make_uint2(pack16<T>(acc[0], acc[1]), pack16<T>(acc[2], acc[3]));
       }
       // ---- what the state contributes, transposed: rows are the wave's columns, columns the tokens
 #pragma unroll
@@ -445,49 +519,55 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_bf16_kernel(Walk
       for (int kp = 0; kp < KP; ++kp) {
         u32x4 u;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) u[e] = pack_bf16(X[kp][e >> 1][2 * (e & 1)], X[kp][e >> 1][2 * (e & 1) + 1]);
-        const bf16x8 x = __builtin_bit_cast(bf16x8, u);
+        for (int e = 0; e < 4; ++e) {
+          const float x0 = X[kp][e >> 1][2 * (e & 1)], x1 = X[kp][e >> 1][2 * (e & 1) + 1];
+          u[e] = F16 ? pack16<T>(x0 * unit_x, x1 * unit_x) : pack16<T>(x0, x1);
+        }
+        const x8<T> x = __builtin_bit_cast(x8<T>, u);
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
-          const bf16x8 y = *(const bf16x8*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
-          O[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, O[it], 0, 0, 0);
+          const x8<T> y = *(const x8<T>*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
+          O[it] = mfma16(x, y, O[it]);
         }
       }
 #pragma unroll
-      for (int it = 0; it < 4; ++it) O[it] *= w.s_o * pw[it * 16 + l16 + 1 - shift];
+      for (int it = 0; it < 4; ++it) O[it] *= w.s_o * pw[it * 16 + l16 + 1 - shift] * back;
     }
     // ---- X = lam^n X + K^T V'
-    bf16x8 v[2];
-    const float f = pw[n - shift];
+    x8<T> v[2];
+    const float f = pw[n - shift] * carry;
+    if constexpr (F16) bound = bound * pw[n - shift] + largest;
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp)
 #pragma unroll
       for (int s = 0; s < 2; ++s) X[kp][s] *= f;
 #pragma unroll
     for (int jj = 0; jj < 2; ++jj) {
-      v[jj] = read_tokens<LD>(sv + jj * 32 * LD + col0, q, l16);
+      v[jj] = read_tokens<LD, T>(sv + jj * 32 * LD + col0, q, l16);
       u32x4 t[3];
       const float* f8 = pv + DB_C - n + jj * 32 + 8 * q;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const unsigned u = __builtin_bit_cast(u32x4, v[jj])[e];
-        float y0 = low_bf16(u) * f8[2 * e], y1 = high_bf16(u) * f8[2 * e + 1];
+        float y0 = low16<T>(u) * (F16 ? unit_v * f8[2 * e] : f8[2 * e]), y1 = high16<T>(u) * (F16 ? unit_v * f8[2 * e + 1] : f8[2 * e + 1]);
+        // the compiler may round the exact product, not y, to fp16 in one of the two places that read the first term, and the
+        // terms would then not add up: y is fixed before it is split
+        if constexpr (F16) asm("" : "+v"(y0), "+v"(y1));
 #pragma unroll
         for (int z = 0; z < 3; ++z) {
-          const unsigned c = pack_bf16(y0, y1);
+          const unsigned c = pack16<T>(y0, y1);
           t[z][e] = c;
-          y0 -= low_bf16(c);
-          y1 -= high_bf16(c);
+          y0 -= low16<T>(c);
+          y1 -= high16<T>(c);
         }
       }
 #pragma unroll
       for (int kp = 0; kp < KP; ++kp)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          const bf16x8 x = read_tokens<LD>(sk + jj * 32 * LD + kp * 32 + 16 * s, q, l16);
+          const x8<T> x = read_tokens<LD, T>(sk + jj * 32 * LD + kp * 32 + 16 * s, q, l16);
 #pragma unroll
-          for (int z = 2; z >= 0; --z)
-            X[kp][s] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, __builtin_bit_cast(bf16x8, t[z]), X[kp][s], 0, 0, 0);
+          for (int z = 2; z >= 0; --z) X[kp][s] = mfma16(x, __builtin_bit_cast(x8<T>, t[z]), X[kp][s]);
         }
     }
     // every wave is done with the tiles and has left its weights: the next chunk's tiles may be written from here on, its
@@ -499,21 +579,22 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_bf16_kernel(Walk
       for (int jj = 0; jj < 2; ++jj)
 #pragma unroll
         for (int it = 2 * jj; it < 4; ++it) {
-          const bf16x8 y = *(const bf16x8*)(sp + (it * 16 + l16) * LDP + jj * 32 + 8 * q);
-          O[it] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[jj], y, O[it], 0, 0, 0);
+          const x8<T> y = *(const x8<T>*)(sp + (it * 16 + l16) * LDP + jj * 32 + 8 * q);
+          O[it] = mfma16(v[jj], y, O[it]);
         }
       const int col = col0 + 4 * q;
       const auto rs = chunk_rows(ob + (w.reverse ? len - c0 - n : c0) * w.so.t, n, w.so.t, w.dv);
 #pragma unroll
       for (int it = 0; it < 4; ++it) {
         const int i = it * 16 + l16;
-        const u32x2 y = {pack_bf16(O[it][0], O[it][1]), pack_bf16(O[it][2], O[it][3])};
+        if constexpr (F16) O[it] *= 1.f / unit_p;
+        const u32x2 y = {pack16<T>(O[it][0], O[it][1]), pack16<T>(O[it][2], O[it][3])};
         const int row = w.reverse ? n - 1 - i : i;
         if (VEC) {
           __builtin_amdgcn_raw_buffer_store_b64(y, rs, chunk_offset(row * 2 * (int)w.so.t + 2 * col, col < w.dv), 0, 0);
         } else if (i < n) {
-          bf16_t* op = ob + ((w.reverse ? len - c0 - n : c0) + row) * w.so.t + col;
-          const bf16x4 z = __builtin_bit_cast(bf16x4, y);
+          T* op = ob + ((w.reverse ? len - c0 - n : c0) + row) * w.so.t + col;
+          const auto z = __builtin_bit_cast(typename VecOf<T, 4>::type, y);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (col + e < w.dv) op[e] = z[e];
@@ -524,7 +605,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_bf16_kernel(Walk
   // ---- state behind the segment
   float* dst = STATE_ONLY ? w.seg + ((size_t)bh * w.nseg + seg) * mat : seg == last_seg && w.x_end ? w.x_end + (size_t)bh * mat : nullptr;
   if (!dst) return;
-  const float f = !STATE_ONLY && w.end_decay && len > 0 ? pw[1] : 1.f;
+  const float f = (!STATE_ONLY && w.end_decay && len > 0 ? pw[1] : 1.f) * (F16 ? pow2(-E) : 1.f);
 #pragma unroll
   for (int kp = 0; kp < KP; ++kp)
 #pragma unroll
@@ -612,7 +693,7 @@ __global__ __launch_bounds__(256) void step_kernel(const T* __restrict__ q, Stri
 bool rows_vec(const void* p, const Strides& s, int v, int esize) {
   return ((uintptr_t)p % (v * esize)) == 0 && s.b % v == 0 && s.t % v == 0 && s.h % v == 0;
 }
-// ... and as a piece of a chunk's buffer (bf16 kernels): whole pieces, rows apart, offsets below 2^31 bytes.
+// ... and as a piece of a chunk's buffer (16-bit kernels): whole pieces, rows apart, offsets below 2^31 bytes.
 bool rows_buffer(const void* p, const Strides& s, int width) {
   return rows_vec(p, s, 8, 2) && width % 8 == 0 && s.t >= width && s.t < (1L << 23);
 }
@@ -621,18 +702,14 @@ void scan_launch(const WalkArgs& w, hipStream_t st) {
   hipLaunchKernelGGL(walk_scan_kernel, dim3(noise_cdiv((long)w.dk * w.dv, 256), w.B * w.H), dim3(256), 0, st, w);
 }
 
-void walk_launch_bf16(const WalkArgs& w, hipStream_t st) {
+void walk_launch_f32(const WalkArgs& w, hipStream_t st) {
   const int d = w.dk > w.dv ? w.dk : w.dv;
   const unsigned grid = (unsigned)w.B * w.H * w.nseg;
-  const bool vec = w.va && w.vk && w.vv && w.vo;
-#define GO(P, ONLY)                                                                                        \
-  do {                                                                                                     \
-    if (vec) hipLaunchKernelGGL((walk_bf16_kernel<P, ONLY, true>), dim3(grid), dim3(P * 4), 0, st, w);     \
-    else hipLaunchKernelGGL((walk_bf16_kernel<P, ONLY, false>), dim3(grid), dim3(P * 4), 0, st, w);        \
-  } while (0)
+#define GO(P, ONLY) hipLaunchKernelGGL((walk_f32_kernel<P, ONLY>), dim3(grid), dim3(P >= 64 ? 256 : P * 4), 0, st, w)
 #define PICK(ONLY)             \
   do {                         \
-    if (d <= 32) GO(32, ONLY); \
+    if (d <= 16) GO(16, ONLY); \
+    else if (d <= 32) GO(32, ONLY); \
     else if (d <= 64) GO(64, ONLY); \
     else GO(128, ONLY);        \
   } while (0)
@@ -646,14 +723,18 @@ void walk_launch_bf16(const WalkArgs& w, hipStream_t st) {
 }
 
 template <typename T>
-void walk_launch(const WalkArgs& w, hipStream_t st) {
+void walk_launch_16(const WalkArgs& w, hipStream_t st) {
   const int d = w.dk > w.dv ? w.dk : w.dv;
   const unsigned grid = (unsigned)w.B * w.H * w.nseg;
-#define GO(P, ONLY) hipLaunchKernelGGL((walk_f32_kernel<T, P, ONLY>), dim3(grid), dim3(P >= 64 ? 256 : P * 4), 0, st, w)
+  const bool vec = w.va && w.vk && w.vv && w.vo;
+#define GO(P, ONLY)                                                                                         \
+  do {                                                                                                      \
+    if (vec) hipLaunchKernelGGL((walk_16_kernel<T, P, ONLY, true>), dim3(grid), dim3(P * 4), 0, st, w);     \
+    else hipLaunchKernelGGL((walk_16_kernel<T, P, ONLY, false>), dim3(grid), dim3(P * 4), 0, st, w);        \
+  } while (0)
 #define PICK(ONLY)             \
   do {                         \
-    if (d <= 16) GO(16, ONLY); \
-    else if (d <= 32) GO(32, ONLY); \
+    if (d <= 32) GO(32, ONLY); \
     else if (d <= 64) GO(64, ONLY); \
     else GO(128, ONLY);        \
   } while (0)
@@ -673,10 +754,10 @@ void walk_launch(const WalkArgs& w, hipStream_t st) {
 // pairs 133 / 186 / 198 / 234, 128 pairs 92 / 73 / 60 / 61; heads of 32: 512 pairs 93 / 106 / 122 / 130, 128 pairs 82 / 62 / 44 /
 // 42; fp32, heads of 128: 256 pairs 489 / 554 / 568 / 641, heads of 16: 1024 pairs 183 / 205 / 239 / 246, 256 pairs 159 / 112 / 69 / 70.
 // No segment is shorter than 64 tokens or than twice the head: its state is written, scanned and read again.
-int walk_segments(long bh, int T, int d, bool bf16) {
+int walk_segments(long bh, int T, int d, bool half) {
   static const int fill[2][4][2] = {{{1024, 2048}, {1024, 2048}, {256, 1024}, {256, 512}},
                                     {{512, 1024}, {512, 1024}, {512, 512}, {256, 512}}};
-  const int* f = fill[bf16][d <= 16 ? 0 : d <= 32 ? 1 : d <= 64 ? 2 : 3];
+  const int* f = fill[half][d <= 16 ? 0 : d <= 32 ? 1 : d <= 64 ? 2 : 3];
   if (bh >= f[0]) return 1;
   const long want = (f[1] + bh - 1) / bh, most = T / (d <= 32 ? 64 : 2 * d);
   const long n = want < most ? want : most;
@@ -696,7 +777,7 @@ const char* walk_check(int B, int T, int H, int dk, int dv, int dtype) {
 // Floats of workspace a walk of this shape needs.
 NOISE_EXPORT long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv, int dtype) {
   if (walk_check(B, T, H, dk, dv, dtype)) return 0;
-  const int n = walk_segments((long)B * H, T, dk > dv ? dk : dv, dtype == NOISE_BF16);
+  const int n = walk_segments((long)B * H, T, dk > dv ? dk : dv, dtype != NOISE_F32);
   return n > 1 ? (long)B * H * n * dk * dv : 0;
 }
 
@@ -719,20 +800,19 @@ NOISE_EXPORT int noise_decay_attn_walk(const void* a, const void* k, const void*
   w.s_o = s_o, w.s_kv = s_kv;
   w.B = B, w.T = T, w.H = H, w.dk = dk, w.dv = dv;
   w.reverse = reverse, w.shift = reverse, w.end_decay = reverse, w.seg_tr = reuse;
-  w.nseg = walk_segments((long)B * H, T, dk > dv ? dk : dv, dtype == NOISE_BF16);
+  w.nseg = walk_segments((long)B * H, T, dk > dv ? dk : dv, dtype != NOISE_F32);
   w.seg_len = (noise_cdiv(T, w.nseg) + DB_C - 1) / DB_C * DB_C;
   w.nseg = noise_cdiv(T, w.seg_len);
   NOISE_REQUIRE(w.nseg == 1 || workspace, "noise_decay_attn_walk: this shape needs a workspace");
-  if (dtype == NOISE_BF16) {
-    w.va = rows_buffer(a, w.sa, dk), w.vk = rows_buffer(k, w.sk, dk), w.vv = rows_buffer(v, w.sv, dv), w.vo = rows_buffer(o, w.so, dv);
+  if (dtype == NOISE_F32) {
+    w.va = rows_vec(a, w.sa, 4, 4), w.vk = rows_vec(k, w.sk, 4, 4), w.vv = rows_vec(v, w.sv, 4, 4), w.vo = 0;
   } else {
-    const int es = dtype == NOISE_F32 ? 4 : 2;
-    w.va = rows_vec(a, w.sa, 4, es), w.vk = rows_vec(k, w.sk, 4, es), w.vv = rows_vec(v, w.sv, 4, es), w.vo = 0;
+    w.va = rows_buffer(a, w.sa, dk), w.vk = rows_buffer(k, w.sk, dk), w.vv = rows_buffer(v, w.sv, dv), w.vo = rows_buffer(o, w.so, dv);
   }
   hipStream_t st = (hipStream_t)stream;
-  if (dtype == NOISE_F32) walk_launch<float>(w, st);
-  else if (dtype == NOISE_BF16) walk_launch_bf16(w, st);
-  else walk_launch<f16_t>(w, st);
+  if (dtype == NOISE_F32) walk_launch_f32(w, st);
+  else if (dtype == NOISE_BF16) walk_launch_16<bf16_t>(w, st);
+  else walk_launch_16<f16_t>(w, st);
   NOISE_CHECK_LAUNCH("noise_decay_attn_walk");
   return 0;
 }

@@ -143,6 +143,26 @@ def test_padding_is_never_read(dtype):
     assert torch.equal(got["end"][1], c["state"][1]) and torch.equal(got["d_state"][1], c["d_state"][1])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("q,k,v,state,do", [(6, -8, 9, 14, -6), (-9, 7, -10, -30, -12), (5, 5, 0, 20, 0), (0, 0, -14, 0, 10), (7, 4, 12, -100, 3)])
+def test_magnitudes_far_from_one(q, k, v, state, do, dtype):
+    """Inputs scaled by powers of two up to the type's ends, and a piece of silence: the 16-bit operands inside carry their own
+    scales, so the error stays relative to the terms.  Results that leave the type's range are left out."""
+    c = make(2, 300, 2, 64, 40, dtype, 17)
+    for n, e in (("q", q), ("k", k), ("v", v), ("do", do)):
+        c[n] = (c[n].double() * 2.0 ** e).to(dtype)
+    c["v"][:, 70:200] = 0
+    c["state"], c["d_state"] = c["state"] * 2.0 ** state, c["d_state"] * 2.0 ** state
+    c["log_decay"] = torch.tensor([-0.02, 0.0], device=DEV)
+    got = run_all(c)
+    want, mag = recurrence(c, 64 ** -0.5), recurrence(c, 64 ** -0.5, True)
+    top = torch.finfo(dtype).max
+    for name, g in got.items():
+        fits = want[name].abs() < (0.9 * top if name in ("o", "dq", "dk", "dv") else float("inf"))
+        t = tolerance(name, want[name], mag[name], dtype, 300, 64, 40)
+        assert ((g.double() - want[name]).abs() <= t)[fits].all(), (name, ((g.double() - want[name]).abs() / t)[fits].max())
+
+
 def test_views_strides_and_orders():
     """Packed projections, a (B, H, T, D) layout, a sliced axis, a broadcast clip and a last axis with a stride: the numbers of
     packed copies."""
