@@ -41,13 +41,13 @@ def _unit(t):
 
 def _check(q, k, v, log_decay, state, tokens):
     _lib.require_cuda(q, k, v, log_decay, state)
-    dims = 4 if tokens else 3
-    if q.dim() != dims or k.shape != q.shape or v.dim() != dims or v.shape[:-1] != q.shape[:-1]:
+    qs, vs, dims = q.shape, v.shape, 4 if tokens else 3
+    if len(qs) != dims or k.shape != qs or len(vs) != dims or vs[:-1] != qs[:-1]:
         raise ValueError(f"q, k must be {'(B, T, H, Dk)' if tokens else '(B, H, Dk)'} and v the same with Dv: got {tuple(q.shape)}, "
                          f"{tuple(k.shape)}, {tuple(v.shape)}")
     if q.dtype not in _lib.DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"q, k, v must share one of float32, bfloat16, float16: got {q.dtype}, {k.dtype}, {v.dtype}")
-    B, H, dk, dv = q.shape[0], q.shape[-2], q.shape[-1], v.shape[-1]
+    B, H, dk, dv = qs[0], qs[-2], qs[-1], vs[-1]
     if not (1 <= dk <= MAX_HEAD and 1 <= dv <= MAX_HEAD):
         raise ValueError(f"head sizes of 1 to {MAX_HEAD} are supported, got {dk} and {dv}")
     if log_decay.shape != (H,) or log_decay.dtype != torch.float32:
@@ -57,7 +57,7 @@ def _check(q, k, v, log_decay, state, tokens):
 
 
 def _check_state(name, state, shape):
-    if state is not None and (tuple(state.shape) != shape or state.dtype != torch.float32):
+    if state is not None and (state.shape != shape or state.dtype != torch.float32):
         raise ValueError(f"{name} must be float32 {shape}, got {state.dtype} {tuple(state.shape)}")
 
 
@@ -76,10 +76,10 @@ def _walk(a, k, v, log_decay, lengths, x0, x0_transposed, x_end, s_o, s_kv, reve
     B, T, H, dk = a.shape
     dv = v.shape[-1]
     a, k, v = _unit(a), _unit(k), _unit(v)
-    o = torch.empty(B, T, H, dv, device=a.device, dtype=a.dtype)
+    o = a.new_empty(B, T, H, dv)
     n = _lib.lib.noise_decay_attn_workspace(B, T, H, dk, dv, _lib.DTYPES[a.dtype])
-    ws = swapped if swapped is not None else torch.empty(n, device=a.device, dtype=torch.float32) if n else None
-    strides = (_L * 12)(*a.stride()[:3], *k.stride()[:3], *v.stride()[:3], *o.stride()[:3])
+    ws = swapped if swapped is not None else a.new_empty(n, dtype=torch.float32) if n else None
+    strides = (_L * 12)(*a.stride()[:3], *k.stride()[:3], *v.stride()[:3], T * H * dv, H * dv, dv)
     _lib.call("noise_decay_attn_walk", ptr(a), ptr(k), ptr(v), ptr(o), strides, ptr(log_decay), ptr(lengths), ptr(x0),
               int(x0_transposed), ptr(x_end), ptr(ws), s_o, s_kv, int(reverse), int(swapped is not None), B, T, H, dk, dv, _lib.DTYPES[a.dtype], _lib.stream(),
               nbytes=a.element_size() * 2 * (a.numel() + v.numel()))
@@ -95,7 +95,7 @@ def decay_attention_fwd(q, k, v, log_decay, state=None, lengths=None, scale=None
         if q.numel() == 0:      # no token: the state as it was
             end = torch.zeros(B, H, dk, dv, device=q.device) if state is None else state.clone()
             return torch.empty(v.shape, device=v.device, dtype=v.dtype), end
-        end = torch.empty(B, H, dk, dv, device=q.device, dtype=torch.float32)
+        end = q.new_empty(B, H, dk, dv, dtype=torch.float32)
         x0 = state.contiguous() if state is not None else None
         o, _ = _walk(q, k, v, log_decay.contiguous(), lengths, x0, False, end, scale, 1.0, False)
         return o, end
@@ -111,7 +111,7 @@ def decay_attention_bwd(do, q, k, v, log_decay, state=None, lengths=None, scale=
     _check_state("d_state", d_state, (B, H, dk, dv))
     scale = dk ** -0.5 if scale is None else float(scale)
     with _lib.on_device(q, do, k, v, log_decay, state, lengths, d_state):
-        d0 = torch.empty(B, H, dk, dv, device=q.device, dtype=torch.float32)
+        d0 = q.new_empty(B, H, dk, dv, dtype=torch.float32)
         if q.numel() == 0:
             d0.copy_(d_state) if d_state is not None else d0.zero_()
             return torch.empty_like(q), torch.empty_like(k), torch.empty_like(v), d0
@@ -160,7 +160,7 @@ def decay_attention_step(q, k, v, log_decay, state, scale=None, out=None):
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, state)):
         raise RuntimeError("decay_attention_step has no backward pass: call it under torch.no_grad() or detach its inputs")
     if out is None:
-        out = torch.empty(B, H, dv, device=q.device, dtype=q.dtype)
+        out = q.new_empty(B, H, dv)
     elif tuple(out.shape) != (B, H, dv) or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError(f"out must be a packed {q.dtype} {(B, H, dv)}, got {out.dtype} {tuple(out.shape)}")
     scale = dk ** -0.5 if scale is None else float(scale)

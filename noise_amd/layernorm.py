@@ -46,7 +46,7 @@ def _check(x, weight, bias):
     for name, p in (("weight", weight), ("bias", bias)):
         if p is None:
             continue
-        if tuple(p.shape) != (D,):
+        if p.shape != (D,):
             raise ValueError(f"{name} must be ({D},), got {tuple(p.shape)}")
         if p.dtype not in (torch.float32, x.dtype) or (wdtype is not None and p.dtype != wdtype):
             raise TypeError(f"weight and bias must both be float32 or both {x.dtype}, got {name} in {p.dtype}")
@@ -59,14 +59,15 @@ def layer_norm_fwd(x, weight=None, bias=None, eps=1e-6):
     D, wdtype = _check(x, weight, bias)
     with _lib.on_device(x, weight, bias):
         xr, ld = _rows(x, D)
-        y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        stats = torch.empty((2,) + x.shape[:-1], device=x.device, dtype=torch.float32)
+        y = x.new_empty(x.shape)
+        mean, rstd = (x.new_empty(x.shape[:-1], dtype=torch.float32) for _ in range(2))
         rows = x.numel() // D
         if rows:
-            w, b = (p.contiguous() if p is not None else None for p in (weight, bias))
-            _lib.call("noise_layer_norm_fwd", ptr(xr), ld, ptr(w), ptr(b), float(eps), ptr(y), ptr(stats[0]), ptr(stats[1]), rows, D,
+            w = weight.contiguous() if weight is not None else None
+            b = bias.contiguous() if bias is not None else None
+            _lib.call("noise_layer_norm_fwd", ptr(xr), ld, ptr(w), ptr(b), eps, ptr(y), ptr(mean), ptr(rstd), rows, D,
                       _lib.DTYPES[x.dtype], _lib.DTYPES[wdtype], _lib.stream(), nbytes=2 * x.numel() * x.element_size())
-        return y, stats[0], stats[1]
+        return y, mean, rstd
 
 
 def layer_norm_bwd(dy, x, mean, rstd, weight=None, need_params=True):
@@ -82,16 +83,16 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, need_params=True):
     with _lib.on_device(x, dy, mean, rstd, weight):
         xr, ldx = _rows(x, D)
         gr, ldg = _rows(dy, D)
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        dx = x.new_empty(x.shape)
         rows = x.numel() // D
         dw = db = slab = None
         if need_params:
-            dw, db = (torch.empty(D, device=x.device, dtype=wdtype) for _ in range(2))
+            dw, db = (x.new_empty(D, dtype=wdtype) for _ in range(2))
             if rows == 0:
                 dw.zero_()
                 db.zero_()
             else:
-                slab = torch.empty(_lib.lib.noise_layer_norm_bwd_rows(rows, D) * 2 * D, device=x.device, dtype=torch.float32)
+                slab = x.new_empty(_lib.lib.noise_layer_norm_bwd_rows(rows, D) * 2 * D, dtype=torch.float32)
         if rows:
             mean, rstd = mean.contiguous(), rstd.contiguous()
             w = weight.contiguous() if weight is not None else None

@@ -5,7 +5,7 @@ Same update rule and defaults as the optimizer the reference wires through Light
 (train/main.py:13-14, train/configs/spectralv2.yaml:99-111): decoupled weight decay, no amsgrad.
 """
 import array
-import ctypes
+from operator import attrgetter
 
 import torch
 
@@ -112,6 +112,9 @@ class MultiTensorAdamW:
             self.state = {"exp_avg": torch.zeros(total, **z), "exp_avg_sq": torch.zeros(total, **z)}
         self.step_count = torch.zeros(n, dtype=torch.int64, **z)
         self._coef = torch.empty(n, 2, **z)
+        self._device = self.params[0].get_device()
+        self._shapes = [p.shape for p in self.params]
+        self._types = [p.dtype for p in self.params]
 
     def zero_grad(self, set_to_none=True):
         for p in self.params:
@@ -124,37 +127,26 @@ class MultiTensorAdamW:
     def step(self, grad_scale=1.0, grads=None):
         """One update from `grads` (one tensor or None per parameter), the parameters' own `.grad` when omitted.
         `grad_scale` multiplies every gradient (1 / world size of a summed data-parallel gradient)."""
-        params = self.params
-        grads = [p.grad for p in params] if grads is None else list(grads)
-        n = len(params)
+        params, n = self.params, len(self.params)
+        grads = list(map(attrgetter("grad"), params)) if grads is None else list(grads)
         if len(grads) != n:
             raise ValueError(f"{len(grads)} gradients for {n} parameters")
-        live = [i for i in range(n) if grads[i] is not None]
-        if len(live) == 0:
+        live = [i for i, g in enumerate(grads) if g is not None]
+        if not live:
             return
-        self._check(live, grads)
-        if len(live) < n:
-            keep = list(live)
-            params, grads = [params[i] for i in keep], [grads[i] for i in keep]
-        groups = {}
-        kinds = list(zip((p.dtype for p in params), (g.dtype for g in grads)))
-        if len(set(kinds)) == 1:
-            groups[kinds[0]] = range(len(params))
-        else:
-            for j, kind in enumerate(kinds):
-                groups.setdefault(kind, []).append(j)
-        for pd, gd in groups:
-            if pd not in _lib.DTYPES or (gd != pd and not (pd == torch.float32 and gd in _lib.DTYPES)):
+        whole = len(live) == n
+        pick = (lambda a: a) if whole else (lambda a: [a[i] for i in live])
+        params, grads, shapes, types = pick(params), pick(grads), pick(self._shapes), pick(self._types)
+        self._check(live, params, grads, shapes, types)
+        gtypes = list(map(attrgetter("dtype"), grads))
+        kinds = set(zip(types, gtypes))
+        for pd, gd in kinds:
+            if gd != pd and not (pd == torch.float32 and gd in _lib.DTYPES):
                 raise TypeError(f"a {pd} parameter cannot take a {gd} gradient")
-        index = array.array("i", live)
-        off = array.array("l", self.offsets if len(live) == n else [self.offsets[i] for i in live])
-        numel = array.array("l", self._numel if len(live) == n else [self._numel[i] for i in live])
-        pp = array.array("Q", map(torch.Tensor.data_ptr, params))
-        gp = array.array("Q", map(torch.Tensor.data_ptr, grads))
-        words = [0] * ((n + 63) // 64)
-        if len(live) == n:
-            words = [0xffffffffffffffff] * len(words)
-        else:
+        lists = [array.array("Q", map(torch.Tensor.data_ptr, params)), array.array("Q", map(torch.Tensor.data_ptr, grads)),
+                 array.array("l", pick(self._numel)), array.array("l", pick(self.offsets)), array.array("i", live)]
+        words = [0xffffffffffffffff if whole else 0] * ((n + 63) // 64)
+        if not whole:
             for i in live:
                 words[i >> 6] |= 1 << (i & 63)
         mask = array.array("Q", words)
@@ -164,31 +156,34 @@ class MultiTensorAdamW:
         else:
             bufs = (s["exp_avg"], None, s["exp_avg_sq"], None)
         bufs = [ptr(b) for b in bufs]
-        addr = lambda a: ctypes.c_void_p(a.buffer_info()[0])
         with _lib.on_device(self.step_count):
             st = _lib.stream()
-            _lib.call("noise_adamw_multi_begin", ptr(self.step_count), ptr(self._coef), addr(mask), n, self.lr, *self.betas, st)
-            for (pd, gd), js in groups.items():
-                lists = [pp, gp, numel, off, index]
-                if len(js) < len(params):
-                    lists = [array.array(a.typecode, [a[j] for j in js]) for a in lists]
+            _lib.call("noise_adamw_multi_begin", ptr(self.step_count), ptr(self._coef), mask.buffer_info()[0], n, self.lr, *self.betas, st)
+            for pd, gd in kinds:
+                part = lists
+                if len(kinds) > 1:
+                    mine = [j for j in range(len(params)) if types[j] == pd and gtypes[j] == gd]
+                    part = [array.array(a.typecode, [a[j] for j in mine]) for a in lists]
                 state_bytes = 4 if self.state_bits == 8 else 16
-                _lib.call("noise_adamw_multi", *map(addr, lists), len(js), _lib.DTYPES[pd], _lib.DTYPES[gd], self.state_bits,
-                          ptr(self._coef), *bufs, self.lr, *self.betas, self.eps, self.weight_decay, float(grad_scale), st,
-                          nbytes=sum(lists[2]) * (state_bytes + 2 * pd.itemsize + gd.itemsize) if _lib.PROFILE is not None else 0)
+                _lib.call("noise_adamw_multi", *(a.buffer_info()[0] for a in part), len(part[0]), _lib.DTYPES[pd], _lib.DTYPES[gd],
+                          self.state_bits, ptr(self._coef), *bufs, self.lr, *self.betas, self.eps, self.weight_decay, grad_scale, st,
+                          nbytes=sum(part[2]) * (state_bytes + 2 * pd.itemsize + gd.itemsize) if _lib.PROFILE is not None else 0)
         # the kernel wrote through raw pointers: autograd's and the models' stale-weight checks go by the version counters
         torch.autograd.graph.increment_version(params)
 
-    def _check(self, live, grads):
-        dev = self.step_count.device
-        for i in live:
-            g, p = grads[i], self.params[i]
-            if g.shape != p.shape or g.device != dev:
-                raise ValueError(f"gradient {i} is {tuple(g.shape)} on {g.device}, its parameter {tuple(p.shape)} on {dev}")
-            if not g.is_contiguous():
-                grads[i] = g.contiguous()
-            if p.device != dev or p.numel() != self._numel[i] or not p.is_contiguous():
-                raise RuntimeError(f"parameter {i} was moved, resized or transposed after the optimizer was built")
+    def _check(self, live, params, grads, shapes, types):
+        """Whole-list comparisons first: a step of many small tensors is as fast as this loop over them is."""
+        T = torch.Tensor
+        here = [self._device] * len(live)
+        if list(map(attrgetter("shape"), grads)) != shapes or list(map(T.get_device, grads)) != here:
+            for i, g, shape in zip(live, grads, shapes):
+                if g.shape != shape or g.get_device() != self._device:
+                    raise ValueError(f"gradient {i} is {tuple(g.shape)} on {g.device}, its parameter {tuple(shape)} on {self.step_count.device}")
+        if not all(map(T.is_contiguous, grads)):
+            grads[:] = [g.contiguous() for g in grads]
+        if (list(map(attrgetter("shape"), params)) != shapes or list(map(T.get_device, params)) != here
+                or list(map(attrgetter("dtype"), params)) != types or not all(map(T.is_contiguous, params))):
+            raise RuntimeError("a parameter was moved, resized, converted or transposed after the optimizer was built")
 
     def state_dict(self):
         return {**{k: v.clone() for k, v in self.state.items()}, "step": self.step_count.clone(), "state_bits": self.state_bits,
@@ -201,8 +196,6 @@ class MultiTensorAdamW:
             if k not in sd or sd[k].shape != v.shape or sd[k].dtype != v.dtype:
                 raise ValueError(f"state {k!r} must be {v.dtype} {tuple(v.shape)}")
         for k, v in self.state.items():
-            # bytes: 8-bit values are copied as they are
-            (v.view(torch.uint8) if self.state_bits == 8 and v.dtype == torch.float8_e4m3fn else v).copy_(
-                sd[k].view(torch.uint8) if v.dtype == torch.float8_e4m3fn else sd[k])
+            v.view(torch.uint8).copy_(sd[k].view(torch.uint8))      # the bytes, of 8-bit values too
         self.step_count.copy_(sd["step"])
         self.lr, self.betas, self.eps, self.weight_decay = sd["lr"], tuple(sd["betas"]), sd["eps"], sd["weight_decay"]
