@@ -35,7 +35,7 @@ struct AdamIndex {
 };
 struct AdamCoef {
   float beta1, beta2, omb1, omb2, eps, decay, grad_scale;
-  double dbeta1, dbeta2;
+  double dbeta1, dbeta2, domb1, domb2;
 };
 struct AdamMask {
   unsigned long long w[ADAM_MASK_WORDS];
@@ -61,19 +61,20 @@ __device__ __forceinline__ int adam_find(const AdamList& l, int unit) {
   return lo;
 }
 
-// Four values of a tensor, elementwise where the address does not allow a vector access or the tensor ends inside.
-template <typename T>
+// Four values of a tensor, elementwise where the address does not allow a vector access or the tensor ends inside
+// (FULL: neither can be).
+template <bool FULL, typename T>
 __device__ __forceinline__ void load4(const T* base, int i, int n, bool vec, float (&out)[4]) {
-  if (vec && i + 4 <= n) {
+  if (FULL || (vec && i + 4 <= n)) {
     load_vec<T, 4>(base + i, out);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[j] = i + j < n ? (float)base[i + j] : 0.f;
   }
 }
-template <typename T>
+template <bool FULL, typename T>
 __device__ __forceinline__ void store4(T* base, int i, int n, bool vec, const float (&in)[4]) {
-  if (vec && i + 4 <= n) {
+  if (FULL || (vec && i + 4 <= n)) {
     store_vec<T, 4>(base + i, in);
   } else {
 #pragma unroll
@@ -82,123 +83,145 @@ __device__ __forceinline__ void store4(T* base, int i, int n, bool vec, const fl
   }
 }
 
+// p, g and the states of one workgroup's 4096 values
 template <typename P, typename G>
-__global__ __launch_bounds__(256) void adam32_kernel(AdamList l, AdamIndex ix, const float2* __restrict__ coef,
-                                                     float* __restrict__ ms, float* __restrict__ vs, AdamCoef c) {
-  const int unit = blockIdx.x;
-  const int t = adam_find(l, unit);
+struct AdamUnit {
+  P* p;
+  const G* g;
+  size_t state;      // first value in the state buffers
+  float2 coef;
+  int n;             // values, 4096 except in a tensor's last workgroup
+  bool vec;
+};
+template <typename P, typename G>
+__device__ __forceinline__ AdamUnit<P, G> adam_unit(const AdamList& l, const AdamIndex& ix, const float2* coef) {
+  const int unit = blockIdx.x, t = adam_find(l, unit);
   const int local = unit - (t ? l.end_unit[t - 1] : 0);
-  const bool last = unit == l.end_unit[t] - 1;
-  const int n = last ? l.numel_lo[t] : ADAM_UNIT;
   const size_t at = (size_t)local * ADAM_UNIT;
-  P* p = (P*)l.p[t] + at;
-  const G* g = (const G*)l.g[t] + at;
-  float *m = ms + l.off[t] + at, *v = vs + l.off[t] + at;
-  const float2 k = coef[ix.idx[t]];
-  const bool vec = ((uintptr_t)p % (4 * sizeof(P))) == 0 && ((uintptr_t)g % (4 * sizeof(G))) == 0;
+  AdamUnit<P, G> u;
+  u.p = (P*)l.p[t] + at;
+  u.g = (const G*)l.g[t] + at;
+  u.state = (size_t)l.off[t] + at;
+  u.coef = coef[ix.idx[t]];
+  u.n = unit == l.end_unit[t] - 1 ? l.numel_lo[t] : ADAM_UNIT;
+  u.vec = ((uintptr_t)u.p % (4 * sizeof(P))) == 0 && ((uintptr_t)u.g % (4 * sizeof(G))) == 0;
+  return u;
+}
+
+template <bool FULL, typename P, typename G>
+__device__ __forceinline__ void adam32_unit(const AdamUnit<P, G>& t, float* m, float* v, const AdamCoef& c) {
+  const int n = t.n, whole = (n + 3) & ~3;   // the states are padded to blocks of 256: a vector never leaves them
   float pv[4][4], gv[4][4], mv[4][4], vv[4][4];
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     const int i = (u * 256 + threadIdx.x) * 4;
-    load4(p, i, n, vec, pv[u]);
-    load4(g, i, n, vec, gv[u]);
-    // the states are padded to whole blocks of 256 values: a vector that starts inside the tensor ends inside its padding
-    load4(m, i, (n + 3) & ~3, true, mv[u]);
-    load4(v, i, (n + 3) & ~3, true, vv[u]);
+    load4<FULL>(t.p, i, n, t.vec, pv[u]);
+    load4<FULL>(t.g, i, n, t.vec, gv[u]);
+    load4<FULL>(m, i, whole, true, mv[u]);
+    load4<FULL>(v, i, whole, true, vv[u]);
   }
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     const int i = (u * 256 + threadIdx.x) * 4;
-    if (i >= n) break;
+    if (!FULL && i >= n) break;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float gi = gv[u][j] * c.grad_scale;
       const float mi = mv[u][j] * c.beta1 + c.omb1 * gi;
       const float vi = vv[u][j] * c.beta2 + c.omb2 * (gi * gi);
-      const float denom = sqrtf(vi) / k.y + c.eps;
-      pv[u][j] = pv[u][j] * c.decay - k.x * (mi / denom);
+      const float denom = sqrtf(vi) / t.coef.y + c.eps;
+      pv[u][j] = pv[u][j] * c.decay - t.coef.x * (mi / denom);
       mv[u][j] = mi;
       vv[u][j] = vi;
     }
-    store4(p, i, n, vec, pv[u]);
-    store4(m, i, (n + 3) & ~3, true, mv[u]);
-    store4(v, i, (n + 3) & ~3, true, vv[u]);
+    store4<FULL>(t.p, i, n, t.vec, pv[u]);
+    store4<FULL>(m, i, whole, true, mv[u]);
+    store4<FULL>(v, i, whole, true, vv[u]);
   }
 }
 
-__device__ __forceinline__ double wave_max(double v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
-  return v;
+template <typename P, typename G>
+__global__ __launch_bounds__(256) void adam32_kernel(AdamList l, AdamIndex ix, const float2* __restrict__ coef,
+                                                     float* __restrict__ ms, float* __restrict__ vs, AdamCoef c) {
+  const AdamUnit<P, G> t = adam_unit<P, G>(l, ix, coef);
+  if (t.vec && t.n == ADAM_UNIT) adam32_unit<true>(t, ms + t.state, vs + t.state, c);
+  else adam32_unit<false>(t, ms + t.state, vs + t.state, c);
+}
+
+// Largest of a 32-bit value over the wave, in a scalar register: four steps as DPP operands, then one value per 16 lanes.
+__device__ __forceinline__ unsigned wave_max_u32(unsigned v) {
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, true));
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, true));
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, true));
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, true));
+  const unsigned a = __builtin_amdgcn_readlane((int)v, 0), b = __builtin_amdgcn_readlane((int)v, 16);
+  const unsigned c = __builtin_amdgcn_readlane((int)v, 32), d = __builtin_amdgcn_readlane((int)v, 48);
+  return max(max(a, b), max(c, d));
 }
 
 // A double as the float that rounds to the same 8-bit value: cut off, with the lowest bit set where something was lost, so
 // that the second rounding sees which side of a border the value lies on.
 __device__ __forceinline__ float to_odd(double x) {
-  unsigned long long b = __double_as_longlong(x);
-  const bool lost = (b & 0x1fffffffull) != 0;
-  b &= ~0x1fffffffull;
-  if (lost) b |= 0x20000000ull;
-  return (float)__longlong_as_double(b);
+  const unsigned long long b = __double_as_longlong(x);
+  unsigned lo = (unsigned)b;
+  lo = (lo & 0xe0000000u) | ((lo & 0x1fffffffu) ? 0x20000000u : 0u);
+  return (float)__longlong_as_double((long long)((b & 0xffffffff00000000ull) | lo));
 }
 
-// Four values of a 256-value block as e4m3 codes under the scale max / 448; the whole wave takes part.
+// Four values of a 256-value block as e4m3 codes under the scale max / 448; the whole wave takes part.  The largest magnitude
+// is found on the bits of the doubles (their order is the integers', and a NaN or infinity is above all others): the high
+// words first, then the low words of those that share the highest.
 template <bool POSITIVE>
 __device__ __forceinline__ unsigned quantise4(const double (&x)[4], float& scale) {
-  double top = 0.0;
-  bool bad = false;
+  unsigned hi[4], lo[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const double a = fabs(x[j]);
-    bad |= !(a < 1e300);
-    top = fmax(top, a);
+    const unsigned long long b = __double_as_longlong(x[j]);
+    hi[j] = (unsigned)(b >> 32) & 0x7fffffffu;
+    lo[j] = (unsigned)b;
   }
-  top = wave_max(top);
+  const unsigned th = wave_max_u32(max(max(hi[0], hi[1]), max(hi[2], hi[3])));
+  unsigned l = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) l = max(l, hi[j] == th ? lo[j] : 0u);
+  const double top = __longlong_as_double((long long)((unsigned long long)th << 32 | wave_max_u32(l)));
   scale = (float)(top * (1.0 / 448.0));
   const double inv = scale > 0.f ? 1.0 / (double)scale : 0.0;
   float q[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float y = to_odd(x[j] * inv);
-    q[j] = fminf(fmaxf(y, -448.f), 448.f);
-  }
+  for (int j = 0; j < 4; ++j) q[j] = __builtin_amdgcn_fmed3f(to_odd(x[j] * inv), -448.f, 448.f);
   int code = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
   code = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], code, true);
   if (POSITIVE) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (x[j] > 0.0 && ((code >> (8 * j)) & 0xff) == 0) code |= 1 << (8 * j);
+      if ((hi[j] | lo[j]) != 0 && (code & (0xff << (8 * j))) == 0) code |= 1 << (8 * j);
   }
-  if (__any(bad)) scale = __int_as_float(0x7fc00000);
+  if (th >= 0x7ff00000u) scale = __int_as_float(0x7fc00000);
   return (unsigned)code;
 }
 
-__device__ __forceinline__ void decode4(unsigned code, float scale, double (&x)[4]) {
-  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, false);
-  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, true);
-  const double s = (double)scale;
-  x[0] = (double)lo[0] * s;
-  x[1] = (double)lo[1] * s;
-  x[2] = (double)hi[0] * s;
-  x[3] = (double)hi[1] * s;
+// sqrt in 64 bits to about 46: the hardware's reciprocal root and one step of Newton's method.
+__device__ __forceinline__ double root64(double v) {
+  const double y = __builtin_amdgcn_rsq(v), s = v * y;
+  const double r = s + 0.5 * y * __builtin_fma(-s, s, v);
+  return v > 0.0 && v < 1e300 ? r : v;        // zero, and what is not finite, as they are
 }
 
-template <typename P, typename G>
-__global__ __launch_bounds__(256) void adam8_kernel(AdamList l, AdamIndex ix, const float2* __restrict__ coef,
-                                                    unsigned* __restrict__ ms, float* __restrict__ mscale,
-                                                    unsigned* __restrict__ rs, float* __restrict__ rscale, AdamCoef c) {
-  const int unit = blockIdx.x;
-  const int t = adam_find(l, unit);
-  const int local = unit - (t ? l.end_unit[t - 1] : 0);
-  const bool last = unit == l.end_unit[t] - 1;
-  const int n = last ? l.numel_lo[t] : ADAM_UNIT;
-  const size_t at = (size_t)local * ADAM_UNIT;
-  P* p = (P*)l.p[t] + at;
-  const G* g = (const G*)l.g[t] + at;
-  const size_t s0 = ((size_t)l.off[t] + at);
-  const float2 k = coef[ix.idx[t]];
-  const bool vec = ((uintptr_t)p % (4 * sizeof(P))) == 0 && ((uintptr_t)g % (4 * sizeof(G))) == 0;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+// a / b: the hardware's reciprocal and one correction (within one unit of the last place); the division itself where an
+// intermediate value could leave the range.
+__device__ __forceinline__ float quotient(float a, float b) {
+  const float y = __builtin_amdgcn_rcpf(b), q = a * y;
+  float r = __builtin_fmaf(__builtin_fmaf(-q, b, a), y, q);
+  if (!(b > 1e-30f && b < 1e30f && fabsf(q) < 1e30f)) r = a / b;
+  return r;
+}
+
+template <bool FULL, typename P, typename G>
+__device__ __forceinline__ void adam8_unit(const AdamUnit<P, G>& t, unsigned* ms, float* mscale, unsigned* rs, float* rscale,
+                                           const AdamCoef& c) {
+  const int n = t.n, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const float inv_root = 1.f / t.coef.y;
   float pv[4][4], gv[4][4], msc[4], rsc[4];
   unsigned mc[4], rc[4];
 #pragma unroll
@@ -206,10 +229,10 @@ __global__ __launch_bounds__(256) void adam8_kernel(AdamList l, AdamIndex ix, co
     const int b = (u * 4 + wave) * ADAM_BLOCK, i = b + lane * 4;   // uniform per wave: one block of values
     mc[u] = rc[u] = 0;
     msc[u] = rsc[u] = 0.f;
-    if (b < n) {
-      const size_t q = (s0 + i) / 4, sc = (s0 + b) / ADAM_BLOCK;
-      load4(p, i, n, vec, pv[u]);
-      load4(g, i, n, vec, gv[u]);
+    if (FULL || b < n) {
+      const size_t q = (t.state + i) / 4, sc = (t.state + b) / ADAM_BLOCK;
+      load4<FULL>(t.p, i, n, t.vec, pv[u]);
+      load4<FULL>(t.g, i, n, t.vec, gv[u]);
       mc[u] = ms[q];
       rc[u] = rs[q];
       msc[u] = mscale[sc];
@@ -219,29 +242,45 @@ __global__ __launch_bounds__(256) void adam8_kernel(AdamList l, AdamIndex ix, co
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     const int b = (u * 4 + wave) * ADAM_BLOCK, i = b + lane * 4;
-    if (b >= n) break;
+    if (!FULL && b >= n) break;
+    float cm[4], cr[4];
+    {
+      const auto m0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[u], false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[u], true);
+      const auto r0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)rc[u], false), r1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)rc[u], true);
+      cm[0] = m0[0], cm[1] = m0[1], cm[2] = m1[0], cm[3] = m1[1];
+      cr[0] = r0[0], cr[1] = r0[1], cr[2] = r1[0], cr[3] = r1[1];
+    }
+    const double sm = (double)msc[u], sr = (double)rsc[u];
+    const double fm = c.dbeta1 * sm, fr = c.dbeta2 * (sr * sr);
     double m[4], r[4];
-    decode4(mc[u], msc[u], m);
-    decode4(rc[u], rsc[u], r);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const double gi = (double)(gv[u][j] * c.grad_scale);
-      m[j] = c.dbeta1 * m[j] + (1.0 - c.dbeta1) * gi;
-      r[j] = sqrt(c.dbeta2 * r[j] * r[j] + (1.0 - c.dbeta2) * gi * gi);
-      const float denom = (float)r[j] / k.y + c.eps;
-      pv[u][j] = pv[u][j] * c.decay - k.x * ((float)m[j] / denom);
+      m[j] = __builtin_fma((double)cm[j], fm, c.domb1 * gi);
+      r[j] = root64(__builtin_fma((double)(cr[j] * cr[j]), fr, c.domb2 * (gi * gi)));   // a code's square has 8 bits
+      const float denom = (float)r[j] * inv_root + c.eps;
+      pv[u][j] = pv[u][j] * c.decay - t.coef.x * quotient((float)m[j], denom);
     }
-    store4(p, i, n, vec, pv[u]);
-    float sm, sr;
-    const unsigned cm = quantise4<false>(m, sm), cr = quantise4<true>(r, sr);
-    const size_t q = (s0 + i) / 4, sc = (s0 + b) / ADAM_BLOCK;
-    ms[q] = cm;
-    rs[q] = cr;
+    store4<FULL>(t.p, i, n, t.vec, pv[u]);
+    float nm, nr;
+    const unsigned am = quantise4<false>(m, nm), ar = quantise4<true>(r, nr);
+    const size_t q = (t.state + i) / 4, sc = (t.state + b) / ADAM_BLOCK;
+    ms[q] = am;
+    rs[q] = ar;
     if (lane == 0) {
-      mscale[sc] = sm;
-      rscale[sc] = sr;
+      mscale[sc] = nm;
+      rscale[sc] = nr;
     }
   }
+}
+
+template <typename P, typename G>
+__global__ __launch_bounds__(256) void adam8_kernel(AdamList l, AdamIndex ix, const float2* __restrict__ coef,
+                                                    unsigned* __restrict__ ms, float* __restrict__ mscale,
+                                                    unsigned* __restrict__ rs, float* __restrict__ rscale, AdamCoef c) {
+  const AdamUnit<P, G> t = adam_unit<P, G>(l, ix, coef);
+  if (t.vec && t.n == ADAM_UNIT) adam8_unit<true>(t, ms, mscale, rs, rscale, c);
+  else adam8_unit<false>(t, ms, mscale, rs, rscale, c);
 }
 
 template <typename P, typename G>
@@ -288,7 +327,7 @@ NOISE_EXPORT int noise_adamw_multi(const unsigned long long* p, const unsigned l
   AdamCoef c;
   c.beta1 = (float)beta1, c.beta2 = (float)beta2, c.omb1 = (float)(1.0 - beta1), c.omb2 = (float)(1.0 - beta2);
   c.eps = (float)eps, c.decay = (float)(1.0 - lr * weight_decay), c.grad_scale = (float)grad_scale;
-  c.dbeta1 = beta1, c.dbeta2 = beta2;
+  c.dbeta1 = beta1, c.dbeta2 = beta2, c.domb1 = 1.0 - beta1, c.domb2 = 1.0 - beta2;
   const bool small = bits == 8;
   for (int i = 0; i < count;) {
     AdamList l;

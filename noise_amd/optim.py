@@ -115,6 +115,10 @@ class MultiTensorAdamW:
         self._device = self.params[0].get_device()
         self._shapes = [p.shape for p in self.params]
         self._types = [p.dtype for p in self.params]
+        # what a step hands to the kernel when every parameter has a gradient
+        self._addresses = array.array("Q", map(torch.Tensor.data_ptr, self.params))
+        self._whole = (array.array("l", self._numel), array.array("l", self.offsets), array.array("i", range(n)),
+                       array.array("Q", [0xffffffffffffffff] * ((n + 63) // 64)))
 
     def zero_grad(self, set_to_none=True):
         for p in self.params:
@@ -135,21 +139,21 @@ class MultiTensorAdamW:
         if not live:
             return
         whole = len(live) == n
-        pick = (lambda a: a) if whole else (lambda a: [a[i] for i in live])
-        params, grads, shapes, types = pick(params), pick(grads), pick(self._shapes), pick(self._types)
-        self._check(live, params, grads, shapes, types)
+        numel, off, index, mask = self._whole
+        shapes, types, addresses = self._shapes, self._types, self._addresses
+        if not whole:
+            params, grads, shapes, types = ([a[i] for i in live] for a in (params, grads, shapes, types))
+            numel, off, addresses = (array.array(a.typecode, [a[i] for i in live]) for a in (numel, off, addresses))
+            index, mask = array.array("i", live), array.array("Q", bytes(len(mask) * 8))
+            for i in live:
+                mask[i >> 6] |= 1 << (i & 63)
+        addresses = self._check(live, params, grads, shapes, types, addresses)
         gtypes = list(map(attrgetter("dtype"), grads))
         kinds = set(zip(types, gtypes))
         for pd, gd in kinds:
             if gd != pd and not (pd == torch.float32 and gd in _lib.DTYPES):
                 raise TypeError(f"a {pd} parameter cannot take a {gd} gradient")
-        lists = [array.array("Q", map(torch.Tensor.data_ptr, params)), array.array("Q", map(torch.Tensor.data_ptr, grads)),
-                 array.array("l", pick(self._numel)), array.array("l", pick(self.offsets)), array.array("i", live)]
-        words = [0xffffffffffffffff if whole else 0] * ((n + 63) // 64)
-        if not whole:
-            for i in live:
-                words[i >> 6] |= 1 << (i & 63)
-        mask = array.array("Q", words)
+        lists = [addresses, array.array("Q", map(torch.Tensor.data_ptr, grads)), numel, off, index]
         s = self.state
         if self.state_bits == 8:
             bufs = (s["exp_avg"], s["exp_avg_scale"], s["exp_avg_sq_root"], s["exp_avg_sq_root_scale"])
@@ -171,8 +175,9 @@ class MultiTensorAdamW:
         # the kernel wrote through raw pointers: autograd's and the models' stale-weight checks go by the version counters
         torch.autograd.graph.increment_version(params)
 
-    def _check(self, live, params, grads, shapes, types):
-        """Whole-list comparisons first: a step of many small tensors is as fast as this loop over them is."""
+    def _check(self, live, params, grads, shapes, types, addresses):
+        """The parameters' addresses, after the checks.  Whole-list comparisons first: a step of many small tensors is as fast
+        as the loops over them are."""
         T = torch.Tensor
         here = [self._device] * len(live)
         if list(map(attrgetter("shape"), grads)) != shapes or list(map(T.get_device, grads)) != here:
@@ -181,9 +186,12 @@ class MultiTensorAdamW:
                     raise ValueError(f"gradient {i} is {tuple(g.shape)} on {g.device}, its parameter {tuple(shape)} on {self.step_count.device}")
         if not all(map(T.is_contiguous, grads)):
             grads[:] = [g.contiguous() for g in grads]
-        if (list(map(attrgetter("shape"), params)) != shapes or list(map(T.get_device, params)) != here
-                or list(map(attrgetter("dtype"), params)) != types or not all(map(T.is_contiguous, params))):
+        now = array.array("Q", map(T.data_ptr, params))
+        if not all(map(T.is_contiguous, params)) or (now != addresses and (
+                list(map(attrgetter("shape"), params)) != shapes or list(map(T.get_device, params)) != here
+                or list(map(attrgetter("dtype"), params)) != types)):
             raise RuntimeError("a parameter was moved, resized, converted or transposed after the optimizer was built")
+        return now
 
     def state_dict(self):
         return {**{k: v.clone() for k, v in self.state.items()}, "step": self.step_count.clone(), "state_bits": self.state_bits,
