@@ -5,8 +5,8 @@
 // with one device-side step count t per tensor, so a captured launch replays correctly.
 //
 // Bound: HBM, 28 bytes per fp32 value with 32-bit states, 16 with 8-bit ones.  Pointers and sizes travel as kernel arguments
-// (nothing is uploaded, nothing outlives the call); a workgroup takes 4096 values of one tensor, all of a thread's loads
-// requested before the first use.
+// (nothing is uploaded, nothing outlives the call); a workgroup takes 1024 values of one tensor (4096, four vectors per
+// thread, reached 4.9 instead of 5.2 TB/s at 150 M values: many short workgroups keep the accesses in flight close together).
 //
 // 8-bit states: m and r = sqrt(v) as e4m3 values with one fp32 scale = max|.| / 448 per 256 consecutive values of a tensor,
 // i.e. one wave's four values per lane.  r rather than v: its range within a block (2^18 : 1) is then v's 2^36 : 1.  A
@@ -18,7 +18,7 @@
 namespace {
 
 constexpr int ADAM_MAX = 96;         // tensors per launch: 36 bytes each in the 4 KB of kernel arguments
-constexpr int ADAM_UNIT = 4096;      // values per workgroup
+constexpr int ADAM_UNIT = 1024;      // values per workgroup: one vector per thread, one block of values per wave
 constexpr int ADAM_BLOCK = 256;      // values per scale of the 8-bit states
 constexpr int ADAM_MASK_WORDS = 64;  // 64-bit words of the active mask per launch of the coefficient kernel
 
@@ -83,14 +83,14 @@ __device__ __forceinline__ void store4(T* base, int i, int n, bool vec, const fl
   }
 }
 
-// p, g and the states of one workgroup's 4096 values
+// p, g and the states of one workgroup's values
 template <typename P, typename G>
 struct AdamUnit {
   P* p;
   const G* g;
   size_t state;      // first value in the state buffers
   float2 coef;
-  int n;             // values, 4096 except in a tensor's last workgroup
+  int n;             // values, ADAM_UNIT except in a tensor's last workgroup
   bool vec;
 };
 template <typename P, typename G>
@@ -111,33 +111,24 @@ __device__ __forceinline__ AdamUnit<P, G> adam_unit(const AdamList& l, const Ada
 template <bool FULL, typename P, typename G>
 __device__ __forceinline__ void adam32_unit(const AdamUnit<P, G>& t, float* m, float* v, const AdamCoef& c) {
   const int n = t.n, whole = (n + 3) & ~3;   // the states are padded to blocks of 256: a vector never leaves them
-  float pv[4][4], gv[4][4], mv[4][4], vv[4][4];
+  const int i = threadIdx.x * 4;
+  if (!FULL && i >= n) return;
+  float pv[4], gv[4], mv[4], vv[4];
+  load4<FULL>(t.p, i, n, t.vec, pv);
+  load4<FULL>(t.g, i, n, t.vec, gv);
+  load4<FULL>(m, i, whole, true, mv);
+  load4<FULL>(v, i, whole, true, vv);
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int i = (u * 256 + threadIdx.x) * 4;
-    load4<FULL>(t.p, i, n, t.vec, pv[u]);
-    load4<FULL>(t.g, i, n, t.vec, gv[u]);
-    load4<FULL>(m, i, whole, true, mv[u]);
-    load4<FULL>(v, i, whole, true, vv[u]);
+  for (int j = 0; j < 4; ++j) {
+    const float gi = gv[j] * c.grad_scale;
+    mv[j] = mv[j] * c.beta1 + c.omb1 * gi;
+    vv[j] = vv[j] * c.beta2 + c.omb2 * (gi * gi);
+    const float denom = sqrtf(vv[j]) / t.coef.y + c.eps;
+    pv[j] = pv[j] * c.decay - t.coef.x * (mv[j] / denom);
   }
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int i = (u * 256 + threadIdx.x) * 4;
-    if (!FULL && i >= n) break;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float gi = gv[u][j] * c.grad_scale;
-      const float mi = mv[u][j] * c.beta1 + c.omb1 * gi;
-      const float vi = vv[u][j] * c.beta2 + c.omb2 * (gi * gi);
-      const float denom = sqrtf(vi) / t.coef.y + c.eps;
-      pv[u][j] = pv[u][j] * c.decay - t.coef.x * (mi / denom);
-      mv[u][j] = mi;
-      vv[u][j] = vi;
-    }
-    store4<FULL>(t.p, i, n, t.vec, pv[u]);
-    store4<FULL>(m, i, whole, true, mv[u]);
-    store4<FULL>(v, i, whole, true, vv[u]);
-  }
+  store4<FULL>(t.p, i, n, t.vec, pv);
+  store4<FULL>(m, i, whole, true, mv);
+  store4<FULL>(v, i, whole, true, vv);
 }
 
 template <typename P, typename G>
@@ -170,107 +161,89 @@ __device__ __forceinline__ float to_odd(double x) {
 
 // Four values of a 256-value block as e4m3 codes under the scale max / 448; the whole wave takes part.  The largest magnitude
 // is found on the bits of the doubles (their order is the integers', and a NaN or infinity is above all others): the high
-// words first, then the low words of those that share the highest.
+// words first, then, where several lanes share the highest, the low words.
 template <bool POSITIVE>
 __device__ __forceinline__ unsigned quantise4(const double (&x)[4], float& scale) {
-  unsigned hi[4], lo[4];
+  double t = fabs(x[0]);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const unsigned long long b = __double_as_longlong(x[j]);
-    hi[j] = (unsigned)(b >> 32) & 0x7fffffffu;
-    lo[j] = (unsigned)b;
-  }
-  const unsigned th = wave_max_u32(max(max(hi[0], hi[1]), max(hi[2], hi[3])));
-  unsigned l = 0;
+  for (int j = 1; j < 4; ++j) t = t >= fabs(x[j]) ? t : fabs(x[j]);      // a NaN among x[1..3] is taken over, one in t is lost:
+  bool nan = false;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) l = max(l, hi[j] == th ? lo[j] : 0u);
-  const double top = __longlong_as_double((long long)((unsigned long long)th << 32 | wave_max_u32(l)));
+  for (int j = 0; j < 4; ++j) nan |= x[j] != x[j];                         // hence this
+  const unsigned hi = nan ? 0x7ff80000u : (unsigned)(__double_as_longlong(t) >> 32), lo = (unsigned)__double_as_longlong(t);
+  const unsigned th = wave_max_u32(hi);
+  const unsigned long long who = __ballot(hi == th);
+  unsigned tl;
+  if ((who & (who - 1)) == 0) tl = (unsigned)__builtin_amdgcn_readlane((int)lo, __builtin_ctzll(who));
+  else tl = wave_max_u32(hi == th ? lo : 0u);
+  const double top = __longlong_as_double((long long)((unsigned long long)th << 32 | tl));
   scale = (float)(top * (1.0 / 448.0));
-  const double inv = scale > 0.f ? 1.0 / (double)scale : 0.0;
+  // 1 / scale to the last bits of a double: a float's reciprocal and two steps of Newton's method; a block whose scale is below
+  // the normal floats is divided by it
+  const double d = (double)scale;
+  double inv = (double)__builtin_amdgcn_rcpf(scale);
+  inv = __builtin_fma(__builtin_fma(-d, inv, 1.0), inv, inv);
+  inv = __builtin_fma(__builtin_fma(-d, inv, 1.0), inv, inv);
+  if (!(scale > 1e-36f && scale < 1e36f)) inv = scale > 0.f ? 1.0 / d : 0.0;
   float q[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) q[j] = __builtin_amdgcn_fmed3f(to_odd(x[j] * inv), -448.f, 448.f);
+  for (int j = 0; j < 4; ++j) q[j] = __builtin_amdgcn_fmed3f(to_odd(x[j] * inv), POSITIVE && x[j] > 0.0 ? 0x1p-9f : -448.f, 448.f);
   int code = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
   code = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], code, true);
-  if (POSITIVE) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if ((hi[j] | lo[j]) != 0 && (code & (0xff << (8 * j))) == 0) code |= 1 << (8 * j);
-  }
   if (th >= 0x7ff00000u) scale = __int_as_float(0x7fc00000);
   return (unsigned)code;
 }
 
-// sqrt in 64 bits to about 46: the hardware's reciprocal root and one step of Newton's method.
+// sqrt of a value >= 0 in 64 bits to about 46: the hardware's reciprocal root and one step of Newton's method.
 __device__ __forceinline__ double root64(double v) {
-  const double y = __builtin_amdgcn_rsq(v), s = v * y;
-  const double r = s + 0.5 * y * __builtin_fma(-s, s, v);
-  return v > 0.0 && v < 1e300 ? r : v;        // zero, and what is not finite, as they are
+  const double y = __builtin_amdgcn_rsq(v + 1e-300), s = v * y;      // 1e-300: zero gives zero
+  return __builtin_fma(0.5 * y, __builtin_fma(-s, s, v), s);
 }
 
-// a / b: the hardware's reciprocal and one correction (within one unit of the last place); the division itself where an
-// intermediate value could leave the range.
+// a / b: the hardware's reciprocal and one correction (within one unit of the last place); the division itself where b or its
+// reciprocal is near the ends of the range.
 __device__ __forceinline__ float quotient(float a, float b) {
   const float y = __builtin_amdgcn_rcpf(b), q = a * y;
   float r = __builtin_fmaf(__builtin_fmaf(-q, b, a), y, q);
-  if (!(b > 1e-30f && b < 1e30f && fabsf(q) < 1e30f)) r = a / b;
+  if (!(b > 1e-30f && b < 1e30f)) r = a / b;
   return r;
 }
 
 template <bool FULL, typename P, typename G>
 __device__ __forceinline__ void adam8_unit(const AdamUnit<P, G>& t, unsigned* ms, float* mscale, unsigned* rs, float* rscale,
                                            const AdamCoef& c) {
-  const int n = t.n, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int n = t.n, i = threadIdx.x * 4, b = i & ~(ADAM_BLOCK - 1);   // the wave's block of values
+  if (!FULL && b >= n) return;
   const float inv_root = 1.f / t.coef.y;
-  float pv[4][4], gv[4][4], msc[4], rsc[4];
-  unsigned mc[4], rc[4];
-#pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int b = (u * 4 + wave) * ADAM_BLOCK, i = b + lane * 4;   // uniform per wave: one block of values
-    mc[u] = rc[u] = 0;
-    msc[u] = rsc[u] = 0.f;
-    if (FULL || b < n) {
-      const size_t q = (t.state + i) / 4, sc = (t.state + b) / ADAM_BLOCK;
-      load4<FULL>(t.p, i, n, t.vec, pv[u]);
-      load4<FULL>(t.g, i, n, t.vec, gv[u]);
-      mc[u] = ms[q];
-      rc[u] = rs[q];
-      msc[u] = mscale[sc];
-      rsc[u] = rscale[sc];
-    }
+  float pv[4], gv[4], cm[4], cr[4];
+  const size_t q = (t.state + i) / 4, sc = (t.state + b) / ADAM_BLOCK;
+  load4<FULL>(t.p, i, n, t.vec, pv);
+  load4<FULL>(t.g, i, n, t.vec, gv);
+  const unsigned mc = ms[q], rc = rs[q];
+  const double sm = (double)mscale[sc], sr = (double)rscale[sc];
+  {
+    const auto m0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mc, false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mc, true);
+    const auto r0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)rc, false), r1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)rc, true);
+    cm[0] = m0[0], cm[1] = m0[1], cm[2] = m1[0], cm[3] = m1[1];
+    cr[0] = r0[0], cr[1] = r0[1], cr[2] = r1[0], cr[3] = r1[1];
   }
+  const double fm = c.dbeta1 * sm, fr = c.dbeta2 * (sr * sr);
+  double m[4], r[4];
 #pragma unroll
-  for (int u = 0; u < 4; ++u) {
-    const int b = (u * 4 + wave) * ADAM_BLOCK, i = b + lane * 4;
-    if (!FULL && b >= n) break;
-    float cm[4], cr[4];
-    {
-      const auto m0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[u], false), m1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)mc[u], true);
-      const auto r0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)rc[u], false), r1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)rc[u], true);
-      cm[0] = m0[0], cm[1] = m0[1], cm[2] = m1[0], cm[3] = m1[1];
-      cr[0] = r0[0], cr[1] = r0[1], cr[2] = r1[0], cr[3] = r1[1];
-    }
-    const double sm = (double)msc[u], sr = (double)rsc[u];
-    const double fm = c.dbeta1 * sm, fr = c.dbeta2 * (sr * sr);
-    double m[4], r[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const double gi = (double)(gv[u][j] * c.grad_scale);
-      m[j] = __builtin_fma((double)cm[j], fm, c.domb1 * gi);
-      r[j] = root64(__builtin_fma((double)(cr[j] * cr[j]), fr, c.domb2 * (gi * gi)));   // a code's square has 8 bits
-      const float denom = (float)r[j] * inv_root + c.eps;
-      pv[u][j] = pv[u][j] * c.decay - t.coef.x * quotient((float)m[j], denom);
-    }
-    store4<FULL>(t.p, i, n, t.vec, pv[u]);
-    float nm, nr;
-    const unsigned am = quantise4<false>(m, nm), ar = quantise4<true>(r, nr);
-    const size_t q = (t.state + i) / 4, sc = (t.state + b) / ADAM_BLOCK;
-    ms[q] = am;
-    rs[q] = ar;
-    if (lane == 0) {
-      mscale[sc] = nm;
-      rscale[sc] = nr;
-    }
+  for (int j = 0; j < 4; ++j) {
+    const double gi = (double)(gv[j] * c.grad_scale);
+    m[j] = __builtin_fma((double)cm[j], fm, c.domb1 * gi);
+    r[j] = root64(__builtin_fma((double)(cr[j] * cr[j]), fr, c.domb2 * (gi * gi)));   // a code's square has 8 bits
+    const float denom = (float)r[j] * inv_root + c.eps;
+    pv[j] = pv[j] * c.decay - t.coef.x * quotient((float)m[j], denom);
+  }
+  store4<FULL>(t.p, i, n, t.vec, pv);
+  float nm, nr;
+  ms[q] = quantise4<false>(m, nm);
+  rs[q] = quantise4<true>(r, nr);
+  if ((threadIdx.x & 63) == 0) {
+    mscale[sc] = nm;
+    rscale[sc] = nr;
   }
 }
 
