@@ -27,7 +27,7 @@ __device__ __forceinline__ float row_sum(float v, float* red, int& phase) {
   }
 }
 
-template <typename T, typename W, int VEC, int LANES, int NV>
+template <typename T, typename W, int VEC, int LANES, int NV, bool NT>
 __global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, long ldx, const W* __restrict__ w,
                                                      const W* __restrict__ b, float eps, T* __restrict__ y,
                                                      float* __restrict__ mean, float* __restrict__ rstd, long rows, int D) {
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, lo
       if (b) o += bb[i];
       v[k][i] = o;
     }
-    store_vec<T, VEC>(yr + c, v[k]);
+    store_vec_nt<NT, T, VEC>(yr + c, v[k]);
   }
   if (lane == 0) {
     if (mean) mean[row] = m;
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(256) void ln_fwd_wide_kernel(const T* __restrict__ 
 // A workgroup walks its rows; a lane keeps the sums of dw and db of its columns in registers, the row groups of a workgroup
 // are added in LDS in a fixed order, and each workgroup leaves one slab row [dw | db] for ln_fold_kernel: no atomics, the
 // same result on every run.  A row's sums are fp32 over rows / (grid x groups) terms, the fold is in double.
-template <typename T, typename W, int VEC, int LANES, int NV>
+template <typename T, typename W, int VEC, int LANES, int NV, bool NT>
 __global__ __launch_bounds__(256) void ln_bwd_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ x, long ldx,
                                                      const float* __restrict__ mean, const float* __restrict__ rstd,
                                                      const W* __restrict__ w, T* __restrict__ dx, float* __restrict__ slab,
@@ -143,22 +143,45 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const T* __restrict__ dy, l
     if (w && c < D) load_vec<W, VEC>(w + c, ww[k]);
   }
   const float inv = 1.f / (float)D;
-  for (long row = (long)blockIdx.x * RPB + grp; row < rows; row += (long)gridDim.x * RPB) {
+  // the next row is requested before the current one is worked on
+  using Piece = typename VecOf<T, VEC>::type;
+  Piece nx[NV], ng[NV];
+  float nm = 0.f, nr = 0.f;
+  auto request = [&](long row) {
     const T *xr = x + (size_t)row * ldx, *gr = dy + (size_t)row * lddy;
-    const float m = mean[row], r = rstd[row];
-    float h[NV][VEC], g[NV][VEC];
-    float s1 = 0.f, s2 = 0.f;
+    nm = mean[row];
+    nr = rstd[row];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
       const int c = (k * LANES + lane) * VEC;
       if (c < D) {
-        load_vec<T, VEC>(xr + c, h[k]);
-        load_vec<T, VEC>(gr + c, g[k]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) h[k][i] = m, g[k][i] = 0.f;
+        nx[k] = *reinterpret_cast<const Piece*>(xr + c);
+        ng[k] = *reinterpret_cast<const Piece*>(gr + c);
       }
     }
+  };
+  const long step = (long)gridDim.x * RPB;
+  long row = (long)blockIdx.x * RPB + grp;
+  if (row < rows) request(row);
+  for (; row < rows; row += step) {
+    const float m = nm, r = nr;
+    float h[NV][VEC], g[NV][VEC];
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const bool in = (k * LANES + lane) * VEC < D;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        if constexpr (VEC == 1) {
+          h[k][i] = in ? (float)nx[k] : m;
+          g[k][i] = in ? (float)ng[k] : 0.f;
+        } else {
+          h[k][i] = in ? (float)nx[k][i] : m;
+          g[k][i] = in ? (float)ng[k][i] : 0.f;
+        }
+      }
+    }
+    if (row + step < rows) request(row + step);
 #pragma unroll
     for (int k = 0; k < NV; ++k)
 #pragma unroll
@@ -179,7 +202,7 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const T* __restrict__ dy, l
       if (c >= D) continue;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) g[k][i] = r * (g[k][i] - s1 - h[k][i] * s2);
-      store_vec<T, VEC>(o + c, g[k]);
+      store_vec_nt<NT, T, VEC>(o + c, g[k]);
     }
   }
   if (!slab) return;
@@ -296,14 +319,19 @@ struct LnGeom {
   int vec, lanes, nv;   // lanes == 0: the wide kernels
 };
 
-// The narrowest group of lanes that holds the row.  `vec` is the 16-byte piece when every row of every tensor starts on a
+// The narrowest group of lanes that holds the row, a wave with at most `most` pieces per lane (forward 4; backward 2, since each
+// piece brings two gradient sums along: 65536 rows of 2048 bf16 values take 179 us with 64 lanes x 4 and 156 with 256 x 1).  `vec` is the 16-byte piece when every row of every tensor starts on a
 // 16-byte boundary and the width is a whole number of pieces, else single values.
-LnGeom ln_geom(int D, int vec) {
-  static const int shapes[][2] = {{16, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 2}, {256, 4}, {256, 8}};
+LnGeom ln_geom(int D, int vec, int most) {
+  static const int shapes[][2] = {{16, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 1}, {256, 2}, {256, 4}, {256, 8}};
   for (auto& s : shapes)
-    if ((long)s[0] * s[1] * vec >= D) return {vec, s[0], s[1]};
+    if ((s[0] == 256 || s[1] <= most) && (long)s[0] * s[1] * vec >= D) return {vec, s[0], s[1]};
   return {vec, 0, 0};
 }
+
+// Results of 128 MB and more are stored past the caches: their reader would not find them there, and the inputs keep the room
+// (65536 rows of 2048 bf16 values: 116 -> 91 us; no difference at 134 MB, nothing lost below).
+bool ln_past_caches(long rows, int D, int esize) { return rows * D * esize >= (1L << 27); }
 
 bool aligned16(const void* p) { return p == nullptr || ((uintptr_t)p & 15) == 0; }
 
@@ -319,44 +347,47 @@ int ln_vec(int D, long ld0, long ld1, std::initializer_list<const void*> ptrs) {
 // A grid holds at most 2^32 threads, so one launch of a workgroup per row covers at most this many rows.
 constexpr long LN_LAUNCH_ROWS = 1L << 23;
 
-#define LN_SHAPES(M, V)                                                     \
-  if (g.lanes == 16) M(V, 16, 1)                                            \
-  else if (g.lanes == 64 && g.nv == 1) M(V, 64, 1)                          \
-  else if (g.lanes == 64 && g.nv == 2) M(V, 64, 2)                          \
-  else if (g.lanes == 64) M(V, 64, 4)                                       \
-  else if (g.nv == 2) M(V, 256, 2)                                          \
-  else if (g.nv == 4) M(V, 256, 4)                                          \
-  else M(V, 256, 8)
+// M(vec, lanes, nv, nt) for the chosen shape; single values are never stored past the caches (rows narrower than a line)
+#define LN_SHAPES(M, V, NT)                                                 \
+  if (g.lanes == 16) M(V, 16, 1, NT)                                        \
+  else if (g.lanes == 64 && g.nv == 1) M(V, 64, 1, NT)                      \
+  else if (g.lanes == 64 && g.nv == 2) M(V, 64, 2, NT)                      \
+  else if (g.lanes == 64) M(V, 64, 4, NT)                                   \
+  else if (g.nv == 1) M(V, 256, 1, NT)                                      \
+  else if (g.nv == 2) M(V, 256, 2, NT)                                      \
+  else if (g.nv == 4) M(V, 256, 4, NT)                                      \
+  else M(V, 256, 8, NT)
+#define LN_PICK(M)                                       \
+  if (g.vec == V && nt) { LN_SHAPES(M, V, true) }        \
+  else if (g.vec == V) { LN_SHAPES(M, V, false) }        \
+  else { LN_SHAPES(M, 1, false) }
 
 template <typename T, typename W>
 void ln_fwd_rows(const LnGeom& g, const T* x, long ldx, const W* w, const W* b, float eps, T* y, float* mean, float* rstd,
-                 long rows, int D, hipStream_t st) {
+                 long rows, int D, bool nt, hipStream_t st) {
   constexpr int V = 16 / sizeof(T);
   if (g.lanes == 0) {
     hipLaunchKernelGGL((ln_fwd_wide_kernel<T, W>), dim3((unsigned)rows), dim3(256), 0, st, x, ldx, w, b, eps, y, mean, rstd, D);
     return;
   }
   const dim3 grid((unsigned)((rows + 256 / g.lanes - 1) / (256 / g.lanes)));
-#define LN_FWD(VV, L, N) hipLaunchKernelGGL((ln_fwd_kernel<T, W, VV, L, N>), grid, dim3(256), 0, st, x, ldx, w, b, eps, y, mean, rstd, rows, D);
-  if (g.vec == V) {
-    LN_SHAPES(LN_FWD, V)
-  } else {
-    LN_SHAPES(LN_FWD, 1)
-  }
+#define LN_FWD(VV, L, N, NT) hipLaunchKernelGGL((ln_fwd_kernel<T, W, VV, L, N, NT>), grid, dim3(256), 0, st, x, ldx, w, b, eps, y, mean, rstd, rows, D);
+  LN_PICK(LN_FWD)
 #undef LN_FWD
 }
 
 template <typename T, typename W>
 void ln_fwd(const void* x, long ldx, const void* w, const void* b, float eps, void* y, float* mean, float* rstd, long rows,
             int D, hipStream_t st) {
-  const LnGeom g = ln_geom(D, ln_vec<T>(D, ldx, D, {x, w, b, y}));
+  const LnGeom g = ln_geom(D, ln_vec<T>(D, ldx, D, {x, w, b, y}), 4);
+  const bool nt = ln_past_caches(rows, D, sizeof(T));
   const W *wp = (const W*)w, *bp = (const W*)b;
   for (const long all = rows; rows > 0; rows -= LN_LAUNCH_ROWS) {
     const long first = all - rows, n = rows < LN_LAUNCH_ROWS ? rows : LN_LAUNCH_ROWS;
     const T* xp = (const T*)x + first * ldx;
     T* yp = (T*)y + first * D;
     float *mp = mean ? mean + first : nullptr, *rp = rstd ? rstd + first : nullptr;
-    ln_fwd_rows<T, W>(g, xp, ldx, wp, bp, eps, yp, mp, rp, n, D, st);
+    ln_fwd_rows<T, W>(g, xp, ldx, wp, bp, eps, yp, mp, rp, n, D, nt, st);
   }
 }
 
@@ -364,7 +395,8 @@ template <typename T, typename W>
 void ln_bwd(const void* dy, long lddy, const void* x, long ldx, const float* mean, const float* rstd, const void* w, void* dx,
             void* dw, void* db, float* slab, long rows, int D, hipStream_t st) {
   constexpr int V = 16 / sizeof(T);
-  const LnGeom g = ln_geom(D, ln_vec<T>(D, ldx, lddy, {dy, x, w, dx}));
+  const LnGeom g = ln_geom(D, ln_vec<T>(D, ldx, lddy, {dy, x, w, dx}), 2);
+  const bool nt = ln_past_caches(rows, D, sizeof(T));
   const T *xp = (const T*)x, *gp = (const T*)dy;
   const W* wp = (const W*)w;
   T* dp = (T*)dx;
@@ -378,14 +410,12 @@ void ln_bwd(const void* dy, long lddy, const void* x, long ldx, const float* mea
     if (sl)
       hipLaunchKernelGGL((ln_bwd_cols_kernel<T>), dim3(noise_cdiv(D, 256), nslab), dim3(256), 0, st, gp, lddy, xp, ldx, mean, rstd, sl, rows, D);
   } else {
-    nslab = noise_grid(rows, 256 / g.lanes, LN_BWD_GRID);
+    // Measured with 256 / 512 / 1024 / 2048 workgroups: 65536 x 1024 bf16 (64 lanes x 2) 107 / 67 / 78 / 83 us, 65536 x 2048 bf16
+    // (256 x 1) - / 159 / 153 / 173, 16384 x 8192 bf16 (256 x 4) 145 / 153 / - / 167
+    nslab = noise_grid(rows, 256 / g.lanes, g.lanes < 256 ? LN_BWD_GRID / 2 : g.nv == 1 ? LN_BWD_GRID : LN_BWD_GRID / 4);
     const dim3 grid(nslab);
-#define LN_BWD(VV, L, N) hipLaunchKernelGGL((ln_bwd_kernel<T, W, VV, L, N>), grid, dim3(256), 0, st, gp, lddy, xp, ldx, mean, rstd, wp, dp, sl, rows, D);
-    if (g.vec == V) {
-      LN_SHAPES(LN_BWD, V)
-    } else {
-      LN_SHAPES(LN_BWD, 1)
-    }
+#define LN_BWD(VV, L, N, NT) hipLaunchKernelGGL((ln_bwd_kernel<T, W, VV, L, N, NT>), grid, dim3(256), 0, st, gp, lddy, xp, ldx, mean, rstd, wp, dp, sl, rows, D);
+    LN_PICK(LN_BWD)
 #undef LN_BWD
   }
   if (sl) {

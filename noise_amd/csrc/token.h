@@ -48,6 +48,19 @@ __device__ __forceinline__ void store_vec(T* p, const float (&in)[V]) {
   }
 }
 
+// The same store past the caches (NT): for results larger than the last-level cache could keep for their reader.
+template <bool NT, typename T, int V>
+__device__ __forceinline__ void store_vec_nt(T* p, const float (&in)[V]) {
+  if constexpr (!NT || V == 1) {
+    store_vec<T, V>(p, in);
+  } else {
+    typename VecOf<T, V>::type v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (T)in[i];
+    __builtin_nontemporal_store(v, reinterpret_cast<typename VecOf<T, V>::type*>(p));
+  }
+}
+
 template <int CTRL>
 __device__ __forceinline__ float dpp_move(float v) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
