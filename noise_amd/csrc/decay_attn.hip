@@ -664,16 +664,27 @@ __global__ __launch_bounds__(256) void step_kernel(const T* __restrict__ q, Stri
     vv[i] = (float)vp[c + i];
   }
   if (grp < groups) {
-    for (int r = grp; r < dk; r += groups) {
-      const float kr = (float)kp[r], qr = (float)qp[r];
-      float x[V];
-      load_vec<float, V>(sp + (size_t)r * dv + c, x);
+    // four rows requested before the first is worked on
+    for (int r0 = grp; r0 < dk; r0 += 4 * groups) {
+      float x[4][V], kr[4], qr[4];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        x[i] = x[i] * lam + kr * vv[i];
-        acc[i] += qr * x[i];
+      for (int u = 0; u < 4; ++u) {
+        const int r = min(r0 + u * groups, dk - 1);
+        load_vec<float, V>(sp + (size_t)r * dv + c, x[u]);
+        kr[u] = (float)kp[r];
+        qr[u] = (float)qp[r];
       }
-      store_vec<float, V>(sp + (size_t)r * dv + c, x);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int r = r0 + u * groups;
+        if (r >= dk) break;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          x[u][i] = x[u][i] * lam + kr[u] * vv[i];
+          acc[i] += qr[u] * x[u][i];
+        }
+        store_vec<float, V>(sp + (size_t)r * dv + c, x[u]);
+      }
     }
   }
 #pragma unroll

@@ -27,66 +27,80 @@ __device__ __forceinline__ float row_sum(float v, float* red, int& phase) {
   }
 }
 
+// A lane group works on `per` rows one after the other, RPB apart, with the parameters in registers and the next row
+// requested ahead: at one row each, 16 KB of weights and biases come from L2 for every 4 KB row of 2048 bf16 values.
 template <typename T, typename W, int VEC, int LANES, int NV, bool NT>
 __global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, long ldx, const W* __restrict__ w,
                                                      const W* __restrict__ b, float eps, T* __restrict__ y,
-                                                     float* __restrict__ mean, float* __restrict__ rstd, long rows, int D) {
+                                                     float* __restrict__ mean, float* __restrict__ rstd, long rows, int D,
+                                                     int per) {
   constexpr int RPB = 256 / LANES;
   __shared__ float red[8];
   int phase = 0;
   const int lane = threadIdx.x % LANES;
-  const long row = (long)blockIdx.x * RPB + threadIdx.x / LANES;
-  if (LANES <= 64 && row >= rows) return;
-  const T* xr = x + (size_t)row * ldx;
-  float v[NV][VEC];
-  float s = 0.f;
+  long row = (long)blockIdx.x * RPB * per + threadIdx.x / LANES;
+  if (row >= rows) return;                                    // LANES == 256: the whole workgroup
+  const long end = min(rows, row + (long)RPB * per);
+  using Piece = typename VecOf<T, VEC>::type;
+  Piece next[NV];
+  auto request = [&](long r) {
+    const T* xr = x + (size_t)r * ldx;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * LANES + lane) * VEC;
+      if (c < D) next[k] = *reinterpret_cast<const Piece*>(xr + c);
+    }
+  };
+  request(row);
+  float ww[NV][VEC], bb[NV][VEC];
 #pragma unroll
   for (int k = 0; k < NV; ++k) {
     const int c = (k * LANES + lane) * VEC;
-    if (c < D) {
-      load_vec<T, VEC>(xr + c, v[k]);
-    } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[k][i] = 0.f;
-    }
+    for (int i = 0; i < VEC; ++i) ww[k][i] = 1.f, bb[k][i] = 0.f;
+    if (w && c < D) load_vec<W, VEC>(w + c, ww[k]);
+    if (b && c < D) load_vec<W, VEC>(b + c, bb[k]);
   }
-#pragma unroll
-  for (int k = 0; k < NV; ++k)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) s += v[k][i];
   const float inv = 1.f / (float)D;
-  const float m = row_sum<LANES>(s, red, phase) * inv;
-  float q = 0.f;
+  for (; row < end; row += RPB) {
+    float v[NV][VEC];
+    float s = 0.f;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const bool in = (k * LANES + lane) * VEC < D;
+    for (int k = 0; k < NV; ++k) {
+      const bool in = (k * LANES + lane) * VEC < D;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      v[k][i] = v[k][i] - m;
-      q += in ? v[k][i] * v[k][i] : 0.f;
+      for (int i = 0; i < VEC; ++i) {
+        if constexpr (VEC == 1) v[k][i] = in ? (float)next[k] : 0.f;
+        else v[k][i] = in ? (float)next[k][i] : 0.f;
+        s += v[k][i];
+      }
     }
-  }
-  const float r = 1.f / sqrtf(row_sum<LANES>(q, red, phase) * inv + eps);
-  T* yr = y + (size_t)row * D;
+    if (row + RPB < end) request(row + RPB);
+    const float m = row_sum<LANES>(s, red, phase) * inv;
+    float q = 0.f;
 #pragma unroll
-  for (int k = 0; k < NV; ++k) {
-    const int c = (k * LANES + lane) * VEC;
-    if (c >= D) continue;
-    float ww[VEC], bb[VEC];
-    if (w) load_vec<W, VEC>(w + c, ww);
-    if (b) load_vec<W, VEC>(b + c, bb);
+    for (int k = 0; k < NV; ++k) {
+      const bool in = (k * LANES + lane) * VEC < D;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      float o = v[k][i] * r;
-      if (w) o *= ww[i];
-      if (b) o += bb[i];
-      v[k][i] = o;
+      for (int i = 0; i < VEC; ++i) {
+        v[k][i] = v[k][i] - m;
+        q += in ? v[k][i] * v[k][i] : 0.f;
+      }
     }
-    store_vec_nt<NT, T, VEC>(yr + c, v[k]);
-  }
-  if (lane == 0) {
-    if (mean) mean[row] = m;
-    if (rstd) rstd[row] = r;
+    const float r = 1.f / sqrtf(row_sum<LANES>(q, red, phase) * inv + eps);
+    T* yr = y + (size_t)row * D;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const int c = (k * LANES + lane) * VEC;
+      if (c >= D) continue;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[k][i] = v[k][i] * r * ww[k][i] + bb[k][i];
+      store_vec_nt<NT, T, VEC>(yr + c, v[k]);
+    }
+    if (lane == 0) {
+      if (mean) mean[row] = m;
+      if (rstd) rstd[row] = r;
+    }
   }
 }
 
@@ -323,7 +337,7 @@ struct LnGeom {
 // piece brings two gradient sums along: 65536 rows of 2048 bf16 values take 179 us with 64 lanes x 4 and 156 with 256 x 1).  `vec` is the 16-byte piece when every row of every tensor starts on a
 // 16-byte boundary and the width is a whole number of pieces, else single values.
 LnGeom ln_geom(int D, int vec, int most) {
-  static const int shapes[][2] = {{16, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 1}, {256, 2}, {256, 4}, {256, 8}};
+  static const int shapes[][2] = {{16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 1}, {256, 2}, {256, 4}, {256, 8}};
   for (auto& s : shapes)
     if ((s[0] == 256 || s[1] <= most) && (long)s[0] * s[1] * vec >= D) return {vec, s[0], s[1]};
   return {vec, 0, 0};
@@ -347,9 +361,15 @@ int ln_vec(int D, long ld0, long ld1, std::initializer_list<const void*> ptrs) {
 // A grid holds at most 2^32 threads, so one launch of a workgroup per row covers at most this many rows.
 constexpr long LN_LAUNCH_ROWS = 1L << 23;
 
+// Rows per lane group of a forward call, where 2048 workgroups remain: more of them amortise the parameters, fewer keep the
+// accesses in flight close together.  1 / 2 / 4 / 8 rows: 65536 x 2048 bf16 107 / 93 / 99 / 109 us, 16384 x 8192 bf16 - / 96 / 98 /
+// 109, 524288 x 128 fp32 - / 93 / 97 / 97.
+constexpr int LN_FWD_PER = 2, LN_FWD_FULL = 2048;
+
 // M(vec, lanes, nv, nt) for the chosen shape; single values are never stored past the caches (rows narrower than a line)
 #define LN_SHAPES(M, V, NT)                                                 \
   if (g.lanes == 16) M(V, 16, 1, NT)                                        \
+  else if (g.lanes == 32) M(V, 32, 1, NT)                                   \
   else if (g.lanes == 64 && g.nv == 1) M(V, 64, 1, NT)                      \
   else if (g.lanes == 64 && g.nv == 2) M(V, 64, 2, NT)                      \
   else if (g.lanes == 64) M(V, 64, 4, NT)                                   \
@@ -370,8 +390,10 @@ void ln_fwd_rows(const LnGeom& g, const T* x, long ldx, const W* w, const W* b, 
     hipLaunchKernelGGL((ln_fwd_wide_kernel<T, W>), dim3((unsigned)rows), dim3(256), 0, st, x, ldx, w, b, eps, y, mean, rstd, D);
     return;
   }
-  const dim3 grid((unsigned)((rows + 256 / g.lanes - 1) / (256 / g.lanes)));
-#define LN_FWD(VV, L, N, NT) hipLaunchKernelGGL((ln_fwd_kernel<T, W, VV, L, N, NT>), grid, dim3(256), 0, st, x, ldx, w, b, eps, y, mean, rstd, rows, D);
+  const long rpb = 256 / g.lanes, groups = (rows + rpb - 1) / rpb;
+  const int per = groups >= (long)LN_FWD_FULL * LN_FWD_PER ? LN_FWD_PER : 1;
+  const dim3 grid((unsigned)((groups + per - 1) / per));
+#define LN_FWD(VV, L, N, NT) hipLaunchKernelGGL((ln_fwd_kernel<T, W, VV, L, N, NT>), grid, dim3(256), 0, st, x, ldx, w, b, eps, y, mean, rstd, rows, D, per);
   LN_PICK(LN_FWD)
 #undef LN_FWD
 }
