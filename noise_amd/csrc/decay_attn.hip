@@ -123,11 +123,7 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
       rv[s] = row4(vb + t * w.sv.t, live, c, w.dv, w.vv);
     }
   };
-  fetch(p0);
-  for (int c0 = p0; c0 < p1; c0 += DA_C) {
-    const int n = min(DA_C, p1 - c0);                       // tokens in this chunk
-    const int shift = w.shift && c0 == 0 ? 1 : 0;
-    __syncthreads();                                        // the previous chunk's readers are done
+  auto put = [&]() {
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
       const int i = (s * NTHR + tid) / (P / 4), c = (s * NTHR + tid) % (P / 4) * 4;
@@ -135,6 +131,12 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
       *(f32x4*)(sk + i * LD + c) = rk[s];
       *(f32x4*)(sv + i * LD + c) = rv[s];
     }
+  };
+  fetch(p0);
+  put();
+  for (int c0 = p0; c0 < p1; c0 += DA_C) {
+    const int n = min(DA_C, p1 - c0);                       // tokens in this chunk
+    const int shift = w.shift && c0 == 0 ? 1 : 0;
     __syncthreads();
     if (c0 + DA_C < p1) fetch(c0 + DA_C);
     f32x4 O[2][NT];
@@ -219,6 +221,8 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
         }
       }
     }
+    __syncthreads();                                        // every wave is done with the tiles
+    if (c0 + DA_C < p1) put();                              // before this chunk's stores, which nobody waits for then
     if (!STATE_ONLY) {
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
@@ -326,23 +330,24 @@ __device__ __forceinline__ int scale_for(float bound, int top) { return max(min(
 // Rows of a chunk as a buffer: accesses behind its end read zero and store nothing, so that neither the clip's last chunk nor
 // columns behind the head need a branch.  `rows` of them, `stride` elements apart, `width` elements each.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_rows(const void* first, int rows, long stride, int width) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)first, 0, (int)(((rows - 1) * stride + width) * 2), 0x00020000);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)first, 0, rows > 0 ? (int)(((rows - 1) * stride + width) * 2) : 0, 0x00020000);
 }
 // A byte offset into such a buffer; one before its start, or of a column that does not exist, lands far behind its end.
 __device__ __forceinline__ int chunk_offset(int off, bool exists) { return (int)min((unsigned)(exists ? off : -1), 0x80000000u); }
 
 // VEC: every row of a, k, v and o starts on a 16-byte boundary, rows do not overlap and a chunk spans less than 2 GB.
-template <typename T, int P, bool STATE_ONLY, bool VEC>
+template <typename T, int P, int CC, bool STATE_ONLY, bool VEC>
 __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkArgs w) {
   constexpr bool F16 = __is_same(T, f16_t);
+  constexpr int C = CC, NI = C / 16, TILES = NI * (NI + 1) / 2;
   constexpr int NTHR = P * 4, NW = P / 16, KP = P / 32;      // KP: pairs of state row tiles
-  constexpr int LD = P + 16, LDP = DB_C + 8, SLOTS = DB_C * P / 8 / NTHR;
-  __shared__ __attribute__((aligned(16))) T sa[STATE_ONLY ? 8 : DB_C * LD];
-  __shared__ __attribute__((aligned(16))) T sk[DB_C * LD], sv[DB_C * LD];
-  __shared__ __attribute__((aligned(16))) T sp[STATE_ONLY ? 8 : DB_C * LDP];
-  __shared__ float pw[DB_C + 1];                             // lam^i
-  __shared__ float pv[2 * DB_C];                             // s_kv lam^{63-i}; a chunk of n tokens starts at 64 - n
-  __shared__ float pp[DB_C + 16];                            // [15 + i - j]: s_o s_kv lam^{i-j}
+  constexpr int LD = P + 16, LDP = C + 8, SLOTS = C * P / 8 / NTHR;
+  __shared__ __attribute__((aligned(16))) T sa[STATE_ONLY ? 8 : C * LD];
+  __shared__ __attribute__((aligned(16))) T sk[C * LD], sv[C * LD];
+  __shared__ __attribute__((aligned(16))) T sp[STATE_ONLY ? 8 : C * LDP];
+  __shared__ float pw[C + 1];                             // lam^i
+  __shared__ float pv[2 * C];                             // s_kv lam^{63-i}; a chunk of n tokens starts at 64 - n
+  __shared__ float pp[C + 16];                            // [15 + i - j]: s_o s_kv lam^{i-j}
   __shared__ unsigned top[F16 ? 3 * NW : 1];                 // largest a, k, v of the waves' pieces, as bits
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, q = lane >> 4, l16 = lane & 15;
   const int bh = blockIdx.x % (w.B * w.H), seg = blockIdx.x / (w.B * w.H);
@@ -358,14 +363,14 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkAr
   }
   if (STATE_ONLY ? seg >= last_seg : seg > last_seg) return;
   const float g2 = w.log_decay[h] * 1.44269504088896341f;
-  for (int i = tid; i < 2 * DB_C; i += NTHR) {
-    if (i <= DB_C) pw[i] = decay_pow(g2, i);
-    if (i < DB_C + 16) pp[i] = w.s_o * w.s_kv * decay_pow(g2, i - 15);
-    pv[i] = w.s_kv * decay_pow(g2, DB_C - 1 - i);
+  for (int i = tid; i < 2 * C; i += NTHR) {
+    if (i <= C) pw[i] = decay_pow(g2, i);
+    if (i < C + 16) pp[i] = w.s_o * w.s_kv * decay_pow(g2, i - 15);
+    pv[i] = w.s_kv * decay_pow(g2, C - 1 - i);
   }
   if (!STATE_ONLY) {
     // the weight tiles (0, 1) and (2, 3) lie above the diagonal but in a pair that is read: they stay zero
-    for (int i = tid; i < 32 * 16; i += NTHR) {
+    for (int i = tid; i < C / 32 * 256; i += NTHR) {
       const int half = i >> 8, r = i >> 4 & 15, c = i & 15;
       sp[(half * 32 + r) * LDP + half * 32 + 16 + c] = (T)0.f;
     }
@@ -413,7 +418,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkAr
   const int dir = w.reverse ? -1 : 1;
   u32x4 ra[STATE_ONLY ? 1 : SLOTS], rk[SLOTS], rv[SLOTS];
   auto rows8 = [&](const T* base, const Strides& st, int width, bool vec, int c0, u32x4 (&out)[SLOTS]) {
-    const int n = min(DB_C, p1 - c0);
+    const int n = min(C, p1 - c0);                       // none or fewer behind the last chunk
     if (VEC) {
       const auto rs = chunk_rows(base + (w.reverse ? len - c0 - n : c0) * st.t, n, st.t, width);
       const int step = dir * RS * 2 * (int)st.t;
@@ -435,10 +440,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkAr
     rows8(kb, w.sk, w.dk, w.vk, c0, rk);
     rows8(vb, w.sv, w.dv, w.vv, c0, rv);
   };
-  if (p0 < p1) fetch(p0);
-  for (int c0 = p0; c0 < p1; c0 += DB_C) {
-    const int n = min(DB_C, p1 - c0);                       // tokens in this chunk
-    const int shift = w.shift && c0 == 0 ? 1 : 0;
+  auto put = [&]() {
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
       const int at = (i0 + s * RS) * LD + cc;
@@ -466,8 +468,16 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkAr
         if (lane == 0) top[z * NW + wave] = u;
       }
     }
+  };
+  if (p0 < p1) {
+    fetch(p0);
+    put();
+  }
+  for (int c0 = p0; c0 < p1; c0 += C) {
+    const int n = min(C, p1 - c0);                       // tokens in this chunk
+    const int shift = w.shift && c0 == 0 ? 1 : 0;
     __syncthreads();
-    if (c0 + DB_C < p1) fetch(c0 + DB_C);
+    if (P < 128 || c0 + C < p1) fetch(c0 + C);              // behind the last chunk: zeros, without an access
     float unit_p = 1.f, unit_x = 1.f, back = 1.f, unit_v = 1.f, carry = 1.f, largest = 0.f;
     if constexpr (F16) {
       float big[3];
@@ -488,14 +498,14 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkAr
       E = ev;
       largest = fabsf(w.s_kv) * big[1] * big[2] * (float)n;
     }
-    f32x4 O[STATE_ONLY ? 1 : 4];
+    f32x4 O[STATE_ONLY ? 1 : NI];
     if (!STATE_ONLY) {
-      // ---- weights, transposed tile by tile (rows j, columns i) so that a lane holds four neighbouring j of one i: the ten
+      // ---- weights, transposed tile by tile (rows j, columns i) so that a lane holds four neighbouring j of one i: the
       // 16 x 16 tiles on and below the diagonal, in the order (0,0) (1,0) (1,1) (2,0) ..., are dealt over the waves
 #pragma unroll P == 128 ? 1 : 5   // eight waves have two tiles at most, and no registers for both at once
-      for (int u = 0; u * NW < 10; ++u) {
+      for (int u = 0; u * NW < TILES; ++u) {
         const int tile = u * NW + wave;
-        if ((u + 1) * NW > 10 && tile >= 10) break;
+        if ((u + 1) * NW > TILES && tile >= TILES) break;
         const int it = 0xffa94 >> (2 * tile) & 3, jt = tile - it * (it + 1) / 2;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -507,14 +517,19 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkAr
           acc = mfma16(x, y, acc);
         }
         const int i = it * 16 + l16, j = jt * 16 + 4 * q;
-        const bool diag = it == jt;
+        float f[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[r] = diag && l16 < 4 * q + r ? 0.f : acc[r] * (F16 ? unit_p * pp[15 + i - j - r] : pp[15 + i - j - r]);
+        for (int r = 0; r < 4; ++r) f[r] = pp[15 + i - j - r];
+        // all four are read, whether they count or not: a branch around each would wait for each
+        asm("" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]));
+        const int last = it == jt ? l16 - 4 * q : 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[r] = r <= last ? acc[r] * (F16 ? unit_p * f[r] : f[r]) : 0.f;
         *(uint2*)(sp + i * LDP + j) = make_uint2(pack16<T>(acc[0], acc[1]), pack16<T>(acc[2], acc[3]));
       }
       // ---- what the state contributes, transposed: rows are the wave's columns, columns the tokens
 #pragma unroll
-      for (int it = 0; it < 4; ++it) O[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int it = 0; it < NI; ++it) O[it] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kp = 0; kp < KP; ++kp) {
         u32x4 u;
@@ -525,16 +540,16 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkAr
         }
         const x8<T> x = __builtin_bit_cast(x8<T>, u);
 #pragma unroll
-        for (int it = 0; it < 4; ++it) {
+        for (int it = 0; it < NI; ++it) {
           const x8<T> y = *(const x8<T>*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
           O[it] = mfma16(x, y, O[it]);
         }
       }
 #pragma unroll
-      for (int it = 0; it < 4; ++it) O[it] *= w.s_o * pw[it * 16 + l16 + 1 - shift] * back;
+      for (int it = 0; it < NI; ++it) O[it] *= w.s_o * pw[it * 16 + l16 + 1 - shift] * back;
     }
     // ---- X = lam^n X + K^T V'
-    x8<T> v[2];
+    x8<T> v[C / 32];
     const float f = pw[n - shift] * carry;
     if constexpr (F16) bound = bound * pw[n - shift] + largest;
 #pragma unroll
@@ -542,10 +557,10 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkAr
 #pragma unroll
       for (int s = 0; s < 2; ++s) X[kp][s] *= f;
 #pragma unroll
-    for (int jj = 0; jj < 2; ++jj) {
+    for (int jj = 0; jj < C / 32; ++jj) {
       v[jj] = read_tokens<LD, T>(sv + jj * 32 * LD + col0, q, l16);
       u32x4 t[3];
-      const float* f8 = pv + DB_C - n + jj * 32 + 8 * q;
+      const float* f8 = pv + C - n + jj * 32 + 8 * q;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const unsigned u = __builtin_bit_cast(u32x4, v[jj])[e];
@@ -576,16 +591,21 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkAr
     if (!STATE_ONLY) {
       // ---- O += P V
 #pragma unroll
-      for (int jj = 0; jj < 2; ++jj)
+      for (int jj = 0; jj < C / 32; ++jj)
 #pragma unroll
-        for (int it = 2 * jj; it < 4; ++it) {
+        for (int it = 2 * jj; it < NI; ++it) {
           const x8<T> y = *(const x8<T>*)(sp + (it * 16 + l16) * LDP + jj * 32 + 8 * q);
           O[it] = mfma16(v[jj], y, O[it]);
         }
+    }
+    // the next tiles go in before this chunk's rows go out: waiting for loads that are older than a store is not waiting for the
+    // store (memory operations are counted in order).  Wide heads have no registers to hold both, and other waves to run.
+    if constexpr (P < 128) put();
+    if (!STATE_ONLY) {
       const int col = col0 + 4 * q;
       const auto rs = chunk_rows(ob + (w.reverse ? len - c0 - n : c0) * w.so.t, n, w.so.t, w.dv);
 #pragma unroll
-      for (int it = 0; it < 4; ++it) {
+      for (int it = 0; it < NI; ++it) {
         const int i = it * 16 + l16;
         if constexpr (F16) O[it] *= 1.f / unit_p;
         const u32x2 y = {pack16<T>(O[it][0], O[it][1]), pack16<T>(O[it][2], O[it][3])};
@@ -601,6 +621,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkAr
         }
       }
     }
+    if constexpr (P == 128) put();
   }
   // ---- state behind the segment
   float* dst = STATE_ONLY ? w.seg + ((size_t)bh * w.nseg + seg) * mat : seg == last_seg && w.x_end ? w.x_end + (size_t)bh * mat : nullptr;
@@ -738,16 +759,16 @@ void walk_launch_16(const WalkArgs& w, hipStream_t st) {
   const int d = w.dk > w.dv ? w.dk : w.dv;
   const unsigned grid = (unsigned)w.B * w.H * w.nseg;
   const bool vec = w.va && w.vk && w.vv && w.vo;
-#define GO(P, ONLY)                                                                                         \
+#define GO(P, C, ONLY)                                                                                      \
   do {                                                                                                      \
-    if (vec) hipLaunchKernelGGL((walk_16_kernel<T, P, ONLY, true>), dim3(grid), dim3(P * 4), 0, st, w);     \
-    else hipLaunchKernelGGL((walk_16_kernel<T, P, ONLY, false>), dim3(grid), dim3(P * 4), 0, st, w);        \
+    if (vec) hipLaunchKernelGGL((walk_16_kernel<T, P, C, ONLY, true>), dim3(grid), dim3(P * 4), 0, st, w);  \
+    else hipLaunchKernelGGL((walk_16_kernel<T, P, C, ONLY, false>), dim3(grid), dim3(P * 4), 0, st, w);     \
   } while (0)
 #define PICK(ONLY)             \
   do {                         \
-    if (d <= 32) GO(32, ONLY); \
-    else if (d <= 64) GO(64, ONLY); \
-    else GO(128, ONLY);        \
+    if (d <= 32) GO(32, 64, ONLY); \
+    else if (d <= 64) GO(64, 64, ONLY); \
+    else GO(128, 32, ONLY);    \
   } while (0)
   if (w.nseg > 1 && !w.seg_tr) {
     PICK(true);
