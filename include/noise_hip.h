@@ -393,7 +393,8 @@ int noise_layer_norm_bwd(const void* dy, long lddy, const void* x, long ldx, con
 
 /* ---- decay attention: causal linear attention with one decay per head ---------------------------- */
 /* X_p = e^g X_{p-1} + s_kv k_p (x) v_p, o_p = s_o a_p X_p over p < length; a, k [B][T][H][dk], v, o [B][T][H][dv] by strides
- * (elements between clips, tokens, heads of a, k, v, o: 12 values on the HOST; unit stride on the last axis); rows of o at
+ * (elements between clips, tokens, heads of a, k, v, o: 12 values on the HOST; unit stride on the last axis, a token stride
+ * of at least the row's width and below 2^22); rows of o at
  * and behind the length are zero.  log_decay g [H] <= 0; lengths [B] or NULL (all T); x0, x_end [B][H][dk][dv] fp32 or NULL
  * (x0_transposed: x0 is [B][H][dv][dk]).  reverse != 0: last token first, x0 meets the last token undecayed and x_end gets
  * one more decay (the gradient of the state before the first token).  1 <= dk, dv <= 128.

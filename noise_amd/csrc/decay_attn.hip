@@ -40,38 +40,39 @@ struct WalkArgs {
   int B, T, H, dk, dv, nseg, seg_len;
   int reverse, shift, end_decay, x0_tr;
   int seg_tr;               // seg holds the states of the walk with k and v swapped, [dv][dk] each: nothing to sum
-  int va, vk, vv, vo;       // rows allow wide accesses: rows_buffer for 16-bit types, four elements at a time for fp32
+  int va, vk, vv, vo;       // rows allow 16-byte accesses
 };
 
 __device__ __forceinline__ float decay_pow(float g2, int n) { return n <= 0 ? 1.f : exp2f(g2 * (float)n); }
 
-// Four elements of a token row, zero outside the row's width or behind the clip's end.
-__device__ __forceinline__ f32x4 row4(const float* base, bool live, int c, int width, bool vec) {
-  f32x4 r = {0.f, 0.f, 0.f, 0.f};
-  if (!live) return r;
-  if (vec && c + 4 <= width) {
-    r = *reinterpret_cast<const f32x4*>(base + c);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (c + i < width) r[i] = base[c + i];
-  }
-  return r;
+using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
+using u32x2 = __attribute__((ext_vector_type(2))) unsigned;
+
+// Rows of a chunk as a buffer: accesses behind its end read zero and store nothing, so that neither the clip's last chunk nor
+// columns behind the head need a branch.  `rows` of them, `stride` elements of `esize` bytes apart, `width` elements each.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_rows(const void* first, int rows, long stride, int width, int esize) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)first, 0, rows > 0 ? (int)(((rows - 1) * stride + width) * esize) : 0, 0x00020000);
 }
+// A byte offset into such a buffer; one before its start, or of a column that does not exist, lands far behind its end.
+__device__ __forceinline__ int chunk_offset(int off, bool exists) { return (int)min((unsigned)(exists ? off : -1), 0x80000000u); }
 
 // fp32 arithmetic throughout (v_mfma_f32_16x16x4_f32).  P: dk and dv padded to 16, 32, 64 or 128; P / 16 waves up to four,
 // each owning 16 NT of the P state columns.  The contraction index of an MFMA may be permuted as long as both operands agree:
 // lane quarter q takes elements 4q..4q+3 of a 16-wide block over four consecutive instructions, so row-major operands are
 // 16-byte LDS reads and an accumulator tile (row 4q + r in register r) is the next product's operand as it lies: the state
-// never leaves its registers.  Only the C x C weights pass through LDS (each wave computes a share of them).
-template <int P, bool STATE_ONLY>
+// never leaves its registers.  Weights and outputs are computed transposed, so that a lane holds four neighbours of a row.  Only
+// the C x C weights pass through LDS (each wave computes a share of them).
+// VEC: rows of a, k, v and o allow 16-byte accesses; otherwise elements go one by one, through the same buffers.
+template <int P, bool STATE_ONLY, bool VEC>
 __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_f32_kernel(WalkArgs w) {
   constexpr int NW = P >= 64 ? 4 : P / 16, NT = P / 16 / NW, KT = P / 16, NTHR = NW * 64;
-  constexpr int LD = P + 4, LDP = DA_C + 4, SLOTS = DA_C * P / 4 / NTHR;
-  __shared__ float sa[STATE_ONLY ? 4 : DA_C * LD];
-  __shared__ float sk[DA_C * LD], sv[DA_C * LD];
-  __shared__ float sp[STATE_ONLY ? 4 : DA_C * LDP];
-  __shared__ float pw[DA_C + 1];
+  constexpr int LD = P + 4, LDP = DA_C + 4, SLOTS = DA_C * P / 4 / NTHR, RS = NTHR / (P / 4);
+  __shared__ __attribute__((aligned(16))) float sa[STATE_ONLY ? 4 : DA_C * LD];
+  __shared__ __attribute__((aligned(16))) float sk[DA_C * LD], sv[DA_C * LD];
+  __shared__ __attribute__((aligned(16))) float sp[STATE_ONLY ? 4 : DA_C * LDP];
+  __shared__ float pw[DA_C + 1];                             // lam^i
+  __shared__ float pv[2 * DA_C];                             // s_kv lam^{31-i}; a chunk of n tokens starts at 32 - n
+  __shared__ float pp[DA_C + 16];                            // [15 + i - j]: s_o s_kv lam^{i-j}
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, q = lane >> 4, l16 = lane & 15;
   const int bh = blockIdx.x % (w.B * w.H), seg = blockIdx.x / (w.B * w.H);
   const int b = bh / w.H, h = bh % w.H;
@@ -86,12 +87,16 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
   }
   if (STATE_ONLY ? seg >= last_seg : seg > last_seg) return;
   const float g2 = w.log_decay[h] * 1.44269504088896341f;
-  if (tid <= DA_C) pw[tid] = decay_pow(g2, tid);
+  for (int i = tid; i < 2 * DA_C; i += NTHR) {
+    if (i <= DA_C) pw[i] = decay_pow(g2, i);
+    if (i < DA_C + 16) pp[i] = w.s_o * w.s_kv * decay_pow(g2, i - 15);
+    pv[i] = w.s_kv * decay_pow(g2, DA_C - 1 - i);
+  }
   const float* ab = (const float*)w.a + (size_t)b * w.sa.b + (size_t)h * w.sa.h;
   const float* kb = (const float*)w.k + (size_t)b * w.sk.b + (size_t)h * w.sk.h;
   const float* vb = (const float*)w.v + (size_t)b * w.sv.b + (size_t)h * w.sv.h;
 
-  // ---- state before the segment
+  // ---- state before the segment: X[kt][nt][r] = row kt 16 + 4q + r, column (wave NT + nt) 16 + l
   f32x4 X[KT][NT];
   const size_t mat = (size_t)w.dk * w.dv;
   {
@@ -110,38 +115,53 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
         }
   }
 
+  // a thread's SLOTS pieces of a tile are RS rows apart, in the same column
+  const int i0 = tid / (P / 4), cc = tid % (P / 4) * 4;
+  const int dir = w.reverse ? -1 : 1;
   f32x4 ra[STATE_ONLY ? 1 : SLOTS], rk[SLOTS], rv[SLOTS];
-  auto fetch = [&](int c0) {
+  auto rows4 = [&](const float* base, const Strides& st, int width, int c0, f32x4 (&out)[SLOTS]) {
+    const int n = min(DA_C, p1 - c0);                       // none or fewer behind the last chunk
+    const auto rs = chunk_rows(base + (w.reverse ? len - c0 - n : c0) * st.t, n, st.t, width, 4);
+    const int step = dir * RS * 4 * (int)st.t;
+    int off = (w.reverse ? n - 1 - i0 : i0) * 4 * (int)st.t + 4 * cc;
 #pragma unroll
-    for (int s = 0; s < SLOTS; ++s) {
-      const int i = (s * NTHR + tid) / (P / 4), c = (s * NTHR + tid) % (P / 4) * 4;
-      const int p = c0 + i;
-      const bool live = p < p1;
-      const long t = live ? (w.reverse ? len - 1 - p : p) : 0;
-      if (!STATE_ONLY) ra[s] = row4(ab + t * w.sa.t, live, c, w.dk, w.va);
-      rk[s] = row4(kb + t * w.sk.t, live, c, w.dk, w.vk);
-      rv[s] = row4(vb + t * w.sv.t, live, c, w.dv, w.vv);
+    for (int s = 0; s < SLOTS; ++s, off += step) {
+      if (VEC) {
+        out[s] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, chunk_offset(off, cc < width), 0, 0));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          out[s][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, chunk_offset(off < 0 ? off : off + 4 * e, cc + e < width), 0, 0));
+      }
     }
+  };
+  auto fetch = [&](int c0) {
+    if constexpr (!STATE_ONLY) rows4(ab, w.sa, w.dk, c0, ra);
+    rows4(kb, w.sk, w.dk, c0, rk);
+    rows4(vb, w.sv, w.dv, c0, rv);
   };
   auto put = [&]() {
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
-      const int i = (s * NTHR + tid) / (P / 4), c = (s * NTHR + tid) % (P / 4) * 4;
-      if (!STATE_ONLY) *(f32x4*)(sa + i * LD + c) = ra[s];
-      *(f32x4*)(sk + i * LD + c) = rk[s];
-      *(f32x4*)(sv + i * LD + c) = rv[s];
+      const int at = (i0 + s * RS) * LD + cc;
+      if constexpr (!STATE_ONLY) *(f32x4*)(sa + at) = ra[s];
+      *(f32x4*)(sk + at) = rk[s];
+      *(f32x4*)(sv + at) = rv[s];
     }
   };
-  fetch(p0);
-  put();
+  if (p0 < p1) {
+    fetch(p0);
+    put();
+  }
   for (int c0 = p0; c0 < p1; c0 += DA_C) {
     const int n = min(DA_C, p1 - c0);                       // tokens in this chunk
     const int shift = w.shift && c0 == 0 ? 1 : 0;
     __syncthreads();
-    if (c0 + DA_C < p1) fetch(c0 + DA_C);
+    fetch(c0 + DA_C);                                       // behind the last chunk: zeros, without an access
     f32x4 O[2][NT];
     if (!STATE_ONLY) {
-      // ---- weights lam^{i-j} (a_i . k_j), one 16 x 16 tile per wave; the tile above the diagonal is never read
+      // ---- weights lam^{i-j} (a_i . k_j), transposed: a lane holds four neighbouring j of one i.  One 16 x 16 tile per wave and
+      // turn; the tile above the diagonal is never read
 #pragma unroll
       for (int u = 0; u < 4 / NW; ++u) {
         const int mt = (u * NW + wave) >> 1, jt = (u * NW + wave) & 1;
@@ -152,16 +172,20 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
           const f32x4 x = *(const f32x4*)(sa + (mt * 16 + l16) * LD + kt * 16 + 4 * q);
           const f32x4 y = *(const f32x4*)(sk + (jt * 16 + l16) * LD + kt * 16 + 4 * q);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], y[r], acc, 0, 0, 0);
+          for (int r = 0; r < 4; ++r) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(y[r], x[r], acc, 0, 0, 0);
         }
-        const float s = w.s_o * w.s_kv;
+        const int i = mt * 16 + l16, j = jt * 16 + 4 * q;
+        float f[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = mt * 16 + 4 * q + r, j = jt * 16 + l16;
-          sp[i * LDP + j] = i >= j ? acc[r] * (s * pw[max(i - j, 0)]) : 0.f;
-        }
+        for (int r = 0; r < 4; ++r) f[r] = pp[15 + i - j - r];
+        // all four are read, whether they count or not: a branch around each would wait for each
+        asm("" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]));
+        const int last = mt == jt ? l16 - 4 * q : 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[r] = r <= last ? acc[r] * f[r] : 0.f;
+        *(f32x4*)(sp + i * LDP + j) = acc;
       }
-      // ---- what the state contributes
+      // ---- what the state contributes, transposed: rows are the wave's columns, columns the tokens
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
@@ -172,71 +196,73 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) O[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], X[kt][nt][r], O[mt][nt], 0, 0, 0);
+            for (int r = 0; r < 4; ++r) O[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(X[kt][nt][r], x[r], O[mt][nt], 0, 0, 0);
         }
+        const float f = w.s_o * pw[mt * 16 + l16 + 1 - shift];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float f = w.s_o * pw[mt * 16 + 4 * q + r + 1 - shift];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) O[mt][nt][r] *= f;
-        }
+        for (int nt = 0; nt < NT; ++nt) O[mt][nt] *= f;
       }
-      __syncthreads();
     }
-    // ---- this chunk's values: O += P V and X = lam^n X + K^T V'
+    // ---- X = lam^n X + K^T V'
     const float f = pw[n - shift];
+    f32x4 V[2][NT];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) X[kt][nt][r] *= f;
+      for (int nt = 0; nt < NT; ++nt) X[kt][nt] *= f;
 #pragma unroll
     for (int jt = 0; jt < 2; ++jt) {
-      f32x4 V[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) V[nt][r] = sv[(jt * 16 + 4 * q + r) * LD + (wave * NT + nt) * 16 + l16];
-      if (!STATE_ONLY) {
+        for (int r = 0; r < 4; ++r) V[jt][nt][r] = sv[(jt * 16 + 4 * q + r) * LD + (wave * NT + nt) * 16 + l16];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float g = pv[DA_C - n + jt * 16 + 4 * q + r];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) {
+          const float x = sk[(jt * 16 + 4 * q + r) * LD + kt * 16 + l16];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) X[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, V[jt][nt][r] * g, X[kt][nt], 0, 0, 0);
+        }
+      }
+    }
+    // every wave is done with the tiles and has left its weights: the next chunk's tiles may be written from here on, its
+    // weights only behind the next barrier, i.e. when all have read these
+    __syncthreads();
+    if (!STATE_ONLY) {
+      // ---- O += P V
+#pragma unroll
+      for (int jt = 0; jt < 2; ++jt)
 #pragma unroll
         for (int mt = jt; mt < 2; ++mt) {
           const f32x4 x = *(const f32x4*)(sp + (mt * 16 + l16) * LDP + jt * 16 + 4 * q);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) O[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], V[nt][r], O[mt][nt], 0, 0, 0);
+            for (int r = 0; r < 4; ++r) O[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(V[jt][nt][r], x[r], O[mt][nt], 0, 0, 0);
         }
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float f = w.s_kv * pw[max(n - 1 - (jt * 16 + 4 * q + r), 0)];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) V[nt][r] *= f;
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt) {
-          const float x = sk[(jt * 16 + 4 * q + r) * LD + kt * 16 + l16];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) X[kt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(x, V[nt][r], X[kt][nt], 0, 0, 0);
-        }
-      }
     }
-    __syncthreads();                                        // every wave is done with the tiles
-    if (c0 + DA_C < p1) put();                              // before this chunk's stores, which nobody waits for then
+    // the next tiles go in before this chunk's rows go out: waiting for loads that are older than a store is not waiting for the
+    // store (memory operations are counted in order)
+    put();
     if (!STATE_ONLY) {
+      const auto rs = chunk_rows(ob + (w.reverse ? len - c0 - n : c0) * w.so.t, n, w.so.t, w.dv, 4);
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int mt = 0; mt < 2; ++mt) {
+        const int i = mt * 16 + l16, off = (w.reverse ? n - 1 - i : i) * 4 * (int)w.so.t;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int i = mt * 16 + 4 * q + r;
-          if (i >= n) continue;
-          const long t = w.reverse ? len - 1 - (c0 + i) : c0 + i;
+        for (int nt = 0; nt < NT; ++nt) {
+          const int col = (wave * NT + nt) * 16 + 4 * q;
+          if (VEC) {
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, O[mt][nt]), rs, chunk_offset(off + 4 * col, i < n && col < w.dv), 0, 0);
+          } else {
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const int col = (wave * NT + nt) * 16 + l16;
-            if (col < w.dv) ob[t * w.so.t + col] = O[mt][nt][r];
+            for (int e = 0; e < 4; ++e)
+              __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(O[mt][nt][e]), rs, chunk_offset(off + 4 * (col + e), i < n && col + e < w.dv), 0, 0);
           }
         }
+      }
     }
   }
   // ---- state behind the segment
@@ -278,8 +304,6 @@ template <typename T>
 using x2 = __attribute__((ext_vector_type(2))) T;
 using u16x2 = __attribute__((ext_vector_type(2))) unsigned short;
 using s16x4 = __attribute__((ext_vector_type(4))) short;
-using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
-using u32x2 = __attribute__((ext_vector_type(2))) unsigned;
 
 template <typename T>
 __device__ __forceinline__ u32x4 row8(const T* base, bool live, int c, int width, bool vec) {
@@ -327,15 +351,7 @@ __device__ __forceinline__ float pow2(int e) { return ldexpf(1.f, e); }
 // The exponent that brings a bound below 2^top; a bound of zero, infinity or NaN gives a harmless one.
 __device__ __forceinline__ int scale_for(float bound, int top) { return max(min(top - __builtin_amdgcn_frexp_expf(bound), 60), -60); }
 
-// Rows of a chunk as a buffer: accesses behind its end read zero and store nothing, so that neither the clip's last chunk nor
-// columns behind the head need a branch.  `rows` of them, `stride` elements apart, `width` elements each.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_rows(const void* first, int rows, long stride, int width) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)first, 0, rows > 0 ? (int)(((rows - 1) * stride + width) * 2) : 0, 0x00020000);
-}
-// A byte offset into such a buffer; one before its start, or of a column that does not exist, lands far behind its end.
-__device__ __forceinline__ int chunk_offset(int off, bool exists) { return (int)min((unsigned)(exists ? off : -1), 0x80000000u); }
-
-// VEC: every row of a, k, v and o starts on a 16-byte boundary, rows do not overlap and a chunk spans less than 2 GB.
+// VEC: rows of a, k, v and o allow 16-byte accesses.
 template <typename T, int P, int CC, bool STATE_ONLY, bool VEC>
 __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkArgs w) {
   constexpr bool F16 = __is_same(T, f16_t);
@@ -420,7 +436,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkAr
   auto rows8 = [&](const T* base, const Strides& st, int width, bool vec, int c0, u32x4 (&out)[SLOTS]) {
     const int n = min(C, p1 - c0);                       // none or fewer behind the last chunk
     if (VEC) {
-      const auto rs = chunk_rows(base + (w.reverse ? len - c0 - n : c0) * st.t, n, st.t, width);
+      const auto rs = chunk_rows(base + (w.reverse ? len - c0 - n : c0) * st.t, n, st.t, width, 2);
       const int step = dir * RS * 2 * (int)st.t;
       int off = (w.reverse ? n - 1 - i0 : i0) * 2 * (int)st.t + 2 * cc;
 #pragma unroll
@@ -603,7 +619,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkAr
     if constexpr (P < 128) put();
     if (!STATE_ONLY) {
       const int col = col0 + 4 * q;
-      const auto rs = chunk_rows(ob + (w.reverse ? len - c0 - n : c0) * w.so.t, n, w.so.t, w.dv);
+      const auto rs = chunk_rows(ob + (w.reverse ? len - c0 - n : c0) * w.so.t, n, w.so.t, w.dv, 2);
 #pragma unroll
       for (int it = 0; it < NI; ++it) {
         const int i = it * 16 + l16;
@@ -721,14 +737,12 @@ __global__ __launch_bounds__(256) void step_kernel(const T* __restrict__ q, Stri
   }
 }
 
-// Whether `v` neighbouring elements of a row may be accessed as one.
-bool rows_vec(const void* p, const Strides& s, int v, int esize) {
-  return ((uintptr_t)p % (v * esize)) == 0 && s.b % v == 0 && s.t % v == 0 && s.h % v == 0;
+// Whether pieces of `v` elements of a row may be accessed as one: 16 bytes, and a row is a whole number of them.
+bool rows_vec(const void* p, const Strides& s, int width, int v, int esize) {
+  return ((uintptr_t)p % (v * esize)) == 0 && s.b % v == 0 && s.t % v == 0 && s.h % v == 0 && width % v == 0;
 }
-// ... and as a piece of a chunk's buffer (16-bit kernels): whole pieces, rows apart, offsets below 2^31 bytes.
-bool rows_buffer(const void* p, const Strides& s, int width) {
-  return rows_vec(p, s, 8, 2) && width % 8 == 0 && s.t >= width && s.t < (1L << 23);
-}
+// Whether a chunk's rows make a buffer: rows apart, and offsets below 2^31 bytes.
+bool rows_apart(const Strides& s, int width) { return s.t >= width && s.t < (1L << 22); }
 
 void scan_launch(const WalkArgs& w, hipStream_t st) {
   hipLaunchKernelGGL(walk_scan_kernel, dim3(noise_cdiv((long)w.dk * w.dv, 256), w.B * w.H), dim3(256), 0, st, w);
@@ -737,7 +751,12 @@ void scan_launch(const WalkArgs& w, hipStream_t st) {
 void walk_launch_f32(const WalkArgs& w, hipStream_t st) {
   const int d = w.dk > w.dv ? w.dk : w.dv;
   const unsigned grid = (unsigned)w.B * w.H * w.nseg;
-#define GO(P, ONLY) hipLaunchKernelGGL((walk_f32_kernel<P, ONLY>), dim3(grid), dim3(P >= 64 ? 256 : P * 4), 0, st, w)
+  const bool vec = w.va && w.vk && w.vv && w.vo;
+#define GO(P, ONLY)                                                                                                         \
+  do {                                                                                                                      \
+    if (vec) hipLaunchKernelGGL((walk_f32_kernel<P, ONLY, true>), dim3(grid), dim3(P >= 64 ? 256 : P * 4), 0, st, w);       \
+    else hipLaunchKernelGGL((walk_f32_kernel<P, ONLY, false>), dim3(grid), dim3(P >= 64 ? 256 : P * 4), 0, st, w);          \
+  } while (0)
 #define PICK(ONLY)             \
   do {                         \
     if (d <= 16) GO(16, ONLY); \
@@ -759,6 +778,9 @@ void walk_launch_16(const WalkArgs& w, hipStream_t st) {
   const int d = w.dk > w.dv ? w.dk : w.dv;
   const unsigned grid = (unsigned)w.B * w.H * w.nseg;
   const bool vec = w.va && w.vk && w.vv && w.vo;
+  // tokens per chunk: 32 where 64 would spill registers (heads of 128: 273 -> 251 us for 32 clips of 2048 tokens, 16 heads) or
+  // cost a workgroup per CU (heads of 64 in bf16: 139 -> 126 us for 64 clips of 2048 tokens, 8 heads; in fp16 150 -> 163)
+  constexpr int C64 = __is_same(T, bf16_t) ? 32 : 64;
 #define GO(P, C, ONLY)                                                                                      \
   do {                                                                                                      \
     if (vec) hipLaunchKernelGGL((walk_16_kernel<T, P, C, ONLY, true>), dim3(grid), dim3(P * 4), 0, st, w);  \
@@ -767,7 +789,7 @@ void walk_launch_16(const WalkArgs& w, hipStream_t st) {
 #define PICK(ONLY)             \
   do {                         \
     if (d <= 32) GO(32, 64, ONLY); \
-    else if (d <= 64) GO(64, 64, ONLY); \
+    else if (d <= 64) GO(64, C64, ONLY); \
     else GO(128, 32, ONLY);    \
   } while (0)
   if (w.nseg > 1 && !w.seg_tr) {
@@ -836,11 +858,10 @@ NOISE_EXPORT int noise_decay_attn_walk(const void* a, const void* k, const void*
   w.seg_len = (noise_cdiv(T, w.nseg) + DB_C - 1) / DB_C * DB_C;
   w.nseg = noise_cdiv(T, w.seg_len);
   NOISE_REQUIRE(w.nseg == 1 || workspace, "noise_decay_attn_walk: this shape needs a workspace");
-  if (dtype == NOISE_F32) {
-    w.va = rows_vec(a, w.sa, 4, 4), w.vk = rows_vec(k, w.sk, 4, 4), w.vv = rows_vec(v, w.sv, 4, 4), w.vo = 0;
-  } else {
-    w.va = rows_buffer(a, w.sa, dk), w.vk = rows_buffer(k, w.sk, dk), w.vv = rows_buffer(v, w.sv, dv), w.vo = rows_buffer(o, w.so, dv);
-  }
+  NOISE_REQUIRE(rows_apart(w.sa, dk) && rows_apart(w.sk, dk) && rows_apart(w.sv, dv) && rows_apart(w.so, dv),
+                "noise_decay_attn_walk: a token stride is below the row's width or not below 2^22 elements");
+  const int piece = dtype == NOISE_F32 ? 4 : 8, es = dtype == NOISE_F32 ? 4 : 2;
+  w.va = rows_vec(a, w.sa, dk, piece, es), w.vk = rows_vec(k, w.sk, dk, piece, es), w.vv = rows_vec(w.v, w.sv, dv, piece, es), w.vo = rows_vec(o, w.so, dv, piece, es);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == NOISE_F32) walk_launch_f32(w, st);
   else if (dtype == NOISE_BF16) walk_launch_16<bf16_t>(w, st);

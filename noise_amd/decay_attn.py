@@ -39,6 +39,19 @@ def _unit(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _tokens(t):
+    """(t, its strides) as the walk reads them: unit stride in a row, rows apart and within reach; a packed copy otherwise (a
+    broadcast token axis, overlapping windows).  The stride of an axis of one token says nothing."""
+    t = _unit(t)
+    b, s, h, _ = t.stride()
+    if t.shape[1] == 1:
+        s = t.shape[-1]
+    if not t.shape[-1] <= s < 1 << 22:
+        t = t.contiguous()
+        b, s, h, _ = t.stride()
+    return t, (b, s, h)
+
+
 def _check(q, k, v, log_decay, state, tokens):
     _lib.require_cuda(q, k, v, log_decay, state)
     qs, vs, dims = q.shape, v.shape, 4 if tokens else 3
@@ -75,11 +88,11 @@ def _walk(a, k, v, log_decay, lengths, x0, x0_transposed, x_end, s_o, s_kv, reve
     k and v swapped returned."""
     B, T, H, dk = a.shape
     dv = v.shape[-1]
-    a, k, v = _unit(a), _unit(k), _unit(v)
+    (a, sa), (k, sk), (v, sv) = _tokens(a), _tokens(k), _tokens(v)
     o = a.new_empty(B, T, H, dv)
     n = _lib.lib.noise_decay_attn_workspace(B, T, H, dk, dv, _lib.DTYPES[a.dtype])
     ws = swapped if swapped is not None else a.new_empty(n, dtype=torch.float32) if n else None
-    strides = (_L * 12)(*a.stride()[:3], *k.stride()[:3], *v.stride()[:3], T * H * dv, H * dv, dv)
+    strides = (_L * 12)(*sa, *sk, *sv, T * H * dv, H * dv, dv)
     _lib.call("noise_decay_attn_walk", ptr(a), ptr(k), ptr(v), ptr(o), strides, ptr(log_decay), ptr(lengths), ptr(x0),
               int(x0_transposed), ptr(x_end), ptr(ws), s_o, s_kv, int(reverse), int(swapped is not None), B, T, H, dk, dv, _lib.DTYPES[a.dtype], _lib.stream(),
               nbytes=a.element_size() * 2 * (a.numel() + v.numel()))
