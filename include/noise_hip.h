@@ -392,18 +392,21 @@ int noise_layer_norm_bwd(const void* dy, long lddy, const void* x, long ldx, con
                          void* stream);
 
 /* ---- decay attention: causal linear attention with one decay per head ---------------------------- */
-/* X_p = e^g X_{p-1} + s_kv k_p (x) v_p, o_p = s_o a_p X_p over p < length; a, k [B][T][H][dk], v, o [B][T][H][dv] by strides
- * (elements between clips, tokens, heads of a, k, v, o: 12 values on the HOST; unit stride on the last axis, a token stride
- * of at least the row's width and below 2^22); rows of o at
- * and behind the length are zero.  log_decay g [H] <= 0; lengths [B] or NULL (all T); x0, x_end [B][H][dk][dv] fp32 or NULL
- * (x0_transposed: x0 is [B][H][dv][dk]).  reverse != 0: last token first, x0 meets the last token undecayed and x_end gets
- * one more decay (the gradient of the state before the first token).  1 <= dk, dv <= 128.
- * workspace: noise_decay_attn_workspace() floats (0: may be NULL); reuse != 0: it is as a walk with k and v swapped, x0
- * transposed and all else equal has just left it */
-long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv, int dtype);
-int noise_decay_attn_walk(const void* a, const void* k, const void* v, void* o, const long* strides, const float* log_decay,
-                          const int* lengths, const float* x0, int x0_transposed, float* x_end, float* workspace, float s_o,
-                          float s_kv, int reverse, int reuse, int B, int T, int H, int dk, int dv, int dtype, void* stream);
+/* S_t = e^g S_{t-1} + k_t (x) v_t, o_t = scale q_t S_t over t < length; q, k [B][T][H][dk], v, o [B][T][H][dv] by strides
+ * (elements between clips, tokens and heads of q, k, v, o: 12 values on the HOST; unit stride on the last axis, a token stride
+ * of at least the row's width and below 2^22); rows of o at and behind the length are zero.  log_decay g [H] <= 0; lengths [B]
+ * or NULL (all T); state (before the first token), end (behind the last) [B][H][dk][dv] fp32 or NULL (zero; not wanted).
+ * 1 <= dk, dv <= 128.  workspace: noise_decay_attn_workspace() floats (0: may be NULL) */
+long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv, int dtype, int backward);
+int noise_decay_attn_fwd(const void* q, const void* k, const void* v, void* o, const long* strides, const float* log_decay,
+                         const int* lengths, const float* state, float* end, float* workspace, float scale, int B, int T, int H,
+                         int dk, int dv, int dtype, void* stream);
+/* go, d_end: gradients of o and end (d_end NULL: zero); gq, gk, gv, d_state (or NULL): those of q, k, v and state; strides of
+ * go, q, k, v, gq, gk, gv (21 values on the HOST).  Rows at and behind the length are neither read nor anything but zero */
+int noise_decay_attn_bwd(const void* go, const void* q, const void* k, const void* v, void* gq, void* gk, void* gv,
+                         const long* strides, const float* log_decay, const int* lengths, const float* state, const float* d_end,
+                         float* d_state, float* workspace, float scale, int B, int T, int H, int dk, int dv, int dtype,
+                         void* stream);
 /* one token per clip: state [B][H][dk][dv] updated in place, o [B][H][dv]; strides: (clip, head) of q, k, v on the HOST */
 int noise_decay_attn_step(const void* q, const void* k, const void* v, const long* strides, const float* log_decay, float* state,
                           void* o, float scale, int B, int H, int dk, int dv, int dtype, void* stream);

@@ -18,6 +18,7 @@
 // sums each segment's own contribution to the state, a scan turns them into the state before each segment, and the walk
 // starts from those.
 #include "token.h"
+#include <type_traits>
 
 namespace {
 
@@ -43,6 +44,11 @@ struct WalkArgs {
   int va, vk, vv, vo;       // rows allow 16-byte accesses
 };
 
+// Walks of one shape that run side by side (blockIdx.y): one forward, three of the backward pass.
+struct WalkSet {
+  WalkArgs w[3];
+};
+
 __device__ __forceinline__ float decay_pow(float g2, int n) { return n <= 0 ? 1.f : exp2f(g2 * (float)n); }
 
 using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
@@ -64,7 +70,8 @@ __device__ __forceinline__ int chunk_offset(int off, bool exists) { return (int)
 // the C x C weights pass through LDS (each wave computes a share of them).
 // VEC: rows of a, k, v and o allow 16-byte accesses; otherwise elements go one by one, through the same buffers.
 template <int P, bool STATE_ONLY, bool VEC>
-__global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_f32_kernel(WalkArgs w) {
+__global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_f32_kernel(WalkSet set) {
+  const WalkArgs& w = set.w[blockIdx.y];
   constexpr int NW = P >= 64 ? 4 : P / 16, NT = P / 16 / NW, KT = P / 16, NTHR = NW * 64;
   constexpr int LD = P + 4, LDP = DA_C + 4, SLOTS = DA_C * P / 4 / NTHR, RS = NTHR / (P / 4);
   __shared__ __attribute__((aligned(16))) float sa[STATE_ONLY ? 4 : DA_C * LD];
@@ -353,7 +360,8 @@ __device__ __forceinline__ int scale_for(float bound, int top) { return max(min(
 
 // VEC: rows of a, k, v and o allow 16-byte accesses.
 template <typename T, int P, int CC, bool STATE_ONLY, bool VEC>
-__global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkArgs w) {
+__global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSet set) {
+  const WalkArgs& w = set.w[blockIdx.y];
   constexpr bool F16 = __is_same(T, f16_t);
   constexpr int C = CC, NI = C / 16, TILES = NI * (NI + 1) / 2;
   constexpr int NTHR = P * 4, NW = P / 16, KP = P / 32;      // KP: pairs of state row tiles
@@ -656,7 +664,8 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkAr
 
 // Sums of the segments -> states before the segments, in place: seg[s] = lam^{seg_len} seg[s-1] + sum[s-1], seg[0] = x0.  The
 // shifted first decay of a reversed walk is that of segment 0.
-__global__ __launch_bounds__(256) void walk_scan_kernel(WalkArgs w) {
+__global__ __launch_bounds__(256) void walk_scan_kernel(WalkSet set) {
+  const WalkArgs& w = set.w[blockIdx.z];
   const int mat = w.dk * w.dv;
   const int e = blockIdx.x * 256 + threadIdx.x;
   const int bh = blockIdx.y;
@@ -744,61 +753,69 @@ bool rows_vec(const void* p, const Strides& s, int width, int v, int esize) {
 // Whether a chunk's rows make a buffer: rows apart, and offsets below 2^31 bytes.
 bool rows_apart(const Strides& s, int width) { return s.t >= width && s.t < (1L << 22); }
 
-void scan_launch(const WalkArgs& w, hipStream_t st) {
-  hipLaunchKernelGGL(walk_scan_kernel, dim3(noise_cdiv((long)w.dk * w.dv, 256), w.B * w.H), dim3(256), 0, st, w);
+// The passes of `n` walks of one shape: segment sums and scan for the first `sums` of them (the others reuse those), then the
+// walks themselves.  vec: all rows of all walks allow 16-byte accesses.
+template <typename Launch>
+void walk_passes(const WalkSet& set, int n, int sums, hipStream_t st, Launch launch) {
+  const WalkArgs& w = set.w[0];
+  const dim3 grid((unsigned)w.B * w.H * w.nseg);
+  if (w.nseg > 1) {
+    launch(dim3(grid.x, sums), std::true_type());
+    hipLaunchKernelGGL(walk_scan_kernel, dim3(noise_cdiv((long)w.dk * w.dv, 256), w.B * w.H, sums), dim3(256), 0, st, set);
+  }
+  launch(dim3(grid.x, n), std::false_type());
 }
 
-void walk_launch_f32(const WalkArgs& w, hipStream_t st) {
-  const int d = w.dk > w.dv ? w.dk : w.dv;
-  const unsigned grid = (unsigned)w.B * w.H * w.nseg;
-  const bool vec = w.va && w.vk && w.vv && w.vo;
-#define GO(P, ONLY)                                                                                                         \
-  do {                                                                                                                      \
-    if (vec) hipLaunchKernelGGL((walk_f32_kernel<P, ONLY, true>), dim3(grid), dim3(P >= 64 ? 256 : P * 4), 0, st, w);       \
-    else hipLaunchKernelGGL((walk_f32_kernel<P, ONLY, false>), dim3(grid), dim3(P >= 64 ? 256 : P * 4), 0, st, w);          \
+bool walk_vec(const WalkSet& set, int n) {
+  bool vec = true;
+  for (int i = 0; i < n; ++i) vec = vec && set.w[i].va && set.w[i].vk && set.w[i].vv && set.w[i].vo;
+  return vec;
+}
+
+void walk_launch_f32(const WalkSet& set, int n, int sums, hipStream_t st) {
+  const int d = set.w[0].dk > set.w[0].dv ? set.w[0].dk : set.w[0].dv;
+  const bool vec = walk_vec(set, n);
+  walk_passes(set, n, sums, st, [&](dim3 grid, auto only) {
+    constexpr bool ONLY = decltype(only)::value;
+#define GO(P)                                                                                                         \
+  do {                                                                                                                \
+    if (vec) hipLaunchKernelGGL((walk_f32_kernel<P, ONLY, true>), grid, dim3(P >= 64 ? 256 : P * 4), 0, st, set);     \
+    else hipLaunchKernelGGL((walk_f32_kernel<P, ONLY, false>), grid, dim3(P >= 64 ? 256 : P * 4), 0, st, set);        \
   } while (0)
-#define PICK(ONLY)             \
-  do {                         \
-    if (d <= 16) GO(16, ONLY); \
-    else if (d <= 32) GO(32, ONLY); \
-    else if (d <= 64) GO(64, ONLY); \
-    else GO(128, ONLY);        \
-  } while (0)
-  if (w.nseg > 1 && !w.seg_tr) {
-    PICK(true);
-    scan_launch(w, st);
-  }
-  PICK(false);
-#undef PICK
+    if (d <= 16) GO(16);
+    else if (d <= 32) GO(32);
+    else if (d <= 64) GO(64);
+    else GO(128);
 #undef GO
+  });
 }
 
 template <typename T>
-void walk_launch_16(const WalkArgs& w, hipStream_t st) {
-  const int d = w.dk > w.dv ? w.dk : w.dv;
-  const unsigned grid = (unsigned)w.B * w.H * w.nseg;
-  const bool vec = w.va && w.vk && w.vv && w.vo;
+void walk_launch_16(const WalkSet& set, int n, int sums, hipStream_t st) {
+  const int d = set.w[0].dk > set.w[0].dv ? set.w[0].dk : set.w[0].dv;
+  const bool vec = walk_vec(set, n);
   // tokens per chunk: 32 where 64 would spill registers (heads of 128: 273 -> 251 us for 32 clips of 2048 tokens, 16 heads) or
   // cost a workgroup per CU (heads of 64 in bf16: 139 -> 126 us for 64 clips of 2048 tokens, 8 heads; in fp16 150 -> 163)
   constexpr int C64 = __is_same(T, bf16_t) ? 32 : 64;
-#define GO(P, C, ONLY)                                                                                      \
-  do {                                                                                                      \
-    if (vec) hipLaunchKernelGGL((walk_16_kernel<T, P, C, ONLY, true>), dim3(grid), dim3(P * 4), 0, st, w);  \
-    else hipLaunchKernelGGL((walk_16_kernel<T, P, C, ONLY, false>), dim3(grid), dim3(P * 4), 0, st, w);     \
+  walk_passes(set, n, sums, st, [&](dim3 grid, auto only) {
+    constexpr bool ONLY = decltype(only)::value;
+#define GO(P, C)                                                                                       \
+  do {                                                                                                 \
+    if (vec) hipLaunchKernelGGL((walk_16_kernel<T, P, C, ONLY, true>), grid, dim3(P * 4), 0, st, set); \
+    else hipLaunchKernelGGL((walk_16_kernel<T, P, C, ONLY, false>), grid, dim3(P * 4), 0, st, set);    \
   } while (0)
-#define PICK(ONLY)             \
-  do {                         \
-    if (d <= 32) GO(32, 64, ONLY); \
-    else if (d <= 64) GO(64, C64, ONLY); \
-    else GO(128, 32, ONLY);    \
-  } while (0)
-  if (w.nseg > 1 && !w.seg_tr) {
-    PICK(true);
-    scan_launch(w, st);
-  }
-  PICK(false);
-#undef PICK
+    if (d <= 32) GO(32, 64);
+    else if (d <= 64) GO(64, C64);
+    else GO(128, 32);
 #undef GO
+  });
+}
+
+int walk_launch(const WalkSet& set, int n, int sums, int dtype, hipStream_t st) {
+  if (dtype == NOISE_F32) walk_launch_f32(set, n, sums, st);
+  else if (dtype == NOISE_BF16) walk_launch_16<bf16_t>(set, n, sums, st);
+  else walk_launch_16<f16_t>(set, n, sums, st);
+  return 0;
 }
 
 // Segments of the token axis.  From `full` (clip, head) pairs on, clips and heads fill the GPU well enough that the second
@@ -828,45 +845,81 @@ const char* walk_check(int B, int T, int H, int dk, int dv, int dtype) {
 
 }  // namespace
 
-// Floats of workspace a walk of this shape needs.
-NOISE_EXPORT long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv, int dtype) {
-  if (walk_check(B, T, H, dk, dv, dtype)) return 0;
-  const int n = walk_segments((long)B * H, T, dk > dv ? dk : dv, dtype != NOISE_F32);
-  return n > 1 ? (long)B * H * n * dk * dv : 0;
+// Fills in what a walk derives from its shape; an error text, or null.
+static const char* walk_plan(WalkArgs& w, int nseg, int dtype) {
+  w.seg_len = (noise_cdiv(w.T, nseg) + DB_C - 1) / DB_C * DB_C;
+  w.nseg = noise_cdiv(w.T, w.seg_len);
+  if (w.nseg > 1 && !w.seg) return "this shape needs a workspace";
+  if (!(rows_apart(w.sa, w.dk) && rows_apart(w.sk, w.dk) && rows_apart(w.sv, w.dv) && rows_apart(w.so, w.dv)))
+    return "a token stride is below the row's width or not below 2^22 elements";
+  const int piece = dtype == NOISE_F32 ? 4 : 8, es = dtype == NOISE_F32 ? 4 : 2;
+  w.va = rows_vec(w.a, w.sa, w.dk, piece, es), w.vk = rows_vec(w.k, w.sk, w.dk, piece, es);
+  w.vv = rows_vec(w.v, w.sv, w.dv, piece, es), w.vo = rows_vec(w.o, w.so, w.dv, piece, es);
+  return nullptr;
 }
 
-// strides: (clip, token, head) of a, k, v and o; reverse: last token first, with the undecayed first step and the decayed end;
-// reuse: the workspace is as the walk with k and v (and x0 with its transpose) swapped left it
-NOISE_EXPORT int noise_decay_attn_walk(const void* a, const void* k, const void* v, void* o, const long* strides,
-                                       const float* log_decay, const int* lengths, const float* x0, int x0_transposed,
-                                       float* x_end, float* workspace, float s_o, float s_kv, int reverse, int reuse, int B, int T, int H,
-                                       int dk, int dv, int dtype, void* stream) {
+static int walk_nseg(int B, int T, int H, int dk, int dv, int dtype, int backward) {
+  return walk_segments((long)B * H * (backward ? 3 : 1), T, dk > dv ? dk : dv, dtype != NOISE_F32);
+}
+
+// Floats of workspace a forward (backward) pass of this shape needs.
+NOISE_EXPORT long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv, int dtype, int backward) {
+  if (walk_check(B, T, H, dk, dv, dtype)) return 0;
+  const int n = walk_nseg(B, T, H, dk, dv, dtype, backward);
+  return n > 1 ? (long)B * H * n * dk * dv * (backward ? 2 : 1) : 0;
+}
+
+// strides: (clip, token, head) of q, k, v and o
+NOISE_EXPORT int noise_decay_attn_fwd(const void* q, const void* k, const void* v, void* o, const long* strides,
+                                      const float* log_decay, const int* lengths, const float* state, float* end,
+                                      float* workspace, float scale, int B, int T, int H, int dk, int dv, int dtype, void* stream) {
   const char* why = walk_check(B, T, H, dk, dv, dtype);
-  NOISE_REQUIRE(!why, "noise_decay_attn_walk: %s (B %d, T %d, H %d, head sizes %d and %d)", why, B, T, H, dk, dv);
-  NOISE_REQUIRE(a && k && v && o && strides && log_decay, "noise_decay_attn_walk: null pointer");
-  WalkArgs w;
-  w.a = a, w.k = k, w.v = v, w.o = o;
-  w.sa = {strides[0], strides[1], strides[2]};
-  w.sk = {strides[3], strides[4], strides[5]};
-  w.sv = {strides[6], strides[7], strides[8]};
-  w.so = {strides[9], strides[10], strides[11]};
-  w.log_decay = log_decay, w.lengths = lengths, w.x0 = x0, w.x0_tr = x0_transposed, w.x_end = x_end, w.seg = workspace;
-  w.s_o = s_o, w.s_kv = s_kv;
+  NOISE_REQUIRE(!why, "noise_decay_attn_fwd: %s (B %d, T %d, H %d, head sizes %d and %d)", why, B, T, H, dk, dv);
+  NOISE_REQUIRE(q && k && v && o && strides && log_decay, "noise_decay_attn_fwd: null pointer");
+  const Strides* st = (const Strides*)strides;
+  WalkSet set = {};
+  WalkArgs& w = set.w[0];
+  w.a = q, w.k = k, w.v = v, w.o = o, w.sa = st[0], w.sk = st[1], w.sv = st[2], w.so = st[3];
+  w.log_decay = log_decay, w.lengths = lengths, w.x0 = state, w.x_end = end, w.seg = workspace, w.s_o = scale, w.s_kv = 1.f;
   w.B = B, w.T = T, w.H = H, w.dk = dk, w.dv = dv;
-  w.reverse = reverse, w.shift = reverse, w.end_decay = reverse, w.seg_tr = reuse;
-  w.nseg = walk_segments((long)B * H, T, dk > dv ? dk : dv, dtype != NOISE_F32);
-  w.seg_len = (noise_cdiv(T, w.nseg) + DB_C - 1) / DB_C * DB_C;
-  w.nseg = noise_cdiv(T, w.seg_len);
-  NOISE_REQUIRE(w.nseg == 1 || workspace, "noise_decay_attn_walk: this shape needs a workspace");
-  NOISE_REQUIRE(rows_apart(w.sa, dk) && rows_apart(w.sk, dk) && rows_apart(w.sv, dv) && rows_apart(w.so, dv),
-                "noise_decay_attn_walk: a token stride is below the row's width or not below 2^22 elements");
-  const int piece = dtype == NOISE_F32 ? 4 : 8, es = dtype == NOISE_F32 ? 4 : 2;
-  w.va = rows_vec(a, w.sa, dk, piece, es), w.vk = rows_vec(k, w.sk, dk, piece, es), w.vv = rows_vec(w.v, w.sv, dv, piece, es), w.vo = rows_vec(o, w.so, dv, piece, es);
-  hipStream_t st = (hipStream_t)stream;
-  if (dtype == NOISE_F32) walk_launch_f32(w, st);
-  else if (dtype == NOISE_BF16) walk_launch_16<bf16_t>(w, st);
-  else walk_launch_16<f16_t>(w, st);
-  NOISE_CHECK_LAUNCH("noise_decay_attn_walk");
+  why = walk_plan(w, walk_nseg(B, T, H, dk, dv, dtype, 0), dtype);
+  NOISE_REQUIRE(!why, "noise_decay_attn_fwd: %s", why);
+  walk_launch(set, 1, 1, dtype, (hipStream_t)stream);
+  NOISE_CHECK_LAUNCH("noise_decay_attn_fwd");
+  return 0;
+}
+
+// strides: (clip, token, head) of do, q, k, v, dq, dk, dv
+NOISE_EXPORT int noise_decay_attn_bwd(const void* go, const void* q, const void* k, const void* v, void* dq, void* gk, void* gv,
+                                      const long* strides, const float* log_decay, const int* lengths, const float* state,
+                                      const float* d_end, float* d_state, float* workspace, float scale, int B, int T, int H,
+                                      int dk, int dv, int dtype, void* stream) {
+  const char* why = walk_check(B, T, H, dk, dv, dtype);
+  NOISE_REQUIRE(!why, "noise_decay_attn_bwd: %s (B %d, T %d, H %d, head sizes %d and %d)", why, B, T, H, dk, dv);
+  NOISE_REQUIRE(go && q && k && v && dq && gk && gv && strides && log_decay, "noise_decay_attn_bwd: null pointer");
+  const Strides* st = (const Strides*)strides;
+  const int nseg = walk_nseg(B, T, H, dk, dv, dtype, 1);
+  float* ws2 = workspace ? workspace + (size_t)B * H * nseg * dk * dv : nullptr;
+  WalkSet set = {};
+  WalkArgs &x = set.w[0], &y = set.w[1], &z = set.w[2];
+  // dq: first token first, X = S^T
+  x.a = go, x.k = v, x.v = k, x.o = dq, x.sa = st[0], x.sk = st[3], x.sv = st[2], x.so = st[4];
+  x.x0 = state, x.x0_tr = 1, x.seg = workspace, x.s_o = scale, x.s_kv = 1.f, x.dk = dv, x.dv = dk;
+  // dv: last token first, X = dS
+  y.a = k, y.k = q, y.v = go, y.o = gv, y.sa = st[2], y.sk = st[1], y.sv = st[0], y.so = st[6];
+  y.x0 = d_end, y.x_end = d_state, y.seg = ws2, y.s_o = 1.f, y.s_kv = scale, y.dk = dk, y.dv = dv;
+  // dk: the same with X transposed; it starts from the segments' states of dv
+  z.a = v, z.k = go, z.v = q, z.o = gk, z.sa = st[3], z.sk = st[0], z.sv = st[1], z.so = st[5];
+  z.x0 = d_end, z.x0_tr = 1, z.seg = ws2, z.seg_tr = 1, z.s_o = 1.f, z.s_kv = scale, z.dk = dv, z.dv = dk;
+  for (int i = 0; i < 3; ++i) {
+    WalkArgs& w = set.w[i];
+    w.log_decay = log_decay, w.lengths = lengths, w.B = B, w.T = T, w.H = H;
+    w.reverse = w.shift = w.end_decay = i > 0;
+    why = walk_plan(w, nseg, dtype);
+    NOISE_REQUIRE(!why, "noise_decay_attn_bwd: %s", why);
+  }
+  walk_launch(set, 3, 2, dtype, (hipStream_t)stream);
+  NOISE_CHECK_LAUNCH("noise_decay_attn_bwd");
   return 0;
 }
 

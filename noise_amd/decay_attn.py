@@ -25,9 +25,10 @@ from . import _lib
 from ._lib import _F, _I, _L, _P, ptr
 
 _lib.register({
-    "noise_decay_attn_walk": [_P] * 8 + [_I, _P, _P, _F, _F] + [_I] * 8 + [_P],
+    "noise_decay_attn_fwd": [_P] * 10 + [_F] + [_I] * 6 + [_P],
+    "noise_decay_attn_bwd": [_P] * 14 + [_F] + [_I] * 6 + [_P],
     "noise_decay_attn_step": [_P] * 7 + [_F] + [_I] * 5 + [_P],
-    "noise_decay_attn_workspace": [_I] * 6,
+    "noise_decay_attn_workspace": [_I] * 7,
 })
 _lib.lib.noise_decay_attn_workspace.restype = _L
 
@@ -83,20 +84,10 @@ def _check_lengths(lengths, B):
     return lengths.to(torch.int32).contiguous()
 
 
-def _walk(a, k, v, log_decay, lengths, x0, x0_transposed, x_end, s_o, s_kv, reverse, swapped=None):
-    """One pass of the operator at the top of csrc/decay_attn.hip: (o, workspace).  `swapped`: the workspace that the pass with
-    k and v swapped returned."""
-    B, T, H, dk = a.shape
-    dv = v.shape[-1]
-    (a, sa), (k, sk), (v, sv) = _tokens(a), _tokens(k), _tokens(v)
-    o = a.new_empty(B, T, H, dv)
-    n = _lib.lib.noise_decay_attn_workspace(B, T, H, dk, dv, _lib.DTYPES[a.dtype])
-    ws = swapped if swapped is not None else a.new_empty(n, dtype=torch.float32) if n else None
-    strides = (_L * 12)(*sa, *sk, *sv, T * H * dv, H * dv, dv)
-    _lib.call("noise_decay_attn_walk", ptr(a), ptr(k), ptr(v), ptr(o), strides, ptr(log_decay), ptr(lengths), ptr(x0),
-              int(x0_transposed), ptr(x_end), ptr(ws), s_o, s_kv, int(reverse), int(swapped is not None), B, T, H, dk, dv, _lib.DTYPES[a.dtype], _lib.stream(),
-              nbytes=a.element_size() * 2 * (a.numel() + v.numel()))
-    return o, ws
+def _workspace(q, dv, backward):
+    B, T, H, dk = q.shape
+    n = _lib.lib.noise_decay_attn_workspace(B, T, H, dk, dv, _lib.DTYPES[q.dtype], backward)
+    return q.new_empty(n, dtype=torch.float32) if n else None
 
 
 def decay_attention_fwd(q, k, v, log_decay, state=None, lengths=None, scale=None):
@@ -110,7 +101,12 @@ def decay_attention_fwd(q, k, v, log_decay, state=None, lengths=None, scale=None
             return torch.empty(v.shape, device=v.device, dtype=v.dtype), end
         end = q.new_empty(B, H, dk, dv, dtype=torch.float32)
         x0 = state.contiguous() if state is not None else None
-        o, _ = _walk(q, k, v, log_decay.contiguous(), lengths, x0, False, end, scale, 1.0, False)
+        T, g, ws = q.shape[1], log_decay.contiguous(), _workspace(q, dv, 0)
+        (q, sq), (k, sk), (v, sv) = _tokens(q), _tokens(k), _tokens(v)
+        o = q.new_empty(B, T, H, dv)
+        strides = (_L * 12)(*sq, *sk, *sv, T * H * dv, H * dv, dv)
+        _lib.call("noise_decay_attn_fwd", ptr(q), ptr(k), ptr(v), ptr(o), strides, ptr(g), ptr(lengths), ptr(x0), ptr(end), ptr(ws),
+                  scale, B, T, H, dk, dv, _lib.DTYPES[q.dtype], _lib.stream(), nbytes=2 * q.element_size() * (q.numel() + v.numel()))
         return o, end
 
 
@@ -131,11 +127,15 @@ def decay_attention_bwd(do, q, k, v, log_decay, state=None, lengths=None, scale=
         g = log_decay.contiguous()
         x0 = state.contiguous() if state is not None else None
         x1 = d_state.contiguous() if d_state is not None else None
-        do = _unit(do)
-        dq, _ = _walk(do, v, k, g, lengths, x0, True, None, scale, 1.0, False)
-        dvv, ws = _walk(k, q, do, g, lengths, x1, False, d0, 1.0, scale, True)
-        dkk, _ = _walk(v, do, q, g, lengths, x1, True, None, 1.0, scale, True, swapped=ws)
-        return dq, dkk, dvv, d0
+        T, ws = q.shape[1], _workspace(q, dv, 1)
+        (do, so), (q, sq), (k, sk), (v, sv) = _tokens(do), _tokens(q), _tokens(k), _tokens(v)
+        gq, gk, gv = q.new_empty(B, T, H, dk), q.new_empty(B, T, H, dk), q.new_empty(B, T, H, dv)
+        narrow, wide = (T * H * dk, H * dk, dk), (T * H * dv, H * dv, dv)
+        strides = (_L * 21)(*so, *sq, *sk, *sv, *narrow, *narrow, *wide)
+        _lib.call("noise_decay_attn_bwd", ptr(do), ptr(q), ptr(k), ptr(v), ptr(gq), ptr(gk), ptr(gv), strides, ptr(g), ptr(lengths),
+                  ptr(x0), ptr(x1), ptr(d0), ptr(ws), scale, B, T, H, dk, dv, _lib.DTYPES[q.dtype], _lib.stream(),
+                  nbytes=q.element_size() * (4 * q.numel() + 3 * v.numel()))
+        return gq, gk, gv, d0
 
 
 class _DecayAttention(torch.autograd.Function):
