@@ -127,3 +127,14 @@ def on_device(*tensors):
         if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors of one call live on different devices: {tensors[0].device} and {t.device}")
     return _HERE_ALREADY if dev == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def written(*tensors):
+    """Tells autograd that a kernel wrote these tensors in place through raw pointers (their version counters move, so that a
+    graph that saved one of them refuses to go backwards over the new values)."""
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:      # tensors made in inference mode have no version
+        for t in tensors:
+            if not t.is_inference():
+                torch.autograd.graph.increment_version(t)

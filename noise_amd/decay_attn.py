@@ -16,6 +16,10 @@ packed projection are read in place; a last axis without unit stride is copied f
 (-inf: no memory), and takes no gradient.  States are (B, H, Dk, Dv) fp32.  `lengths` (B,) integers on the GPU: the tokens of
 clip b at and behind lengths[b] are neither read nor added to the state, their rows of o and of the gradients are zero, and the
 state returned is the one behind the last real token.  `scale` defaults to Dk ** -0.5.
+
+Numbers: states are carried in fp32 accuracy whatever the tokens' type; in 16-bit types the weights inside a chunk and the
+state as it meets q are rounded to the type once each, like the output.  A token that is not finite reaches, besides all later
+ones, the other tokens of its chunk of 32 or 64.
 """
 import ctypes
 
@@ -183,4 +187,5 @@ def decay_attention_step(q, k, v, log_decay, state, scale=None, out=None):
             strides = (_L * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
             _lib.call("noise_decay_attn_step", ptr(q), ptr(k), ptr(v), strides, ptr(log_decay.contiguous()), ptr(state), ptr(out),
                       scale, B, H, dk, dv, _lib.DTYPES[q.dtype], _lib.stream(), nbytes=8 * state.numel())
+    _lib.written(state, out)
     return out

@@ -172,8 +172,7 @@ class MultiTensorAdamW:
                 _lib.call("noise_adamw_multi", *(a.buffer_info()[0] for a in part), len(part[0]), _lib.DTYPES[pd], _lib.DTYPES[gd],
                           self.state_bits, ptr(self._coef), *bufs, self.lr, *self.betas, self.eps, self.weight_decay, grad_scale, st,
                           nbytes=sum(part[2]) * (state_bytes + 2 * pd.itemsize + gd.itemsize) if _lib.PROFILE is not None else 0)
-        # the kernel wrote through raw pointers: autograd's and the models' stale-weight checks go by the version counters
-        torch.autograd.graph.increment_version(params)
+        _lib.written(*params)      # the models' checks for stale weights go by the version counters, too
 
     def _check(self, live, params, grads, shapes, types, addresses):
         """The parameters' addresses, after the checks.  Whole-list comparisons first: a step of many small tensors is as fast

@@ -291,6 +291,37 @@ def test_refusals():
         na.decay_attention_step(*one, s, out=z(2, 3, 7))
 
 
+def test_a_step_over_a_saved_state_is_noticed():
+    """A state that a graph holds for its backward pass and a step then overwrites: the backward pass refuses."""
+    import noise_amd as na
+    c = make(1, 4, 2, 8, 8, torch.float32, 2)
+    q = c["q"].clone().requires_grad_(True)
+    state = c["state"].clone()
+    o, _ = na.decay_attention(q, c["k"], c["v"], c["log_decay"], state)
+    na.decay_attention_step(c["q"][:, 0], c["k"][:, 0], c["v"][:, 0], c["log_decay"], state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    with torch.inference_mode():       # states made in inference mode have no version and need none
+        s2 = torch.zeros(1, 2, 8, 8, device=DEV)
+        na.decay_attention_step(c["q"][:, 0], c["k"][:, 0], c["v"][:, 0], c["log_decay"], s2)
+
+
+def test_calls_on_two_streams_at_once():
+    """Two different calls in flight together: nothing is shared between them."""
+    import noise_amd as na
+    cs = [make(1, 3000, 2, 64, 64, torch.bfloat16, 3), make(1, 2500, 2, 64, 64, torch.bfloat16, 4)]
+    want = [run_all(c) for c in cs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in cs], [None, None]
+    for _ in range(3):
+        for i, (c, s) in enumerate(zip(cs, streams)):
+            with torch.cuda.stream(s):
+                got[i] = run_all(c)
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(w[n], g[n]) for n in w)
+
+
 def test_no_tokens():
     import noise_amd as na
     c = make(2, 5, 3, 8, 6, torch.float32, 1)

@@ -14,6 +14,11 @@ def test_cpu_tensors_are_refused():
         na.layer_norm_bwd(x, x, torch.zeros(2), torch.ones(2))
     with pytest.raises(RuntimeError, match="GPU"):
         na.MultiTensorAdamW([torch.nn.Parameter(x)])
+    t = torch.zeros(1, 3, 2, 8)
+    with pytest.raises(RuntimeError, match="GPU"):
+        na.decay_attention(t, t, t, torch.zeros(2))
+    with pytest.raises(RuntimeError, match="GPU"):
+        na.decay_attention_step(t[:, 0], t[:, 0], t[:, 0], torch.zeros(2), torch.zeros(1, 2, 8, 8))
 
 
 def test_optimizer_arguments():
@@ -49,6 +54,28 @@ def test_c_entry_points_refuse_bad_arguments():
     with pytest.raises(RuntimeError, match="bad argument"):
         _lib.call("noise_adamw_multi_begin", None, None, None, 1, 1e-3, 0.9, 0.99, None)
     import array
+    st = array.array("l", [64, 8, 8] * 7)
+    sp = ctypes.c_void_p(st.buffer_info()[0])
+    low = array.array("l", [64, 7, 8] * 7)
+    lp = ctypes.c_void_p(low.buffer_info()[0])
+
+    def fwd(q=one, strides=sp, B=1, T=8, H=1, dk=8, dv=8, dtype=0):
+        _lib.call("noise_decay_attn_fwd", q, one, one, one, strides, one, None, None, None, None, 1.0, B, T, H, dk, dv, dtype, None)
+
+    def bwd(go=one, strides=sp, B=1, T=8, H=1, dk=8, dv=8, dtype=0):
+        _lib.call("noise_decay_attn_bwd", go, one, one, one, one, one, one, strides, one, None, None, None, None, None, 1.0, B, T, H, dk, dv,
+                  dtype, None)
+    for f, first in ((fwd, "q"), (bwd, "go")):
+        for kw, text in ((dict(B=0), "empty"), (dict(T=0), "empty"), (dict(H=0), "empty"), (dict(dk=0), "head sizes"), (dict(dk=129), "head sizes"),
+                         (dict(dv=129), "head sizes"), (dict(dtype=3), "element type"), (dict(B=1 << 22, H=2), "pairs"), (dict(strides=lp), "token stride"),
+                         (dict(strides=None), "null"), ({first: None}, "null"), (dict(T=100000), "workspace")):
+            with pytest.raises(RuntimeError, match=text):
+                f(**kw)
+    for args, text in (((None, 1, 1, 8, 8, 0), "null"), ((one, 0, 1, 8, 8, 0), "head sizes"), ((one, 1, 1, 129, 8, 0), "head sizes"), ((one, 1, 1, 8, 8, 7), "element type")):
+        with pytest.raises(RuntimeError, match=text):
+            _lib.call("noise_decay_attn_step", args[0], one, one, sp, one, one, one, 1.0, *args[1:], None)
+    assert _lib.lib.noise_decay_attn_workspace(1, 8, 1, 8, 8, 0, 0) == 0 and _lib.lib.noise_decay_attn_workspace(1, 100000, 1, 8, 8, 0, 1) > 0
+    assert _lib.lib.noise_decay_attn_workspace(1, 8, 1, 200, 8, 0, 0) == 0
     q, l, i = array.array("Q", [64]), array.array("l", [4]), array.array("i", [0])
     a = lambda x: ctypes.c_void_p(x.buffer_info()[0])
     off = array.array("l", [0])
