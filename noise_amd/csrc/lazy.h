@@ -9,8 +9,8 @@ enum { ACT_NONE = 0, ACT_RELU6 = 1 };
 __device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 __device__ __forceinline__ void st4(float* p, float4 v) { *reinterpret_cast<float4*>(p) = v; }
 __device__ __forceinline__ float4 f4(float v) { return make_float4(v, v, v, v); }
-// Packed fp32 arithmetic: two lanes of a float4 per instruction (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32); every
-// operation is the IEEE one, so results equal the scalar forms bit for bit.
+// float4 arithmetic on pairs.  Every operation is the IEEE one; the build keeps the compiler from forming packed fp32
+// instructions of them (see the Makefile), so each pair is two scalar instructions with the same results.
 using f32x2 = __attribute__((ext_vector_type(2))) float;
 __device__ __forceinline__ float4 pack4(f32x2 lo, f32x2 hi) { return make_float4(lo.x, lo.y, hi.x, hi.y); }
 __device__ __forceinline__ float4 operator+(float4 a, float4 b) {
