@@ -501,7 +501,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
     const int n = min(C, p1 - c0);                       // tokens in this chunk
     const int shift = w.shift && c0 == 0 ? 1 : 0;
     __syncthreads();
-    if (P < 128 || c0 + C < p1) fetch(c0 + C);              // behind the last chunk: zeros, without an access
+    if (P < 128 || STATE_ONLY || c0 + C < p1) fetch(c0 + C);   // behind the last chunk: zeros, without an access
     float unit_p = 1.f, unit_x = 1.f, back = 1.f, unit_v = 1.f, carry = 1.f, largest = 0.f;
     if constexpr (F16) {
       float big[3];
@@ -795,7 +795,8 @@ void walk_launch_16(const WalkSet& set, int n, int sums, hipStream_t st) {
   const int d = set.w[0].dk > set.w[0].dv ? set.w[0].dk : set.w[0].dv;
   const bool vec = walk_vec(set, n);
   // tokens per chunk: 32 where 64 would spill registers (heads of 128: 273 -> 251 us for 32 clips of 2048 tokens, 16 heads) or
-  // cost a workgroup per CU (heads of 64 in bf16: 139 -> 126 us for 64 clips of 2048 tokens, 8 heads; in fp16 150 -> 163)
+  // cost a workgroup per CU (heads of 64 in bf16: 139 -> 126 us for 64 clips of 2048 tokens, 8 heads; in fp16 150 -> 163); a pass that keeps only the state
+  // has the registers for 64 (60001 tokens, 16 heads of 128: 149 -> 134 us)
   constexpr int C64 = __is_same(T, bf16_t) ? 32 : 64;
   walk_passes(set, n, sums, st, [&](dim3 grid, auto only) {
     constexpr bool ONLY = decltype(only)::value;
@@ -806,7 +807,7 @@ void walk_launch_16(const WalkSet& set, int n, int sums, hipStream_t st) {
   } while (0)
     if (d <= 32) GO(32, 64);
     else if (d <= 64) GO(64, C64);
-    else GO(128, 32);
+    else GO(128, (ONLY ? 64 : 32));
 #undef GO
   });
 }
@@ -820,15 +821,22 @@ int walk_launch(const WalkSet& set, int n, int sums, int dtype, hipStream_t st) 
 
 // Segments of the token axis.  From `full` (clip, head) pairs on, clips and heads fill the GPU well enough that the second
 // read of k and v costs more than it gives; below, the axis is cut until there are `target` workgroups.  A workgroup has one wave
-// per 16 columns (fp32: at most four), so narrow heads need more of them.  Measured on 2048 tokens, us per forward pass with
-// 1 / 2 / 4 / 8 segments: bf16, heads of 128: 256 pairs 176 / 197 / 236 / 297, 128 pairs 152 / 132 / 127 / 159; heads of 64: 512
-// pairs 133 / 186 / 198 / 234, 128 pairs 92 / 73 / 60 / 61; heads of 32: 512 pairs 93 / 106 / 122 / 130, 128 pairs 82 / 62 / 44 /
-// 42; fp32, heads of 128: 256 pairs 489 / 554 / 568 / 641, heads of 16: 1024 pairs 183 / 205 / 239 / 246, 256 pairs 159 / 112 / 69 / 70.
+// per 16 columns (fp32: at most four), so narrow heads need more of them; a backward pass has three walks per pair in flight and
+// pays for segments with two sums, so it needs fewer.  Measured on 2048 tokens, us with 1 / 2 / 4 / 8 segments, forward:
+//   bf16, heads of 16: 256 pairs 54 / 62 / 62 / 69, 128 pairs 53 / 52 / 39 / 41; of 64: 256 pairs 79 / 96 / 96 / 106, 192 pairs
+//   74 / 83 / 69 / 73; of 128: 192 pairs 129 / 158 / 160 / 204, 128 pairs 126 / 116 / 107 / 130; fp16, heads of 16: 384 pairs
+//   114 / 97 / 105 / 104; fp32, heads of 128: 192 pairs 422 / 477 / 423 / 445, 128 pairs 419 / 345 / 293 / 306
+// backward: bf16, heads of 64: 128 pairs 91 / 104 / 102 / 116, 64 pairs 76 / 84 / 62 / 65; of 128: 96 pairs 183 / 220 / 208 / 250;
+//   fp32, heads of 128: 128 pairs 670 / 711 / 700 / 746, 96 pairs 668 / 699 / 577 / 576.
 // No segment is shorter than 64 tokens or than twice the head: its state is written, scanned and read again.
-int walk_segments(long bh, int T, int d, bool half) {
-  static const int fill[2][4][2] = {{{1024, 2048}, {1024, 2048}, {256, 1024}, {256, 512}},
-                                    {{512, 1024}, {512, 1024}, {512, 512}, {256, 512}}};
-  const int* f = fill[half][d <= 16 ? 0 : d <= 32 ? 1 : d <= 64 ? 2 : 3];
+int walk_nseg(int B, int T, int H, int dk, int dv, int dtype, int backward) {
+  static const int rule[3][2][4][2] = {   // {full, target} by type, direction and heads of up to 16, 32, 64, 128
+      {{{384, 1024}, {512, 1024}, {256, 768}, {192, 512}}, {{192, 384}, {256, 512}, {128, 256}, {128, 256}}},    // fp32
+      {{{256, 768}, {256, 768}, {256, 768}, {192, 512}}, {{128, 256}, {128, 256}, {128, 256}, {64, 256}}},       // bf16
+      {{{512, 1024}, {512, 1024}, {384, 768}, {192, 512}}, {{192, 384}, {192, 384}, {128, 256}, {96, 256}}}};    // fp16
+  const int d = dk > dv ? dk : dv;
+  const int* f = rule[dtype][backward ? 1 : 0][d <= 16 ? 0 : d <= 32 ? 1 : d <= 64 ? 2 : 3];
+  const long bh = (long)B * H;
   if (bh >= f[0]) return 1;
   const long want = (f[1] + bh - 1) / bh, most = T / (d <= 32 ? 64 : 2 * d);
   const long n = want < most ? want : most;
@@ -856,12 +864,6 @@ static const char* walk_plan(WalkArgs& w, int nseg, int dtype) {
   w.va = rows_vec(w.a, w.sa, w.dk, piece, es), w.vk = rows_vec(w.k, w.sk, w.dk, piece, es);
   w.vv = rows_vec(w.v, w.sv, w.dv, piece, es), w.vo = rows_vec(w.o, w.so, w.dv, piece, es);
   return nullptr;
-}
-
-// The backward pass has three walks per pair in flight, and segments cost it two sums; it is best uncut from about 128 pairs on
-// (heads of 64 in bf16, 128 pairs of 2048 tokens: 89 us, 102 with two segments; heads of 16 in fp32: 94, 81, with four 72).
-static int walk_nseg(int B, int T, int H, int dk, int dv, int dtype, int backward) {
-  return walk_segments((long)B * H * (backward ? 4 : 1), T, dk > dv ? dk : dv, dtype != NOISE_F32);
 }
 
 // Floats of workspace a forward (backward) pass of this shape needs.
