@@ -93,6 +93,7 @@ class MultiTensorAdamW:
                 raise TypeError(f"parameter {i} is {p.dtype}: float32, bfloat16 or float16 expected")
             if not p.is_contiguous():
                 raise ValueError(f"parameter {i} of shape {tuple(p.shape)} is not contiguous")
+        self._apart(self.params)
         self.lr, self.betas, self.eps, self.weight_decay = float(lr), (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
         self.state_bits = state_bits
         n = len(self.params)
@@ -147,7 +148,7 @@ class MultiTensorAdamW:
             index, mask = array.array("i", live), array.array("Q", bytes(len(mask) * 8))
             for i in live:
                 mask[i >> 6] |= 1 << (i & 63)
-        addresses = self._check(live, params, grads, shapes, types, addresses)
+        addresses = self._check(live, params, grads, shapes, types, numel, addresses)
         gtypes = list(map(attrgetter("dtype"), grads))
         kinds = set(zip(types, gtypes))
         for pd, gd in kinds:
@@ -174,7 +175,7 @@ class MultiTensorAdamW:
                           nbytes=sum(part[2]) * (state_bytes + 2 * pd.itemsize + gd.itemsize) if _lib.PROFILE is not None else 0)
         _lib.written(*params)      # the models' checks for stale weights go by the version counters, too
 
-    def _check(self, live, params, grads, shapes, types, addresses):
+    def _check(self, live, params, grads, shapes, types, numel, addresses):
         """The parameters' addresses, after the checks.  Whole-list comparisons first: a step of many small tensors is as fast
         as the loops over them are."""
         T = torch.Tensor
@@ -186,11 +187,21 @@ class MultiTensorAdamW:
         if not all(map(T.is_contiguous, grads)):
             grads[:] = [g.contiguous() for g in grads]
         now = array.array("Q", map(T.data_ptr, params))
-        if not all(map(T.is_contiguous, params)) or (now != addresses and (
-                list(map(attrgetter("shape"), params)) != shapes or list(map(T.get_device, params)) != here
-                or list(map(attrgetter("dtype"), params)) != types)):
+        # types and sizes whatever the addresses: a rebound parameter may have got its old address again
+        if (not all(map(T.is_contiguous, params)) or list(map(attrgetter("dtype"), params)) != types
+                or list(map(T.numel, params)) != list(numel)
+                or (now != addresses and (list(map(attrgetter("shape"), params)) != shapes or list(map(T.get_device, params)) != here))):
             raise RuntimeError("a parameter was moved, resized, converted or transposed after the optimizer was built")
+        if now != addresses:
+            self._apart(params)
         return now
+
+    @staticmethod
+    def _apart(params):
+        """Refuses parameters that share memory: one launch updates them side by side, in no order."""
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("two parameters share memory")
 
     def state_dict(self):
         return {**{k: v.clone() for k, v in self.state.items()}, "step": self.step_count.clone(), "state_bits": self.state_bits,

@@ -265,6 +265,34 @@ def test_refusals():
     assert torch.equal(q, b.params[0])
 
 
+def test_parameters_that_were_rebound_or_share_memory():
+    """A parameter with other values behind its old address is refused; one with new memory of the same kind is followed."""
+    import noise_amd as na
+    make = lambda: [torch.nn.Parameter(torch.ones(1000, device=DEV)), torch.nn.Parameter(torch.ones(64, device=DEV))]
+    grads = [torch.ones(1000, device=DEV), torch.ones(64, device=DEV)]
+    for rebind in (lambda t: t[:500], lambda t: t[:0], lambda t: t.view(torch.bfloat16)[:1000], lambda t: t.view(torch.float16)):
+        for some in (grads, [grads[0], None]):
+            p = make()
+            opt = na.MultiTensorAdamW(p)
+            p[0].data = rebind(p[0].data)
+            with pytest.raises(RuntimeError, match="after the optimizer was built"):
+                opt.step(grads=some)
+            assert not opt.step_count.any() and (p[1] == 1).all()
+    p = make()
+    opt = na.MultiTensorAdamW(p, lr=1e-2, weight_decay=0.0)
+    p[0].data = torch.full((1000,), 2.0, device=DEV)
+    opt.step(grads=grads)
+    assert ((p[0] - 1.99).abs() < 1e-5).all() and ((p[1] - 0.99).abs() < 1e-5).all()
+    p[0].data = torch.ones(1064, device=DEV)[:1000]
+    p[1].data = p[0].data[936:]
+    with pytest.raises(ValueError, match="share memory"):
+        opt.step(grads=grads)
+    both = torch.ones(100, device=DEV)
+    with pytest.raises(ValueError, match="share memory"):
+        na.MultiTensorAdamW([torch.nn.Parameter(both[:60]), torch.nn.Parameter(both[59:])])
+    na.MultiTensorAdamW([torch.nn.Parameter(both[:60]), torch.nn.Parameter(both[60:]), torch.nn.Parameter(both[:0])])
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_captured_step_replays(bits):
     import noise_amd as na
