@@ -55,9 +55,10 @@ using u32x4 = __attribute__((ext_vector_type(4))) unsigned;
 using u32x2 = __attribute__((ext_vector_type(2))) unsigned;
 
 // Rows of a chunk as a buffer: accesses behind its end read zero and store nothing, so that neither the clip's last chunk nor
-// columns behind the head need a branch.  `rows` of them, `stride` elements of `esize` bytes apart, `width` elements each.
+// columns behind the head need a branch.  `rows` of them (at most zero: none), `stride` >= `width` elements of `esize` bytes apart,
+// `width` elements each.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_rows(const void* first, int rows, long stride, int width, int esize) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)first, 0, rows > 0 ? (int)(((rows - 1) * stride + width) * esize) : 0, 0x00020000);
+  return __builtin_amdgcn_make_buffer_rsrc((void*)first, 0, max((rows - 1) * (int)stride + width, 0) * esize, 0x00020000);
 }
 // A byte offset into such a buffer; one before its start, or of a column that does not exist, lands far behind its end.
 __device__ __forceinline__ int chunk_offset(int off, bool exists) { return (int)min((unsigned)(exists ? off : -1), 0x80000000u); }
@@ -70,7 +71,7 @@ __device__ __forceinline__ int chunk_offset(int off, bool exists) { return (int)
 // the C x C weights pass through LDS (each wave computes a share of them).
 // VEC: rows of a, k, v and o allow 16-byte accesses; otherwise elements go one by one, through the same buffers.
 template <int P, bool STATE_ONLY, bool VEC>
-__global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_f32_kernel(WalkSet set) {
+__global__ __launch_bounds__(P >= 64 ? 256 : P * 4, 2) void walk_f32_kernel(WalkSet set) {
   const WalkArgs& w = set.w[blockIdx.y];
   constexpr int NW = P >= 64 ? 4 : P / 16, NT = P / 16 / NW, KT = P / 16, NTHR = NW * 64;
   constexpr int LD = P + 4, LDP = DA_C + 4, SLOTS = DA_C * P / 4 / NTHR, RS = NTHR / (P / 4);
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
   __shared__ float pw[DA_C + 1];                             // lam^i
   __shared__ float pv[2 * DA_C];                             // s_kv lam^{31-i}; a chunk of n tokens starts at 32 - n
   __shared__ float pp[DA_C + 16];                            // [15 + i - j]: s_o s_kv lam^{i-j}
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, q = lane >> 4, l16 = lane & 15;
+  const int tid = threadIdx.x, wave = NW == 1 ? 0 : tid >> 6, lane = tid & 63, q = lane >> 4, l16 = lane & 15;
   const int bh = blockIdx.x % (w.B * w.H), seg = blockIdx.x / (w.B * w.H);
   const int b = bh / w.H, h = bh % w.H;
   const int len = w.lengths ? min(max(w.lengths[b], 0), w.T) : w.T;
@@ -122,15 +123,20 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
         }
   }
 
+  // arguments of the loop stay in registers: loading one again there waits for every LDS read under way (with a chunk's code in
+  // one block, 64 clips of 1001 tokens, 8 heads: fp32 heads of 16 51 -> 44 us forward, of 64 133 -> 127)
+  float s_o = w.s_o;
+  int reverse = w.reverse, dk = w.dk, dv = w.dv, sa_t = (int)w.sa.t, sk_t = (int)w.sk.t, sv_t = (int)w.sv.t, so_t = (int)w.so.t;
+  asm("" : "+s"(s_o), "+s"(reverse), "+s"(dk), "+s"(dv), "+s"(sa_t), "+s"(sk_t), "+s"(sv_t), "+s"(so_t));
   // a thread's SLOTS pieces of a tile are RS rows apart, in the same column
   const int i0 = tid / (P / 4), cc = tid % (P / 4) * 4;
-  const int dir = w.reverse ? -1 : 1;
+  const int dir = reverse ? -1 : 1;
   f32x4 ra[STATE_ONLY ? 1 : SLOTS], rk[SLOTS], rv[SLOTS];
-  auto rows4 = [&](const float* base, const Strides& st, int width, int c0, f32x4 (&out)[SLOTS]) {
+  auto rows4 = [&](const float* base, int st, int width, int c0, f32x4 (&out)[SLOTS]) {
     const int n = min(DA_C, p1 - c0);                       // none or fewer behind the last chunk
-    const auto rs = chunk_rows(base + (w.reverse ? len - c0 - n : c0) * st.t, n, st.t, width, 4);
-    const int step = dir * RS * 4 * (int)st.t;
-    int off = (w.reverse ? n - 1 - i0 : i0) * 4 * (int)st.t + 4 * cc;
+    const auto rs = chunk_rows(base + (reverse ? len - c0 - n : c0) * (long)st, n, st, width, 4);
+    const int step = dir * RS * 4 * st;
+    int off = (reverse ? n - 1 - i0 : i0) * 4 * st + 4 * cc;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s, off += step) {
       if (VEC) {
@@ -143,9 +149,9 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
     }
   };
   auto fetch = [&](int c0) {
-    if constexpr (!STATE_ONLY) rows4(ab, w.sa, w.dk, c0, ra);
-    rows4(kb, w.sk, w.dk, c0, rk);
-    rows4(vb, w.sv, w.dv, c0, rv);
+    if constexpr (!STATE_ONLY) rows4(ab, sa_t, dk, c0, ra);
+    rows4(kb, sk_t, dk, c0, rk);
+    rows4(vb, sv_t, dv, c0, rv);
   };
   auto put = [&]() {
 #pragma unroll
@@ -205,7 +211,7 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
 #pragma unroll
             for (int r = 0; r < 4; ++r) O[mt][nt] = __builtin_amdgcn_mfma_f32_16x16x4f32(X[kt][nt][r], x[r], O[mt][nt], 0, 0, 0);
         }
-        const float f = w.s_o * pw[mt * 16 + l16 + 1 - shift];
+        const float f = s_o * pw[mt * 16 + l16 + 1 - shift];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) O[mt][nt] *= f;
       }
@@ -254,19 +260,19 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
     // store (memory operations are counted in order)
     put();
     if (!STATE_ONLY) {
-      const auto rs = chunk_rows(ob + (w.reverse ? len - c0 - n : c0) * w.so.t, n, w.so.t, w.dv, 4);
+      const auto rs = chunk_rows(ob + (reverse ? len - c0 - n : c0) * (long)so_t, n, so_t, dv, 4);
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
-        const int i = mt * 16 + l16, off = (w.reverse ? n - 1 - i : i) * 4 * (int)w.so.t;
+        const int i = mt * 16 + l16, off = (reverse ? n - 1 - i : i) * 4 * so_t;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const int col = (wave * NT + nt) * 16 + 4 * q;
           if (VEC) {
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, O[mt][nt]), rs, chunk_offset(off + 4 * col, i < n && col < w.dv), 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, O[mt][nt]), rs, chunk_offset(off + 4 * col, i < n && col < dv), 0, 0);
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(O[mt][nt][e]), rs, chunk_offset(off + 4 * (col + e), i < n && col + e < w.dv), 0, 0);
+              __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(O[mt][nt][e]), rs, chunk_offset(off + 4 * (col + e), i < n && col + e < dv), 0, 0);
           }
         }
       }
@@ -287,7 +293,7 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, P == 128 ? 2 : 1) void walk_
       }
 }
 
-// 16-bit tokens on the 16-bit matrix cores (v_mfma_f32_16x16x32_bf16 / _f16), 64 tokens per chunk, P / 16 waves that own 16
+// 16-bit tokens on the 16-bit matrix cores (v_mfma_f32_16x16x32_bf16 / _f16), 32 or 64 tokens per chunk, P / 16 waves that own 16
 // state columns each.  What is rounded to 16 bits on its way into a product, and what is not:
 //   * the weights lam^{i-j} (a_i . k_j) and the state as it meets a_i: once each, like the output they lead to;
 //   * lam^{n-1-j} v_j on its way into the state is split into three terms of the type (24 bits), since the state is fp32,
@@ -436,17 +442,21 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
     bound = wave_reduce_max(bound);
   }
 
+  // as in the fp32 kernel: in registers for the loop
+  float s_o = w.s_o;
+  int reverse = w.reverse, dk = w.dk, dv = w.dv, sa_t = (int)w.sa.t, sk_t = (int)w.sk.t, sv_t = (int)w.sv.t, so_t = (int)w.so.t;
+  asm("" : "+s"(s_o), "+s"(reverse), "+s"(dk), "+s"(dv), "+s"(sa_t), "+s"(sk_t), "+s"(sv_t), "+s"(so_t));
   // a thread's SLOTS pieces of a tile are RS rows apart, in the same column
   constexpr int RS = NTHR / (P / 8);
   const int i0 = tid / (P / 8), cc = tid % (P / 8) * 8;
-  const int dir = w.reverse ? -1 : 1;
+  const int dir = reverse ? -1 : 1;
   u32x4 ra[STATE_ONLY ? 1 : SLOTS], rk[SLOTS], rv[SLOTS];
-  auto rows8 = [&](const T* base, const Strides& st, int width, bool vec, int c0, u32x4 (&out)[SLOTS]) {
+  auto rows8 = [&](const T* base, int st, int width, bool vec, int c0, u32x4 (&out)[SLOTS]) {
     const int n = min(C, p1 - c0);                       // none or fewer behind the last chunk
     if (VEC) {
-      const auto rs = chunk_rows(base + (w.reverse ? len - c0 - n : c0) * st.t, n, st.t, width, 2);
-      const int step = dir * RS * 2 * (int)st.t;
-      int off = (w.reverse ? n - 1 - i0 : i0) * 2 * (int)st.t + 2 * cc;
+      const auto rs = chunk_rows(base + (reverse ? len - c0 - n : c0) * (long)st, n, st, width, 2);
+      const int step = dir * RS * 2 * st;
+      int off = (reverse ? n - 1 - i0 : i0) * 2 * st + 2 * cc;
 #pragma unroll
       for (int s = 0; s < SLOTS; ++s, off += step)
         out[s] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, chunk_offset(off, cc < width), 0, 0));
@@ -455,14 +465,14 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
       for (int s = 0; s < SLOTS; ++s) {
         const int p = c0 + i0 + s * RS;
         const bool live = p < p1;
-        out[s] = row8(base + (live ? (w.reverse ? len - 1 - p : p) : 0) * st.t, live, cc, width, vec);
+        out[s] = row8(base + (live ? (reverse ? len - 1 - p : p) : 0) * (long)st, live, cc, width, vec);
       }
     }
   };
   auto fetch = [&](int c0) {
-    if constexpr (!STATE_ONLY) rows8(ab, w.sa, w.dk, w.va, c0, ra);
-    rows8(kb, w.sk, w.dk, w.vk, c0, rk);
-    rows8(vb, w.sv, w.dv, w.vv, c0, rv);
+    if constexpr (!STATE_ONLY) rows8(ab, sa_t, dk, w.va, c0, ra);
+    rows8(kb, sk_t, dk, w.vk, c0, rk);
+    rows8(vb, sv_t, dv, w.vv, c0, rv);
   };
   auto put = [&]() {
 #pragma unroll
@@ -512,7 +522,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
         for (int i = 0; i < NW; ++i) u = max(u, STATE_ONLY && z == 0 ? 0u : top[z * NW + i]);
         big[z] = (float)__builtin_bit_cast(f16_t, (unsigned short)u);
       }
-      const int ep = scale_for((float)P * fabsf(w.s_o * w.s_kv) * big[0] * big[1], 15), ev = scale_for(fabsf(w.s_kv) * big[2], 15);
+      const int ep = scale_for((float)P * fabsf(s_o * w.s_kv) * big[0] * big[1], 15), ev = scale_for(fabsf(w.s_kv) * big[2], 15);
       const int ex = scale_for(bound, 14);
       unit_p = pow2(ep);                // weights
       unit_x = pow2(ex - E);            // X as an operand
@@ -570,7 +580,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
         }
       }
 #pragma unroll
-      for (int it = 0; it < NI; ++it) O[it] *= w.s_o * pw[it * 16 + l16 + 1 - shift] * back;
+      for (int it = 0; it < NI; ++it) O[it] *= s_o * pw[it * 16 + l16 + 1 - shift] * back;
     }
     // ---- X = lam^n X + K^T V'
     x8<T> v[C / 32];
@@ -627,21 +637,21 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
     if constexpr (P < 128) put();
     if (!STATE_ONLY) {
       const int col = col0 + 4 * q;
-      const auto rs = chunk_rows(ob + (w.reverse ? len - c0 - n : c0) * w.so.t, n, w.so.t, w.dv, 2);
+      const auto rs = chunk_rows(ob + (reverse ? len - c0 - n : c0) * (long)so_t, n, so_t, dv, 2);
 #pragma unroll
       for (int it = 0; it < NI; ++it) {
         const int i = it * 16 + l16;
         if constexpr (F16) O[it] *= 1.f / unit_p;
         const u32x2 y = {pack16<T>(O[it][0], O[it][1]), pack16<T>(O[it][2], O[it][3])};
-        const int row = w.reverse ? n - 1 - i : i;
+        const int row = reverse ? n - 1 - i : i;
         if (VEC) {
-          __builtin_amdgcn_raw_buffer_store_b64(y, rs, chunk_offset(row * 2 * (int)w.so.t + 2 * col, col < w.dv), 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b64(y, rs, chunk_offset(row * 2 * so_t + 2 * col, col < dv), 0, 0);
         } else if (i < n) {
-          T* op = ob + ((w.reverse ? len - c0 - n : c0) + row) * w.so.t + col;
+          T* op = ob + ((reverse ? len - c0 - n : c0) + row) * (long)so_t + col;
           const auto z = __builtin_bit_cast(typename VecOf<T, 4>::type, y);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (col + e < w.dv) op[e] = z[e];
+            if (col + e < dv) op[e] = z[e];
         }
       }
     }
@@ -795,7 +805,8 @@ void walk_launch_16(const WalkSet& set, int n, int sums, hipStream_t st) {
   const int d = set.w[0].dk > set.w[0].dv ? set.w[0].dk : set.w[0].dv;
   const bool vec = walk_vec(set, n);
   // tokens per chunk: 32 where 64 would spill registers (heads of 128: 273 -> 251 us for 32 clips of 2048 tokens, 16 heads) or
-  // cost a workgroup per CU (heads of 64 in bf16: 139 -> 126 us for 64 clips of 2048 tokens, 8 heads; in fp16 150 -> 163); a pass that keeps only the state
+  // cost a workgroup per CU (heads of 64 in bf16: 139 -> 126 us for 64 clips of 2048 tokens, 8 heads; in fp16 150 -> 163; heads of
+  // 16 in bf16, 64 clips of 1001: forward 44 -> 39 us, backward 109 -> 97, one clip of 60001 with 16 heads of 32: 283 -> 331); a pass that keeps only the state
   // has the registers for 64 (60001 tokens, 16 heads of 128: 149 -> 134 us)
   constexpr int C64 = __is_same(T, bf16_t) ? 32 : 64;
   walk_passes(set, n, sums, st, [&](dim3 grid, auto only) {
@@ -805,7 +816,7 @@ void walk_launch_16(const WalkSet& set, int n, int sums, hipStream_t st) {
     if (vec) hipLaunchKernelGGL((walk_16_kernel<T, P, C, ONLY, true>), grid, dim3(P * 4), 0, st, set); \
     else hipLaunchKernelGGL((walk_16_kernel<T, P, C, ONLY, false>), grid, dim3(P * 4), 0, st, set);    \
   } while (0)
-    if (d <= 32) GO(32, 64);
+    if (d <= 32) GO(32, C64);
     else if (d <= 64) GO(64, C64);
     else GO(128, (ONLY ? 64 : 32));
 #undef GO
