@@ -58,7 +58,7 @@ class FusedAdamW:
 
 
 class MultiTensorAdamW:
-    """AdamW over separate parameter tensors (fp32, bf16 or fp16, contiguous, on one GPU), a few launches per step for the
+    """AdamW over separate parameter tensors (fp32, bf16 or fp16, contiguous, apart in memory, on one GPU), a few launches per step for the
     whole list.
 
     Gradients have their parameter's type; an fp32 parameter also takes bf16 or fp16 gradients.  A parameter whose
