@@ -183,9 +183,9 @@ def decay_attention_step(q, k, v, log_decay, state, scale=None, out=None):
     scale = dk ** -0.5 if scale is None else float(scale)
     with _lib.on_device(q, k, v, log_decay, state, out):
         if B * H:
-            q, k, v = _unit(q), _unit(k), _unit(v)
+            q, k, v, g = _unit(q), _unit(k), _unit(v), log_decay.contiguous()
             strides = (_L * 6)(*q.stride()[:2], *k.stride()[:2], *v.stride()[:2])
-            _lib.call("noise_decay_attn_step", ptr(q), ptr(k), ptr(v), strides, ptr(log_decay.contiguous()), ptr(state), ptr(out),
+            _lib.call("noise_decay_attn_step", ptr(q), ptr(k), ptr(v), strides, ptr(g), ptr(state), ptr(out),
                       scale, B, H, dk, dv, _lib.DTYPES[q.dtype], _lib.stream(), nbytes=8 * state.numel())
     _lib.written(state, out)
     return out

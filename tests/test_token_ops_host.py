@@ -86,3 +86,55 @@ def test_c_entry_points_refuse_bad_arguments():
     for bad in (dict(off=array.array("l", [100])), dict(l=array.array("l", [-1])), dict(q=array.array("Q", [0]))):
         with pytest.raises(RuntimeError, match="tensor 0"):
             _lib.call("noise_adamw_multi", a(bad.get("q", q)), a(q), a(bad.get("l", l)), a(bad.get("off", off)), a(i), 1, 0, 0, 32, *tail)
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """The wrappers' own work on CPU tensors: calls of the library go to the list that this returns as (name, arguments) or, when
+    `during` is set, to that function."""
+    import contextlib
+    from noise_amd import _lib
+
+    class Calls(list):
+        during = None
+
+    calls = Calls()
+
+    def call(name, *args, nbytes=0):
+        calls.append((name, args))
+        if calls.during is not None:
+            calls.during(name, args)
+
+    monkeypatch.setattr(_lib, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(_lib, "on_device", lambda *t: contextlib.nullcontext())
+    monkeypatch.setattr(_lib, "stream", lambda: ctypes.c_void_p(0))
+    monkeypatch.setattr(_lib, "call", call)
+    return calls
+
+
+@pytest.mark.parametrize("form", ["step", "fwd", "bwd"])
+def test_copies_live_until_the_kernel_is_launched(on_cpu, monkeypatch, form):
+    """Every tensor whose address goes to a kernel is held until the call has returned, packed copies of strided arguments too:
+    memory that is free before the launch can be handed out and written ahead of it by another thread on the same stream."""
+    import weakref
+    from noise_amd import decay_attn as da
+    seen = []
+
+    def ptr(t):
+        if t is not None:
+            seen.append(weakref.ref(t))
+        return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+    dead = []
+    on_cpu.during = lambda name, args: dead.extend(r for r in seen if r() is None)
+    monkeypatch.setattr(da, "ptr", ptr)
+    strided = lambda *s: torch.zeros(*s, 2)[..., 0]
+    q, k, v = (strided(2, 3, 4, 8) for _ in range(3))
+    g, state, lengths = strided(4), strided(2, 4, 8, 8), torch.zeros(2, 2, dtype=torch.int64)[:, 0]
+    if form == "step":
+        da.decay_attention_step(q[:, 0], k[:, 0], v[:, 0], g, state.contiguous())
+    elif form == "fwd":
+        da.decay_attention_fwd(q, k, v, g, state, lengths)
+    else:
+        da.decay_attention_bwd(v, q, k, v, g, state, lengths, d_state=state)
+    assert len(on_cpu) == 1 and len(seen) >= 6 and not dead
