@@ -144,7 +144,8 @@ def waveform_loss(enhanced, clean, vad_logit, mr_stft_lambda=0.5, fft_sizes=(512
     L = clean.shape[-1]
     B = clean.numel() // L
     label = torch.empty(B, device=clean.device)
-    _lib.call("noise_vad_label", ptr(clean.detach().contiguous()), ptr(label), B, L, int(min_active), _lib.stream())
+    packed = clean.detach().contiguous()
+    _lib.call("noise_vad_label", ptr(packed), ptr(label), B, L, int(min_active), _lib.stream())
     vad_loss = torch.nn.functional.binary_cross_entropy_with_logits(vad_logit.reshape(B), label)
     l1 = smooth_l1_loss(enhanced, clean, beta=0.5)
     mr = mr_stft_lambda * multi_resolution_stft_loss(enhanced, clean, fft_sizes, hop_lengths, win_lengths)

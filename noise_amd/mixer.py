@@ -42,7 +42,8 @@ def activity_batch(audio, fs=16000, energy_thresh=0.13, target_level=-25.0):
     assert audio.dtype == torch.float64 and audio.dim() == 2
     U, L = audio.shape
     out = torch.empty(U, dtype=torch.float64, device=audio.device)
-    _lib.call("noise_activity", _lib.ptr(audio.contiguous()), _lib.ptr(out), U, L, int(fs), float(energy_thresh),
+    audio = audio.contiguous()
+    _lib.call("noise_activity", _lib.ptr(audio), _lib.ptr(out), U, L, int(fs), float(energy_thresh),
               float(target_level), _lib.stream())
     return out
 

@@ -250,17 +250,18 @@ class STFT(torch.nn.Module):
         B, _, F, T = log_magnitude.shape
         sym, _, inv_basisT, _, inv_basisF = self._bases()
         g = grad_out.contiguous().float()
+        lm, ph = log_magnitude.contiguous().float(), phase.contiguous().float()     # held until the launch
         if d_lm is None:
-            d_lm = torch.empty_like(log_magnitude, dtype=torch.float32)
+            d_lm = torch.empty_like(lm)     # packed, whatever the order of log_magnitude's axes
         fft = self._fft()
         if fft is not None:
-            _lib.call("noise_istft_bwd_fft", _lib.ptr(g), _lib.ptr(out), _lib.ptr(log_magnitude.contiguous()),
-                      _lib.ptr(phase.contiguous()), _lib.ptr(fft[1]), _lib.ptr(fft[2]), _lib.ptr(fft[3]),
+            _lib.call("noise_istft_bwd_fft", _lib.ptr(g), _lib.ptr(out), _lib.ptr(lm), _lib.ptr(ph),
+                      _lib.ptr(fft[1]), _lib.ptr(fft[2]), _lib.ptr(fft[3]),
                       _lib.ptr(self.window_sum), _lib.ptr(d_lm), int(accumulate), B, T, self.n_fft, self.hop_length,
                       _lib.stream(), nbytes=8 * g.numel() + (12 + 4 * int(accumulate)) * B * F * T)
             return d_lm
-        _lib.call("noise_istft_bwd_sym" if sym else "noise_istft_bwd", _lib.ptr(g), _lib.ptr(out), _lib.ptr(log_magnitude.contiguous()),
-                  _lib.ptr(phase.contiguous()), _lib.ptr(inv_basisF if sym else inv_basisT), _lib.ptr(self.window_sum), _lib.ptr(d_lm),
+        _lib.call("noise_istft_bwd_sym" if sym else "noise_istft_bwd", _lib.ptr(g), _lib.ptr(out), _lib.ptr(lm),
+                  _lib.ptr(ph), _lib.ptr(inv_basisF if sym else inv_basisT), _lib.ptr(self.window_sum), _lib.ptr(d_lm),
                   int(accumulate), B, T, self.n_fft, self.hop_length, _lib.stream(),
                   nbytes=8 * g.numel() + (12 + 4 * int(accumulate)) * B * F * T)
         return d_lm

@@ -258,3 +258,19 @@ def test_stft_rejects_bad_arguments(dev):
     bad = STFT(100, 320, 100, 320, "hann").to(dev)          # hop does not divide n_fft
     with pytest.raises(RuntimeError):
         bad.forward(torch.zeros(1, 1, 1, 8000, device=dev))
+
+
+@pytest.mark.parametrize("sym", ["fft", True, False])
+def test_istft_backward_of_transposed_inputs(dev, sym):
+    """Spectra whose axes lie in another order: the gradient of the packed ones, value for value."""
+    st = _stft(320, 160, dev, sym=sym)
+    g = torch.Generator().manual_seed(4)
+    lm = (0.3 * torch.randn(3, 1, 21, 161, generator=g)).to(dev).transpose(2, 3)
+    ph = torch.randn(3, 21, 161, generator=g).to(dev).transpose(1, 2)
+    w = torch.randn(3, 1, 1, 20 * 160, generator=g).to(dev)
+    grads = []
+    for a, b in ((lm, ph), (lm.contiguous(), ph.contiguous())):
+        a = a.detach().requires_grad_(True)
+        (st.inverse(a, b) * w).sum().backward()
+        grads.append(a.grad)
+    assert torch.equal(*grads)

@@ -138,3 +138,34 @@ def test_copies_live_until_the_kernel_is_launched(on_cpu, monkeypatch, form):
     else:
         da.decay_attention_bwd(v, q, k, v, g, state, lengths, d_state=state)
     assert len(on_cpu) == 1 and len(seen) >= 6 and not dead
+
+
+def test_copies_of_the_older_wrappers_live_until_the_launch(on_cpu, monkeypatch):
+    """The same for the inverse transform's backward pass, whose two copies would share memory if the first went before the second
+    was made, the activity measure and the activity label."""
+    import weakref
+    from noise_amd import STFT, _lib, losses, mixer
+    seen, dead, got = [], [], {}
+
+    def ptr(t):
+        if t is not None:
+            seen.append(weakref.ref(t))
+            got[t.data_ptr()] = t.is_contiguous()
+        return None if t is None else ctypes.c_void_p(t.data_ptr())
+
+    on_cpu.during = lambda name, args: dead.extend(r for r in seen if r() is None)
+    monkeypatch.setattr(_lib, "ptr", ptr)
+    monkeypatch.setattr(losses, "ptr", ptr)
+    lm, ph = torch.zeros(2, 1, 5, 161).transpose(2, 3), torch.zeros(2, 5, 161).transpose(1, 2)
+    stft = STFT(20, 320, 160, 320, "hann")
+    d_lm = stft._inverse_bwd(torch.zeros(2, 1, 1, 640), torch.zeros(2, 1, 1, 640), lm, ph)
+    assert len(on_cpu) == 1 and not dead and d_lm.shape == lm.shape and all(got.values())
+    seen.clear()
+    mixer.activity_batch(torch.zeros(800, 3, dtype=torch.float64).t())
+    seen.clear()
+    clean = torch.zeros(800, 3).t()
+    monkeypatch.setattr(losses, "smooth_l1_loss", lambda *a, **k: 0.0)
+    monkeypatch.setattr(losses, "multi_resolution_stft_loss", lambda *a, **k: 0.0)
+    monkeypatch.setattr(losses, "_check_pair", lambda *a: None)
+    losses.waveform_loss(clean, clean, torch.zeros(3))
+    assert len(on_cpu) == 3 and not dead
