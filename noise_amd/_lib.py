@@ -8,6 +8,7 @@ import ctypes
 import os
 
 import torch  # imported first so the HIP runtime torch ships is the one the library binds to
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # NOISE_HIP_LIB: another build of the same library (diagnostic builds with phase stamps, see scripts/dbg)
@@ -110,6 +111,16 @@ def require_cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("noise_amd kernels run on the GPU only: got a CPU tensor (no CPU fallback exists)")
+
+
+def no_tangents(*tensors):
+    """Refuses dual tensors of forward-mode differentiation: a kernel's result carries no tangent, which would read as a
+    derivative of zero."""
+    if forward_ad._current_level < 0:      # outside of any dual level: nothing to look for
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("this operator has no forward-mode derivative: use its backward pass")
 
 
 # element types of the token operators (codes of include/noise_hip.h)

@@ -58,6 +58,7 @@ def _tokens(t):
 
 
 def _check(q, k, v, log_decay, state, tokens):
+    _lib.no_tangents(q, k, v, log_decay, state)
     _lib.require_cuda(q, k, v, log_decay, state)
     qs, vs, dims = q.shape, v.shape, 4 if tokens else 3
     if len(qs) != dims or k.shape != qs or len(vs) != dims or vs[:-1] != qs[:-1]:
@@ -118,6 +119,7 @@ def decay_attention_bwd(do, q, k, v, log_decay, state=None, lengths=None, scale=
     """(dq, dk, dv, gradient of `state`) for the gradients `do` of o and `d_state` of the returned state (None: zero)."""
     B, H, dk, dv = _check(q, k, v, log_decay, state, True)
     lengths = _check_lengths(lengths, B)
+    _lib.no_tangents(do, d_state)
     _lib.require_cuda(do, d_state)
     if do.shape != v.shape or do.dtype != v.dtype:
         raise ValueError(f"do must be {tuple(v.shape)} in {v.dtype}, got {tuple(do.shape)} in {do.dtype}")

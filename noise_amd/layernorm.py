@@ -36,6 +36,7 @@ def _rows(t, D):
 
 
 def _check(x, weight, bias):
+    _lib.no_tangents(x, weight, bias)
     _lib.require_cuda(x, weight, bias)
     if x.dtype not in _lib.DTYPES:
         raise TypeError(f"layer_norm takes float32, bfloat16 or float16 activations, got {x.dtype}")
@@ -74,6 +75,7 @@ def layer_norm_bwd(dy, x, mean, rstd, weight=None, need_params=True):
     """(dx, dweight, dbias) for the gradient dy of layer_norm_fwd's y; `weight` None and need_params: the gradients of a
     weight of ones and a bias of zeros, in fp32.  need_params False leaves both None and saves their reduction."""
     D, wdtype = _check(x, weight, None)
+    _lib.no_tangents(dy, mean, rstd)
     _lib.require_cuda(dy, mean, rstd)
     if dy.shape != x.shape or dy.dtype != x.dtype:
         raise ValueError(f"dy must be {tuple(x.shape)} in {x.dtype}, got {tuple(dy.shape)} in {dy.dtype}")

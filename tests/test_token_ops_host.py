@@ -169,3 +169,26 @@ def test_copies_of_the_older_wrappers_live_until_the_launch(on_cpu, monkeypatch)
     monkeypatch.setattr(losses, "_check_pair", lambda *a: None)
     losses.waveform_loss(clean, clean, torch.zeros(3))
     assert len(on_cpu) == 3 and not dead
+
+
+def test_dual_tensors_are_refused(on_cpu):
+    """Forward-mode differentiation: a result without a tangent would be read as a derivative of zero."""
+    import torch.autograd.forward_ad as fwad
+    import noise_amd as na
+    x, w, s = torch.zeros(3, 8), torch.ones(8), torch.zeros(3)
+    t, g, state, one = torch.zeros(1, 3, 2, 8), torch.zeros(2), torch.zeros(1, 2, 8, 8), torch.zeros(1, 2, 8)
+    calls = [(na.layer_norm, (x, w, w)), (na.layer_norm_fwd, (x, w, w)), (na.layer_norm_bwd, (x, x, s, s, w)),
+             (na.decay_attention, (t, t, t, g, state)), (na.decay_attention_fwd, (t, t, t, g, state)),
+             (na.decay_attention_bwd, (t, t, t, t, g, state, None, 1.0, state)), (na.decay_attention_step, (one, one, one, g, state))]
+    for f, args in calls:
+        with fwad.dual_level():
+            f(*args)                    # plain tensors inside a level: as ever
+            done = len(on_cpu)
+            for i, a in enumerate(args):
+                if torch.is_tensor(a):
+                    dual = fwad.make_dual(a, torch.ones_like(a))
+                    with pytest.raises(NotImplementedError, match="forward-mode"):
+                        f(*args[:i], dual, *args[i + 1:])
+                    with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                        f(*args[:i], dual, *args[i + 1:])
+            assert len(on_cpu) == done
