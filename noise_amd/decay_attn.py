@@ -13,9 +13,9 @@ once, this one carries a state of fixed size: whole clips run in chunks, a strea
 
 q and k are (B, T, H, Dk), v is (B, T, H, Dv) with head sizes of 1 to 128, all fp32, bf16 or fp16 with any strides (views of one
 packed projection are read in place; a last axis without unit stride is copied first).  `log_decay` is (H,) fp32, at most 0
-(-inf: no memory), and takes no gradient.  States are (B, H, Dk, Dv) fp32.  `lengths` (B,) integers on the GPU: the tokens of
-clip b at and behind lengths[b] are neither read nor added to the state, their rows of o and of the gradients are zero, and the
-state returned is the one behind the last real token.  `scale` defaults to Dk ** -0.5.
+(-inf: no memory), and takes no gradient.  States are (B, H, Dk, Dv) fp32.  `lengths` (B,) int32 or int64 on the GPU
+(below zero means 0, above T means T): the tokens of clip b at and behind lengths[b] are neither read nor added to the state,
+their rows of o and of the gradients are zero, and the state returned is the one behind the last real token.  `scale` defaults to Dk ** -0.5.
 
 Numbers: states are carried in fp32 accuracy whatever the tokens' type; in 16-bit types the weights inside a chunk and the
 state as it meets q are rounded to the type once each, like the output.  A token that is not finite reaches, besides all later
@@ -80,12 +80,14 @@ def _check_state(name, state, shape):
         raise ValueError(f"{name} must be float32 {shape}, got {state.dtype} {tuple(state.shape)}")
 
 
-def _check_lengths(lengths, B):
+def _check_lengths(lengths, B, T):
     if lengths is None:
         return None
     _lib.require_cuda(lengths)
     if tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"lengths must be ({B},) integers, got {lengths.dtype} {tuple(lengths.shape)}")
+    if lengths.dtype == torch.int64:
+        lengths = lengths.clamp(0, T)       # the kernels' own limits, before the type loses the high bits
     return lengths.to(torch.int32).contiguous()
 
 
@@ -98,7 +100,7 @@ def _workspace(q, dv, backward):
 def decay_attention_fwd(q, k, v, log_decay, state=None, lengths=None, scale=None):
     """(o, state behind the last token): o (B, T, H, Dv) in q's type, the state a new fp32 tensor."""
     B, H, dk, dv = _check(q, k, v, log_decay, state, True)
-    lengths = _check_lengths(lengths, B)
+    lengths = _check_lengths(lengths, B, q.shape[1])
     scale = dk ** -0.5 if scale is None else float(scale)
     with _lib.on_device(q, k, v, log_decay, state, lengths):
         if q.numel() == 0:      # no token: the state as it was
@@ -118,7 +120,7 @@ def decay_attention_fwd(q, k, v, log_decay, state=None, lengths=None, scale=None
 def decay_attention_bwd(do, q, k, v, log_decay, state=None, lengths=None, scale=None, d_state=None):
     """(dq, dk, dv, gradient of `state`) for the gradients `do` of o and `d_state` of the returned state (None: zero)."""
     B, H, dk, dv = _check(q, k, v, log_decay, state, True)
-    lengths = _check_lengths(lengths, B)
+    lengths = _check_lengths(lengths, B, q.shape[1])
     _lib.no_tangents(do, d_state)
     _lib.require_cuda(do, d_state)
     if do.shape != v.shape or do.dtype != v.dtype:

@@ -360,3 +360,17 @@ def test_other_stream_and_captured_graph(dtype):
             eo = na.decay_attention_step(c["q"][:, 0], c["k"][:, 0], c["v"][:, 0], c["log_decay"], st)
             torch.cuda.synchronize()
             assert all(torch.equal(eager[n], held[n]) for n in eager) and torch.equal(eo, step) and torch.equal(st, step_state)
+
+
+@pytest.mark.parametrize("T", [40, 900])
+def test_lengths_outside_of_the_clip(T):
+    """int64 and int32 lengths, below zero and far above T: those of the limits, forwards and backwards."""
+    c = make(6, T, 2, 16, 16, torch.float32, 9)
+    c["lengths"] = torch.tensor([T, T, 0, 0, T, 11], dtype=torch.int32, device=DEV)
+    want = run_all(c)
+    big = torch.iinfo(torch.int64)
+    for lengths in (torch.tensor([2 ** 40, big.max, big.min, -3, T + 1, 11]), torch.tensor([T, 2 ** 32 + 5, -2 ** 32 + 7, 0, 2 ** 31, 11]),
+                    torch.tensor([2 ** 31 - 1, T + 1, -1, -2 ** 31, T, 11], dtype=torch.int32)):
+        c["lengths"] = lengths.to(DEV)
+        got = run_all(c)
+        assert all(torch.equal(want[n], got[n]) for n in want)

@@ -192,3 +192,16 @@ def test_dual_tensors_are_refused(on_cpu):
                     with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
                         f(*args[:i], dual, *args[i + 1:])
             assert len(on_cpu) == done
+
+
+def test_lengths_are_limited_before_they_are_narrowed(on_cpu):
+    """int64 lengths beyond 32 bits mean what they say: all tokens, or none."""
+    import noise_amd as na
+    seen = []
+    on_cpu.during = lambda name, args: seen.append(list((ctypes.c_int * 12).from_address(args[6 if name.endswith("fwd") else 9].value)))
+    big = torch.iinfo(torch.int64)
+    lengths = torch.tensor([2 ** 40, 2 ** 32, 2 ** 32 + 3, big.max, big.min, -2 ** 32 + 2, -1, 0, 3, 7, 8, 2 ** 31])
+    t, g = torch.zeros(12, 7, 1, 8), torch.zeros(1)
+    na.decay_attention_fwd(t, t, t, g, None, lengths)
+    na.decay_attention_bwd(t, t, t, t, g, None, lengths)
+    assert seen == [[min(max(n, 0), 7) for n in lengths.tolist()]] * 2
