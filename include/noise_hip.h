@@ -396,13 +396,14 @@ int noise_layer_norm_bwd(const void* dy, long lddy, const void* x, long ldx, con
  * (elements between clips, tokens and heads of q, k, v, o: 12 values on the HOST; unit stride on the last axis, a token stride
  * of at least the row's width and below 2^22); rows of o at and behind the length are zero.  log_decay g [H] <= 0; lengths [B]
  * or NULL (all T); state (before the first token), end (behind the last) [B][H][dk][dv] fp32 or NULL (zero; not wanted).
- * 1 <= dk, dv <= 128.  workspace: noise_decay_attn_workspace() floats (0: may be NULL) */
+ * state and end must not share memory.  1 <= dk, dv <= 128.  workspace: noise_decay_attn_workspace() floats (0: may be NULL) */
 long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv, int dtype, int backward);
 int noise_decay_attn_fwd(const void* q, const void* k, const void* v, void* o, const long* strides, const float* log_decay,
                          const int* lengths, const float* state, float* end, float* workspace, float scale, int B, int T, int H,
                          int dk, int dv, int dtype, void* stream);
 /* go, d_end: gradients of o and end (d_end NULL: zero); gq, gk, gv, d_state (or NULL): those of q, k, v and state; strides of
- * go, q, k, v, gq, gk, gv (21 values on the HOST).  Rows at and behind the length are neither read nor anything but zero */
+ * go, q, k, v, gq, gk, gv (21 values on the HOST).  Rows at and behind the length are neither read nor anything but zero.
+ * No output may share memory with an input */
 int noise_decay_attn_bwd(const void* go, const void* q, const void* k, const void* v, void* gq, void* gk, void* gv,
                          const long* strides, const float* log_decay, const int* lengths, const float* state, const float* d_end,
                          float* d_state, float* workspace, float scale, int B, int T, int H, int dk, int dv, int dtype,

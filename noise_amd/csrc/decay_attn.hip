@@ -877,6 +877,11 @@ static const char* walk_plan(WalkArgs& w, int nseg, int dtype) {
   return nullptr;
 }
 
+// Whether two buffers of n floats share memory (null: no buffer).
+static bool states_meet(const float* a, const float* b, size_t n) {
+  return a && b && (uintptr_t)a < (uintptr_t)(b + n) && (uintptr_t)b < (uintptr_t)(a + n);
+}
+
 // Floats of workspace a forward (backward) pass of this shape needs.
 NOISE_EXPORT long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv, int dtype, int backward) {
   if (walk_check(B, T, H, dk, dv, dtype)) return 0;
@@ -891,6 +896,8 @@ NOISE_EXPORT int noise_decay_attn_fwd(const void* q, const void* k, const void* 
   const char* why = walk_check(B, T, H, dk, dv, dtype);
   NOISE_REQUIRE(!why, "noise_decay_attn_fwd: %s (B %d, T %d, H %d, head sizes %d and %d)", why, B, T, H, dk, dv);
   NOISE_REQUIRE(q && k && v && o && strides && log_decay, "noise_decay_attn_fwd: null pointer");
+  // the last segment's workgroup writes one while the first's reads the other
+  NOISE_REQUIRE(!states_meet(state, end, (size_t)B * H * dk * dv), "noise_decay_attn_fwd: state and end share memory");
   const Strides* st = (const Strides*)strides;
   WalkSet set = {};
   WalkArgs& w = set.w[0];
@@ -933,6 +940,11 @@ NOISE_EXPORT int noise_decay_attn_bwd(const void* go, const void* q, const void*
     why = walk_plan(w, nseg, dtype);
     NOISE_REQUIRE(!why, "noise_decay_attn_bwd: %s", why);
   }
+  // the three walks run side by side: what one writes no other may read
+  const size_t states = (size_t)B * H * dk * dv;
+  NOISE_REQUIRE(!states_meet(state, d_state, states) && !states_meet(d_end, d_state, states), "noise_decay_attn_bwd: d_state shares memory with state or d_end");
+  for (const void* in : {go, q, k, v})
+    NOISE_REQUIRE(in != dq && in != gk && in != gv, "noise_decay_attn_bwd: a gradient is written over an input");
   walk_launch(set, 3, 2, dtype, (hipStream_t)stream);
   NOISE_CHECK_LAUNCH("noise_decay_attn_bwd");
   return 0;

@@ -205,3 +205,36 @@ def test_lengths_are_limited_before_they_are_narrowed(on_cpu):
     na.decay_attention_fwd(t, t, t, g, None, lengths)
     na.decay_attention_bwd(t, t, t, t, g, None, lengths)
     assert seen == [[min(max(n, 0), 7) for n in lengths.tolist()]] * 2
+
+
+def test_decay_attention_entries_refuse_outputs_over_inputs():
+    """Workgroups of one launch read what such an output would write: refused before any launch."""
+    import array
+    from noise_amd import _lib
+    st = array.array("l", [64, 8, 8] * 7)
+    sp = ctypes.c_void_p(st.buffer_info()[0])
+    at = lambda n: ctypes.c_void_p(n)
+    n = 4 * 2 * 8 * 8          # bytes of a state: one clip, two heads
+
+    def fwd(state, end):
+        _lib.call("noise_decay_attn_fwd", at(16), at(16), at(16), at(16), sp, at(16), None, state, end, None, 1.0, 1, 8, 2, 8, 8, 0, None)
+
+    def bwd(state=None, d_end=None, d_state=None, ins=(16, 32, 48, 64), outs=(80, 96, 112)):
+        _lib.call("noise_decay_attn_bwd", *map(at, ins), *map(at, outs), sp, at(16), None, state, d_end, d_state, None, 1.0, 1, 8, 2, 8, 8, 0, None)
+    for other in (1 << 20, (1 << 20) + n - 4, (1 << 20) - n + 4):
+        with pytest.raises(RuntimeError, match="share"):
+            fwd(at(1 << 20), at(other))
+        with pytest.raises(RuntimeError, match="shares"):
+            bwd(d_end=at(1 << 20), d_state=at(other))
+        with pytest.raises(RuntimeError, match="shares"):
+            bwd(state=at(1 << 20), d_state=at(other))
+    for i in range(4):
+        for o in range(3):
+            outs = [80, 96, 112]
+            outs[o] = 16 * (i + 1)
+            with pytest.raises(RuntimeError, match="over an input"):
+                bwd(outs=tuple(outs))
+    # neighbours are no overlap: these reach the workspace check of a shape cut into segments
+    with pytest.raises(RuntimeError, match="workspace"):
+        _lib.call("noise_decay_attn_fwd", at(16), at(16), at(16), at(16), sp, at(16), None, at(1 << 20), at((1 << 20) + n // 2), None, 1.0, 1, 100000,
+                  1, 8, 8, 0, None)
