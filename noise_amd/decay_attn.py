@@ -13,9 +13,9 @@ once, this one carries a state of fixed size: whole clips run in chunks, a strea
 
 q and k are (B, T, H, Dk), v is (B, T, H, Dv) with head sizes of 1 to 128, all fp32, bf16 or fp16 with any strides (views of one
 packed projection are read in place; a last axis without unit stride is copied first).  `log_decay` is (H,) fp32, at most 0
-(-inf: no memory), and takes no gradient.  States are (B, H, Dk, Dv) fp32.  `lengths` (B,) int32 or int64 on the GPU
-(below zero means 0, above T means T): the tokens of clip b at and behind lengths[b] are neither read nor added to the state,
-their rows of o and of the gradients are zero, and the state returned is the one behind the last real token.  `scale` defaults to Dk ** -0.5.
+(-inf: no memory), and takes no gradient (one that requires it is refused while gradients are recorded).  States are
+(B, H, Dk, Dv) fp32.  `lengths` (B,) int32 or int64 on the GPU (below zero means 0, above T means T): the tokens of clip b at
+and behind lengths[b] are neither read nor added to the state, their rows of o and of the gradients are zero, and the state returned is the one behind the last real token.  `scale` defaults to Dk ** -0.5.
 
 Numbers: states are carried in fp32 accuracy whatever the tokens' type; in 16-bit types the weights inside a chunk and the
 state as it meets q are rounded to the type once each, like the output.  A token that is not finite reaches, besides all later
@@ -163,7 +163,7 @@ class _DecayAttention(torch.autograd.Function):
 
 def decay_attention(q, k, v, log_decay, state=None, lengths=None, scale=None):
     """(o, state behind the last token); back-propagates into q, k, v and state."""
-    if log_decay.requires_grad:
+    if log_decay.requires_grad and torch.is_grad_enabled():
         raise ValueError("log_decay takes no gradient: detach it")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, state)):
         return _DecayAttention.apply(q, k, v, log_decay, state, lengths, scale)

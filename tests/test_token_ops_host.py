@@ -238,3 +238,18 @@ def test_decay_attention_entries_refuse_outputs_over_inputs():
     with pytest.raises(RuntimeError, match="workspace"):
         _lib.call("noise_decay_attn_fwd", at(16), at(16), at(16), at(16), sp, at(16), None, at(1 << 20), at((1 << 20) + n // 2), None, 1.0, 1, 100000,
                   1, 8, 8, 0, None)
+
+
+def test_a_parameter_as_log_decay(on_cpu):
+    """A module may hold log_decay as a parameter and run without gradients; while gradients are recorded it is refused."""
+    import noise_amd as na
+    t, g = torch.zeros(1, 3, 2, 8), torch.nn.Parameter(torch.zeros(2))
+    with pytest.raises(ValueError, match="no gradient"):
+        na.decay_attention(t, t, t, g)
+    assert not on_cpu
+    with torch.no_grad():
+        na.decay_attention(t, t, t, g)
+    with torch.inference_mode():
+        na.decay_attention(t, t, t, g)
+    na.decay_attention(t, t, t, g.detach())
+    assert [name for name, _ in on_cpu] == ["noise_decay_attn_fwd"] * 3
