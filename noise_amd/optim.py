@@ -80,8 +80,7 @@ class MultiTensorAdamW:
             raise ValueError("MultiTensorAdamW got an empty parameter list")
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits is 32 or 8, got {state_bits}")
-        if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and all(0 <= b < 1 for b in betas)):
-            raise ValueError(f"need lr, eps, weight_decay >= 0 and betas in [0, 1): got {lr}, {eps}, {weight_decay}, {betas}")
+        hyper = self._hyper(lr, betas, eps, weight_decay)
         _lib.require_cuda(*self.params)
         if len({id(p) for p in self.params}) < len(self.params):
             raise ValueError("a parameter appears twice in the list")
@@ -94,7 +93,7 @@ class MultiTensorAdamW:
             if not p.is_contiguous():
                 raise ValueError(f"parameter {i} of shape {tuple(p.shape)} is not contiguous")
         self._apart(self.params)
-        self.lr, self.betas, self.eps, self.weight_decay = float(lr), (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
+        self.lr, self.betas, self.eps, self.weight_decay = hyper
         self.state_bits = state_bits
         n = len(self.params)
         self._numel = [p.numel() for p in self.params]
@@ -197,6 +196,12 @@ class MultiTensorAdamW:
         return now
 
     @staticmethod
+    def _hyper(lr, betas, eps, weight_decay):
+        if not (lr >= 0 and eps >= 0 and weight_decay >= 0 and len(betas) == 2 and all(0 <= b < 1 for b in betas)):
+            raise ValueError(f"need lr, eps, weight_decay >= 0 and betas in [0, 1): got {lr}, {eps}, {weight_decay}, {betas}")
+        return float(lr), (float(betas[0]), float(betas[1])), float(eps), float(weight_decay)
+
+    @staticmethod
     def _apart(params):
         """Refuses parameters that share memory: one launch updates them side by side, in no order."""
         spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
@@ -205,15 +210,23 @@ class MultiTensorAdamW:
 
     def state_dict(self):
         return {**{k: v.clone() for k, v in self.state.items()}, "step": self.step_count.clone(), "state_bits": self.state_bits,
-                "lr": self.lr, "betas": self.betas, "eps": self.eps, "weight_decay": self.weight_decay}
+                "sizes": list(self._numel), "lr": self.lr, "betas": self.betas, "eps": self.eps, "weight_decay": self.weight_decay}
 
     def load_state_dict(self, sd):
+        """Everything is checked before the first value is copied.  `sizes`, the parameters' sizes in their order, says which
+        tensor owns which part of the buffers; a checkpoint without it (from before it was kept) is held to the totals only."""
         if sd.get("state_bits") != self.state_bits:
             raise ValueError(f"a checkpoint with {sd.get('state_bits')}-bit states cannot be loaded into {self.state_bits}-bit ones")
         for k, v in {**self.state, "step": self.step_count}.items():
             if k not in sd or sd[k].shape != v.shape or sd[k].dtype != v.dtype:
                 raise ValueError(f"state {k!r} must be {v.dtype} {tuple(v.shape)}")
+        if list(sd.get("sizes", self._numel)) != self._numel:
+            raise ValueError("the checkpoint is of parameters of other sizes or in another order")
+        missing = [k for k in ("lr", "betas", "eps", "weight_decay") if k not in sd]
+        if missing:
+            raise ValueError(f"the checkpoint lacks {', '.join(missing)}")
+        hyper = self._hyper(sd["lr"], sd["betas"], sd["eps"], sd["weight_decay"])
         for k, v in self.state.items():
             v.view(torch.uint8).copy_(sd[k].view(torch.uint8))      # the bytes, of 8-bit values too
         self.step_count.copy_(sd["step"])
-        self.lr, self.betas, self.eps, self.weight_decay = sd["lr"], tuple(sd["betas"]), sd["eps"], sd["weight_decay"]
+        self.lr, self.betas, self.eps, self.weight_decay = hyper

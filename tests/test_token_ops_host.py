@@ -253,3 +253,37 @@ def test_a_parameter_as_log_decay(on_cpu):
         na.decay_attention(t, t, t, g)
     na.decay_attention(t, t, t, g.detach())
     assert [name for name, _ in on_cpu] == ["noise_decay_attn_fwd"] * 3
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_checkpoints_of_other_parameter_lists_are_refused(on_cpu, bits):
+    """Lists of equal totals in another order own other parts of the flat states; a checkpoint that lacks something, or holds a bad
+    number, leaves the optimizer as it was."""
+    import noise_amd as na
+    make = lambda *sizes, **kw: na.MultiTensorAdamW([torch.nn.Parameter(torch.zeros(n)) for n in sizes], state_bits=bits, **kw)
+    fill = lambda opt: [t.view(torch.uint8).fill_(17) for t in opt.state.values()] + [opt.step_count.fill_(5)]
+    src = make(300, 1000, lr=0.5, betas=(0.5, 0.75), eps=0.25, weight_decay=0.125)
+    fill(src)
+    sd = src.state_dict()
+    untouched = lambda o: (o.lr == 1e-4 and o.betas == (0.9, 0.999) and not o.step_count.any()
+                           and not any(t.view(torch.uint8).any() for t in o.state.values()))
+    for sizes in ((1000, 300), (301, 999)):       # both pad to 1536 values of two tensors
+        other = make(*sizes)
+        with pytest.raises(ValueError, match="other sizes"):
+            other.load_state_dict(sd)
+        assert untouched(other)
+    for key in ("lr", "betas", "eps", "weight_decay", "step", "exp_avg", "state_bits"):
+        twin = make(300, 1000)
+        with pytest.raises(ValueError):
+            twin.load_state_dict({k: v for k, v in sd.items() if k != key})
+        assert untouched(twin)
+    for bad in (dict(lr=-1.0), dict(betas=(0.5,)), dict(betas=(0.5, 1.0)), dict(eps=float("nan"))):
+        twin = make(300, 1000)
+        with pytest.raises(ValueError, match="need lr"):
+            twin.load_state_dict({**sd, **bad})
+        assert untouched(twin)
+    for d in (sd, {k: v for k, v in sd.items() if k != "sizes"}):        # the sizes were not always kept
+        twin = make(300, 1000)
+        twin.load_state_dict(d)
+        assert (twin.lr, twin.betas, twin.eps, twin.weight_decay) == (0.5, (0.5, 0.75), 0.25, 0.125) and (twin.step_count == 5).all()
+        assert all((t.view(torch.uint8) == 17).all() for t in twin.state.values())
