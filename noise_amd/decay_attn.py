@@ -15,7 +15,8 @@ q and k are (B, T, H, Dk), v is (B, T, H, Dv) with head sizes of 1 to 128, all f
 packed projection are read in place; a last axis without unit stride is copied first).  `log_decay` is (H,) fp32, at most 0
 (-inf: no memory), and takes no gradient (one that requires it is refused while gradients are recorded).  States are
 (B, H, Dk, Dv) fp32.  `lengths` (B,) int32 or int64 on the GPU (below zero means 0, above T means T): the tokens of clip b at
-and behind lengths[b] are neither read nor added to the state, their rows of o and of the gradients are zero, and the state returned is the one behind the last real token.  `scale` defaults to Dk ** -0.5.
+and behind lengths[b] are neither read nor added to the state, their rows of o and of the gradients are zero, and the state
+returned is the one behind the last real token.  `scale` defaults to Dk ** -0.5.
 
 Numbers: states are carried in fp32 accuracy whatever the tokens' type; in 16-bit types the weights inside a chunk and the
 state as it meets q are rounded to the type once each, like the output.  A token that is not finite reaches, besides all later
@@ -104,7 +105,8 @@ def decay_attention_fwd(q, k, v, log_decay, state=None, lengths=None, scale=None
     scale = dk ** -0.5 if scale is None else float(scale)
     with _lib.on_device(q, k, v, log_decay, state, lengths):
         if q.numel() == 0:      # no token: the state as it was
-            end = torch.zeros(B, H, dk, dv, device=q.device) if state is None else state.clone()
+            end = q.new_empty(B, H, dk, dv, dtype=torch.float32)
+            end.copy_(state) if state is not None else end.zero_()
             return torch.empty(v.shape, device=v.device, dtype=v.dtype), end
         end = q.new_empty(B, H, dk, dv, dtype=torch.float32)
         x0 = state.contiguous() if state is not None else None

@@ -287,3 +287,14 @@ def test_checkpoints_of_other_parameter_lists_are_refused(on_cpu, bits):
         twin.load_state_dict(d)
         assert (twin.lr, twin.betas, twin.eps, twin.weight_decay) == (0.5, (0.5, 0.75), 0.25, 0.125) and (twin.step_count == 5).all()
         assert all((t.view(torch.uint8) == 17).all() for t in twin.state.values())
+
+
+def test_no_tokens_return_a_packed_state(on_cpu):
+    """The state behind no token is a new packed tensor, ready for single tokens, whatever the strides of the one given."""
+    import noise_amd as na
+    t, g = torch.zeros(2, 0, 3, 8), torch.zeros(3)
+    state = torch.arange(2 * 3 * 64, dtype=torch.float32).view(2, 3, 8, 8).transpose(2, 3)
+    o, end = na.decay_attention_fwd(t, t, t, g, state)
+    assert end.is_contiguous() and torch.equal(end, state) and end.data_ptr() != state.data_ptr()
+    na.decay_attention_step(t.new_zeros(2, 3, 8), t.new_zeros(2, 3, 8), t.new_zeros(2, 3, 8), g, end)
+    assert not na.decay_attention_fwd(t, t, t, g)[1].any()
