@@ -102,15 +102,15 @@ class MultiTensorAdamW:
             self.offsets.append(total)
             total += (k + self.BLOCK - 1) // self.BLOCK * self.BLOCK
         total = max(total, self.BLOCK)
-        z = dict(device=dev)
+        z = dict(device=dev, dtype=torch.float32)      # whatever the default type is
         if state_bits == 8:
             # the bytes of +0 are zero
-            small = lambda: torch.zeros(total, dtype=torch.uint8, **z).view(torch.float8_e4m3fn)
+            small = lambda: torch.zeros(total, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn)
             scales = lambda: torch.zeros(total // self.BLOCK, **z)
             self.state = {"exp_avg": small(), "exp_avg_scale": scales(), "exp_avg_sq_root": small(), "exp_avg_sq_root_scale": scales()}
         else:
             self.state = {"exp_avg": torch.zeros(total, **z), "exp_avg_sq": torch.zeros(total, **z)}
-        self.step_count = torch.zeros(n, dtype=torch.int64, **z)
+        self.step_count = torch.zeros(n, dtype=torch.int64, device=dev)
         self._coef = torch.empty(n, 2, **z)
         self._device = self.params[0].get_device()
         self._shapes = [p.shape for p in self.params]

@@ -289,6 +289,29 @@ def test_checkpoints_of_other_parameter_lists_are_refused(on_cpu, bits):
         assert all((t.view(torch.uint8) == 17).all() for t in twin.state.values())
 
 
+@pytest.mark.parametrize("default", [torch.float64, torch.bfloat16])
+def test_buffers_are_fp32_whatever_the_default_type(on_cpu, default):
+    """The kernels read and write the states and coefficients as fp32: in half the bytes they would leave them."""
+    import noise_amd as na
+    t, g, x = torch.zeros(2, 3, 2, 8), torch.zeros(2), torch.zeros(3, 8)
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        for bits in (32, 8):
+            opt = na.MultiTensorAdamW([torch.nn.Parameter(torch.zeros(300, dtype=torch.float32))], state_bits=bits)
+            assert opt._coef.dtype == torch.float32 and opt.step_count.dtype == torch.int64
+            for k, v in opt.state.items():
+                assert v.dtype == (torch.float8_e4m3fn if bits == 8 and not k.endswith("scale") else torch.float32), k
+        for n in (0, 3):
+            a = t[:, :n]
+            assert na.decay_attention_fwd(a, a, a, g)[1].dtype == na.decay_attention_bwd(a, a, a, a, g)[3].dtype == torch.float32
+            y = na.layer_norm_fwd(x[:n], x[0], x[1])
+            assert [s.dtype for s in y] == [torch.float32] * 3
+            assert [s.dtype for s in na.layer_norm_bwd(x[:n], x[:n], y[1], y[2])] == [torch.float32] * 3
+    finally:
+        torch.set_default_dtype(before)
+
+
 def test_no_tokens_return_a_packed_state(on_cpu):
     """The state behind no token is a new packed tensor, ready for single tokens, whatever the strides of the one given."""
     import noise_amd as na
