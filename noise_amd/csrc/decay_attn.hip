@@ -856,6 +856,7 @@ int walk_nseg(int B, int T, int H, int dk, int dv, int dtype, int backward) {
 
 const char* walk_check(int B, int T, int H, int dk, int dv, int dtype) {
   if (B < 1 || T < 1 || H < 1) return "empty shape";
+  if (T > 1 << 30) return "more than 2^30 tokens";   // the token numbers of a segment's last chunk stay below 2^31
   if (dk < 1 || dk > 128 || dv < 1 || dv > 128) return "head sizes are 1..128";
   if ((long)B * H > (1L << 22)) return "more than 2^22 (clip, head) pairs in one call";   // a grid holds at most 2^32 threads
   if (dtype < NOISE_F32 || dtype > NOISE_F16) return "unknown element type";

@@ -38,6 +38,7 @@ _lib.register({
 _lib.lib.noise_decay_attn_workspace.restype = _L
 
 MAX_HEAD = 128
+MAX_TOKENS, MAX_PAIRS = 1 << 30, 1 << 22      # of clips; single tokens take twice the pairs
 
 
 def _unit(t):
@@ -68,6 +69,8 @@ def _check(q, k, v, log_decay, state, tokens):
     if q.dtype not in _lib.DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError(f"q, k, v must share one of float32, bfloat16, float16: got {q.dtype}, {k.dtype}, {v.dtype}")
     B, H, dk, dv = qs[0], qs[-2], qs[-1], vs[-1]
+    if B * H > (MAX_PAIRS if tokens else 2 * MAX_PAIRS) or tokens and qs[1] > MAX_TOKENS:      # sizes travel as 32-bit numbers
+        raise ValueError(f"too many tokens or (clip, head) pairs for one call: {tuple(qs)}")
     if not (1 <= dk <= MAX_HEAD and 1 <= dv <= MAX_HEAD):
         raise ValueError(f"head sizes of 1 to {MAX_HEAD} are supported, got {dk} and {dv}")
     if log_decay.shape != (H,) or log_decay.dtype != torch.float32:

@@ -43,6 +43,8 @@ def _check(x, weight, bias):
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"layer_norm needs at least one value per row, got {tuple(x.shape)}")
     D = x.shape[-1]
+    if D > 1 << 24 or x.numel() // D >= 1 << 31:      # the width travels as a 32-bit number
+        raise ValueError(f"layer_norm takes rows of at most 2^24 values and fewer than 2^31 of them, got {tuple(x.shape)}")
     wdtype = None
     for name, p in (("weight", weight), ("bias", bias)):
         if p is None:

@@ -321,3 +321,35 @@ def test_no_tokens_return_a_packed_state(on_cpu):
     assert end.is_contiguous() and torch.equal(end, state) and end.data_ptr() != state.data_ptr()
     na.decay_attention_step(t.new_zeros(2, 3, 8), t.new_zeros(2, 3, 8), t.new_zeros(2, 3, 8), g, end)
     assert not na.decay_attention_fwd(t, t, t, g)[1].any()
+
+
+def test_sizes_beyond_the_entry_points_numbers_are_refused(on_cpu):
+    """A size that 32 bits cannot carry would arrive as another one; views of one value stand for the large tensors."""
+    import noise_amd as na
+    from noise_amd import _lib
+    z = torch.zeros(())
+    for shape in ((1, 2 ** 30 + 1, 1, 1), (1, 2 ** 32 + 5, 1, 1), (2 ** 22 + 1, 1, 1, 1), (2 ** 32 + 2, 1, 1, 1), (1, 1, 2 ** 32 + 1, 1)):
+        t = z.expand(shape)
+        with pytest.raises(ValueError, match="too many"):
+            na.decay_attention_fwd(t, t, t, z.expand(shape[2]))
+        with pytest.raises(ValueError, match="too many"):
+            na.decay_attention_bwd(t, t, t, t, z.expand(shape[2]))
+    for shape in ((2 ** 23 + 1, 1, 1), (2 ** 32 + 1, 1, 1), (1, 2 ** 32 + 3, 1)):
+        t = z.expand(shape)
+        with pytest.raises(ValueError, match="too many"):
+            na.decay_attention_step(t, t, t, z.expand(shape[1]), z.expand(*shape, 1))
+    for shape in ((2, 2 ** 24 + 1), (1, 2 ** 32 + 8), (2 ** 31, 4)):
+        t = z.expand(shape)
+        with pytest.raises(ValueError, match="rows of at most"):
+            na.layer_norm_fwd(t)
+        with pytest.raises(ValueError, match="rows of at most"):
+            na.layer_norm_bwd(t, t, z.expand(shape[:-1]), z.expand(shape[:-1]))
+    assert not on_cpu
+    import array
+    st = array.array("l", [1 << 31, 8, 8] * 7)
+    one, sp = ctypes.c_void_p(16), ctypes.c_void_p(st.buffer_info()[0])
+    assert _lib.lib.noise_decay_attn_workspace(1, (1 << 30) + 1, 1, 8, 8, 0, 0) == 0
+    assert _lib.lib.noise_decay_attn_workspace(1, 1 << 30, 1, 8, 8, 0, 0) > 0
+    with pytest.raises(RuntimeError, match="2.30 tokens"):
+        rc = _lib.lib.noise_decay_attn_fwd(one, one, one, one, sp, one, None, None, None, None, 1.0, 1, (1 << 30) + 1, 1, 8, 8, 0, None)
+        raise RuntimeError(f"{rc} {_lib.lib.noise_last_error().decode()}")
