@@ -408,7 +408,8 @@ int noise_decay_attn_bwd(const void* go, const void* q, const void* k, const voi
                          const long* strides, const float* log_decay, const int* lengths, const float* state, const float* d_end,
                          float* d_state, float* workspace, float scale, int B, int T, int H, int dk, int dv, int dtype,
                          void* stream);
-/* one token per clip: state [B][H][dk][dv] updated in place, o [B][H][dv]; strides: (clip, head) of q, k, v on the HOST */
+/* one token per clip: state [B][H][dk][dv] updated in place, o [B][H][dv]; strides: (clip, head) of q, k, v on the HOST.
+ * o may be q, k or v itself when that is packed, and shares no other memory with them or with the state */
 int noise_decay_attn_step(const void* q, const void* k, const void* v, const long* strides, const float* log_decay, float* state,
                           void* o, float scale, int B, int H, int dk, int dv, int dtype, void* stream);
 

@@ -958,6 +958,19 @@ NOISE_EXPORT int noise_decay_attn_step(const void* q, const void* k, const void*
   NOISE_REQUIRE(B > 0 && H > 0 && dk > 0 && dk <= 128 && dv > 0 && dv <= 128 && (long)B * H <= (1L << 23),
                 "noise_decay_attn_step: head sizes are 1..128 and at most 2^23 (stream, head) pairs (B %d, H %d, %d and %d)", B, H, dk, dv);
   NOISE_REQUIRE(dtype >= NOISE_F32 && dtype <= NOISE_F16, "noise_decay_attn_step: unknown element type");
+  // o may be q, k or v itself, packed (a workgroup reads its rows before it writes them), but no other part of what is read
+  const int es = dtype == NOISE_F32 ? 4 : 2;
+  const char *o0 = (const char*)o, *o1 = o0 + (size_t)B * H * dv * es, *s0 = (const char*)state;
+  bool meets = o0 < s0 + (size_t)B * H * dk * dv * 4 && s0 < o1;
+  const void* in[3] = {q, k, v};
+  for (int i = 0; i < 3; ++i) {
+    const long sb = B > 1 ? strides[2 * i] : 0, sh = H > 1 ? strides[2 * i + 1] : 0;
+    const int width = i < 2 ? dk : dv;
+    const char *t0 = (const char*)in[i], *t1 = t0 + ((B - 1) * sb + (H - 1) * sh + width) * es;
+    const bool same = t0 == o0 && width == dv && (H == 1 || sh == dv) && (B == 1 || sb == (long)H * dv);
+    meets = meets || (!same && o0 < t1 && t0 < o1);
+  }
+  NOISE_REQUIRE(!meets, "noise_decay_attn_step: o shares memory with the state or with a part of q, k or v");
   const Strides sq = {strides[0], 0, strides[1]}, sk = {strides[2], 0, strides[3]}, sv = {strides[4], 0, strides[5]};
   const bool vec = dv % 4 == 0 && ((uintptr_t)state & 15) == 0;
   hipStream_t st = (hipStream_t)stream;

@@ -177,7 +177,7 @@ def decay_attention(q, k, v, log_decay, state=None, lengths=None, scale=None):
 
 def decay_attention_step(q, k, v, log_decay, state, scale=None, out=None):
     """One token per stream: q, k (B, H, Dk), v (B, H, Dv); `state` (B, H, Dk, Dv) fp32, packed, is updated in place.  Returns
-    o (B, H, Dv) (`out` when given).  No gradient."""
+    o (B, H, Dv) (`out` when given; it may be q, k or v, but no other part of an argument).  No gradient."""
     if state is None:
         raise ValueError("decay_attention_step needs the streams' state")
     B, H, dk, dv = _check(q, k, v, log_decay, state, False)

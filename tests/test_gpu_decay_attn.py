@@ -374,3 +374,21 @@ def test_lengths_outside_of_the_clip(T):
         c["lengths"] = lengths.to(DEV)
         got = run_all(c)
         assert all(torch.equal(want[n], got[n]) for n in want)
+
+
+def test_step_into_its_own_arguments():
+    """out over q, k or v row for row gives the same numbers; over the state it is refused and the state stays."""
+    import noise_amd as na
+    c = make(5, 1, 3, 16, 16, torch.bfloat16, 2)
+    one = [c[n][:, 0].contiguous() for n in "qkv"]
+    state = c["state"].clone()
+    want = na.decay_attention_step(*one, c["log_decay"], state)
+    for i in range(3):
+        again, s = [t.clone() for t in one], c["state"].clone()
+        assert na.decay_attention_step(*again, c["log_decay"], s, out=again[i]) is again[i]
+        assert torch.equal(again[i], want) and torch.equal(s, state)
+    f = [t.float() for t in one]
+    s = c["state"].clone()
+    with pytest.raises(RuntimeError, match="shares memory"):
+        na.decay_attention_step(*f, c["log_decay"], s, out=s.view(-1)[:5 * 3 * 16].view(5, 3, 16))
+    assert torch.equal(s, c["state"])

@@ -353,3 +353,34 @@ def test_sizes_beyond_the_entry_points_numbers_are_refused(on_cpu):
     with pytest.raises(RuntimeError, match="2.30 tokens"):
         rc = _lib.lib.noise_decay_attn_fwd(one, one, one, one, sp, one, None, None, None, None, 1.0, 1, (1 << 30) + 1, 1, 8, 8, 0, None)
         raise RuntimeError(f"{rc} {_lib.lib.noise_last_error().decode()}")
+
+
+def test_step_output_over_other_arguments():
+    """o may be q, k or v itself, row for row, but no part of the state nor a shifted piece of another argument.  What is allowed
+    gets as far as the launch, which needs a GPU; nothing is launched here."""
+    import array
+    from noise_amd import _lib
+    if torch.cuda.is_available():
+        pytest.skip("addresses of no memory: for machines without a GPU")
+    B, H, D = 2, 3, 8
+    row, q, k, v, state = 4 * B * H * D, 1 << 20, 2 << 20, 3 << 20, 4 << 20
+
+    def step(o, q=q, k=k, v=v, strides=(H * D, D) * 3, dk=D, B=B):
+        st = array.array("l", strides)
+        a = [ctypes.c_void_p(x) for x in (q, k, v, st.buffer_info()[0], 16, state, o)]
+        _lib.call("noise_decay_attn_step", *a, 1.0, B, H, dk, D, 0, None)
+    for o in (q, k, v, v + row, v - row, state - row, state + D * row):
+        with pytest.raises(RuntimeError, match="no ROCm-capable device"):
+            step(o)
+    for o in (state, state + D * row - row, state + D * row - 4, state - 4, q + 4, k - 4, v + row - 4):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            step(o)
+    wide = (2 * H * D, 2 * D) + (H * D, D) * 2      # q with gaps: its rows go on behind a packed one's end
+    for o in (q, q + row):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            step(o, strides=wide)
+    with pytest.raises(RuntimeError, match="shares memory"):
+        step(q, dk=D - 1)
+    for strides in ((5, D, 7, D, 9, D), (0, D) * 3):      # one stream: its stride says nothing
+        with pytest.raises(RuntimeError, match="no ROCm-capable device"):
+            step(q, strides=strides, B=1)
