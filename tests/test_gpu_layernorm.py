@@ -206,3 +206,62 @@ def test_other_stream_and_captured_graph():
         eb = na.layer_norm_bwd(sdy, sx, ef[1], ef[2], w)
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(ef + eb, f + bw))
+
+
+# Sizes at which a lane group works on more than one row: forward two rows from 4096 groups on, backward the grid's stride from
+# 512 workgroups on (1024 / 256 for rows of a whole workgroup), each with a remainder; every group width, whole 16-byte pieces and
+# single values, and rows too wide for registers.  (rows, width, type)
+LOOPS = [(65537, 64, torch.float32), (65553, 60, torch.bfloat16), (32777, 128, torch.float32), (32771, 200, torch.bfloat16),
+         (16391, 256, torch.float32), (16385, 512, torch.float32), (16387, 1000, torch.float32), (16389, 1016, torch.float16),
+         (4099, 2048, torch.float32), (4101, 8192, torch.bfloat16), (4097, 6000, torch.float32), (4100, 16384, torch.float16),
+         (65539, 15, torch.bfloat16), (32769, 31, torch.float32), (16389, 63, torch.float16), (16393, 127, torch.float32),
+         (16387, 255, torch.bfloat16), (4103, 511, torch.float32), (4099, 1023, torch.float16), (4101, 2047, torch.bfloat16),
+         (201, 16392, torch.bfloat16), (333, 2051, torch.float32), (131, 8204, torch.float32)]
+
+
+@pytest.mark.parametrize("rows,D,dtype", LOOPS)
+def test_many_rows_per_group(rows, D, dtype):
+    """The sums of a lane run over at most rows / 64 + 32 terms, which check_bwd counts."""
+    import noise_amd as na
+    x, dy, w, b = case(rows, D, dtype, torch.float32, rows + D)
+    y, mean, rstd = na.layer_norm_fwd(x, w, b, 1e-6)
+    check_fwd(x, w, b, y, mean, rstd, 1e-6)
+    got = na.layer_norm_bwd(dy, x, mean, rstd, w)
+    check_bwd(dy, x, mean, rstd, w, *got)
+    again = na.layer_norm_bwd(dy, x, mean, rstd, w)
+    assert all(torch.equal(p, q) for p, q in zip(got, again))
+    # the same rows through views that allow no 16-byte accesses
+    wide = torch.zeros(rows, D + 1, device=DEV, dtype=dtype)
+    wide[:, 1:] = x
+    v = wide[:, 1:]
+    y2, mean2, rstd2 = na.layer_norm_fwd(v, w, b, 1e-6)
+    check_fwd(v, w, b, y2, mean2, rstd2, 1e-6)
+    check_bwd(dy, v, mean, rstd, w, *na.layer_norm_bwd(dy, v, mean, rstd, w))
+
+
+# Results of 128 MB and more go past the caches, in every group width
+@pytest.mark.parametrize("rows,D,dtype", [(524801, 64, torch.float32), (262401, 128, torch.float32), (262147, 256, torch.bfloat16), (65541, 520, torch.float32),
+                                          (70001, 1000, torch.bfloat16), (16400, 4096, torch.float16), (8209, 8192, torch.bfloat16),
+                                          (4100, 16384, torch.bfloat16)])
+def test_results_past_the_caches(rows, D, dtype):
+    import noise_amd as na
+    assert rows * D * dtype.itemsize >= 1 << 27
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    x, dy = ((torch.randn(rows, D, generator=g, device=DEV) * 1.7 + 0.6).to(dtype) for _ in range(2))
+    w, b = (torch.randn(D, generator=g, device=DEV) for _ in range(2))
+    y, mean, rstd = na.layer_norm_fwd(x, w, b, 1e-6)
+    check_fwd(x, w, b, y, mean, rstd, 1e-6)
+    got = na.layer_norm_bwd(dy, x, mean, rstd, w)
+    check_bwd(dy, x, mean, rstd, w, *got)
+
+
+def test_more_rows_than_one_launch_covers():
+    """2^23 rows are one launch's limit."""
+    import noise_amd as na
+    rows, D = (1 << 23) + 5, 3
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x, dy = (torch.randn(rows, D, generator=g, device=DEV) for _ in range(2))
+    w, b = (torch.randn(D, generator=g, device=DEV) for _ in range(2))
+    y, mean, rstd = na.layer_norm_fwd(x, w, b)
+    check_fwd(x, w, b, y, mean, rstd, 1e-6)
+    check_bwd(dy, x, mean, rstd, w, *na.layer_norm_bwd(dy, x, mean, rstd, w))
