@@ -312,3 +312,63 @@ def test_captured_step_replays(bits):
         b.step(grads=grads)
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(params, twin)) and (a.step_count == k + 1).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_tensors_than_one_mask_holds(bits):
+    """4096 tensors are what one launch of the step counter covers; a list beyond that, whole and with gaps."""
+    import noise_amd as na
+    n = 4300
+    g = torch.Generator().manual_seed(2)
+    base, grad = torch.randn(n, 4, generator=g).to(DEV), torch.randn(n, 4, generator=g).to(DEV)
+    params = [torch.nn.Parameter(base[i, :1 + i % 3].clone()) for i in range(n)]
+    opt = na.MultiTensorAdamW(params, lr=1e-2, state_bits=bits)
+    rules = [Rule(p, bits) for p in params]
+    for step, gap in enumerate((0, 7)):
+        grads = [None if gap and i % gap == 3 else grad[i, :1 + i % 3] for i in range(n)]
+        opt.step(grads=grads)
+        now = [p.detach().cpu() for p in params]
+        for i, gr in enumerate(grads):
+            if gr is not None:
+                close_p(now[i], rules[i], rules[i].step(gr, 1e-2, 0.9, 0.999, 1e-8, 1e-2), 1)
+                rules[i].p = now[i].double()
+            else:
+                assert torch.equal(now[i].double(), rules[i].p)
+    want = torch.tensor([1 if i % 7 == 3 else 2 for i in range(n)])
+    assert torch.equal(opt.step_count.cpu(), want)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_waveform_model_trains_with_it(bits):
+    """Steps of the waveform-domain U-Net: its separate gradients go in, the rule holds for every parameter, and the next
+    step runs on the new weights (a second model given them computes the same loss and gradients)."""
+    import copy
+    import noise_amd as na
+    import test_gpu_wave as W
+    x1, clean = (torch.from_numpy(W.G9[f"narrow_{k}"]).to(DEV) for k in ("x1", "val_clean"))
+    m = W.build("narrow", linear_gain=1.0).to(DEV).eval()
+    m(x1)
+    m.train()
+    m.attn_keep_masks = W.g10_masks("narrow", 2)
+    opt = na.MultiTensorAdamW(m.parameters(), lr=1e-3, state_bits=bits)
+    rules = [Rule(p.detach().view(-1), bits) for p in m.parameters()]
+    for step in range(3):
+        opt.zero_grad()
+        loss = m.training_step((x1, clean, None), 0)
+        loss.backward()
+        if step:
+            fresh = W.build("narrow", linear_gain=1.0).to(DEV).eval()
+            fresh(x1)
+            fresh.load_state_dict(before)
+            fresh.train()
+            fresh.attn_keep_masks = W.g10_masks("narrow", 2)
+            other = fresh.training_step((x1, clean, None), 0)
+            other.backward()
+            assert torch.equal(loss, other)
+            assert all(torch.equal(p.grad, q.grad) for p, q in zip(m.parameters(), fresh.parameters()))
+        opt.step()
+        before = copy.deepcopy(m.state_dict())
+        for p, r in zip(m.parameters(), rules):
+            close_p(p.detach().view(-1), r, r.step(p.grad.reshape(-1), 1e-3, 0.9, 0.999, 1e-8, 1e-2), 1)
+            r.p = p.detach().view(-1).double().cpu()
+    assert (opt.step_count == 3).all()
