@@ -392,3 +392,34 @@ def test_step_into_its_own_arguments():
     with pytest.raises(RuntimeError, match="shares memory"):
         na.decay_attention_step(*f, c["log_decay"], s, out=s.view(-1)[:5 * 3 * 16].view(5, 3, 16))
     assert torch.equal(s, c["state"])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,T,D", [(3, 77, 20), (2, 129, 24), (1, 700, 64), (2, 90, 128)])
+def test_layouts_of_every_type(B, T, D, dtype):
+    """Layouts that are read in place, and those that are copied first (a broadcast token axis, overlapping windows, a last axis
+    with a stride): the numbers of packed copies, forwards and backwards."""
+    import noise_amd as na
+    g = torch.Generator().manual_seed(T)
+    H = 3
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype).to(DEV)
+    decay = torch.tensor([-0.1, -0.01, 0.0], device=DEV)
+    big, line = r(B, T, H, 3 * D + 1), r(B, H, 3, T + D)
+    layouts = [[big[..., 1 + i * D:1 + (i + 1) * D] for i in range(3)],               # rows off any 16-byte border
+               [big[..., i * D:(i + 1) * D] for i in range(3)],
+               r(3, B, H, T, D).transpose(2, 3).unbind(0),                             # heads outside of tokens
+               r(3, B, T, H, D, 2)[..., 1].unbind(0),                                  # a strided last axis
+               r(3, 1, T, H, D).expand(3, B, T, H, D).unbind(0),                       # one clip for all
+               r(3, B, T, 1, D).expand(3, B, T, H, D).unbind(0),                       # one head for all
+               r(3, B, 1, H, D).expand(3, B, T, H, D).unbind(0),                       # one token for all: copied
+               line.unfold(-1, D, 1)[..., :T, :].permute(2, 0, 3, 1, 4).unbind(0),     # windows that overlap: copied
+               r(3, B, 2 * T, H, D)[:, :, ::2].unbind(0)]
+    state = torch.randn(B, H, D, D, generator=g).to(DEV)
+    for q, k, v in layouts:
+        assert q.shape == k.shape == v.shape == (B, T, H, D)
+        packed = [t.contiguous() for t in (q, k, v)]
+        a, b = (na.decay_attention_fwd(*t, decay, state) for t in ((q, k, v), packed))
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+        a = na.decay_attention_bwd(k, q, k, v, decay, state)
+        b = na.decay_attention_bwd(packed[1], *packed, decay, state)
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
