@@ -300,7 +300,8 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, 2) void walk_f32_kernel(Walk
 //     carried over any number of chunks and returned: X keeps fp32 accuracy at three products per term.
 // fp16 has the fraction for that but not the range, so those three operands go in scaled by powers of two that bounds give
 // (dk max|a| max|k| for the weights, max|v| for the split values, and for the state the recurrence of the bound itself); X is
-// kept in the units of the last chunk's values.  The bounds may be far too large: fp16 stays normal over 2^29.
+// kept in the units of the last chunk's values, or in those in which it stays finite.  The bounds may be far too large: fp16
+// stays normal over 2^29.
 // Operands: lane (q = lane / 16, l = lane % 16) of an MFMA takes eight contraction indices 8q..8q+7 of row l, and an
 // accumulator tile holds rows 4q + r of column l.  Two state tiles whose rows are dealt as 8q + 4s + r (s = tile) together
 // are the eight indices the next product wants, so the state stays in registers.  Contractions over tokens read K and V
@@ -361,8 +362,8 @@ __device__ __forceinline__ f32x4 mfma16(x8<f16_t> a, x8<f16_t> b, f32x4 c) { ret
 // Largest magnitude among the fp16 values of a register, as bits (their order is the integers').
 __device__ __forceinline__ u16x2 abs_max16(u16x2 m, unsigned u) { return __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, u & 0x7fff7fffu)); }
 __device__ __forceinline__ float pow2(int e) { return ldexpf(1.f, e); }
-// The exponent that brings a bound below 2^top; a bound of zero, infinity or NaN gives a harmless one.
-__device__ __forceinline__ int scale_for(float bound, int top) { return max(min(top - __builtin_amdgcn_frexp_expf(bound), 60), -60); }
+// The exponent that brings a bound below 2^top, at most 60; a bound of zero, infinity or NaN gives a harmless one.
+__device__ __forceinline__ int scale_for(float bound, int top) { return min(top - __builtin_amdgcn_frexp_expf(bound), 60); }
 
 // VEC: rows of a, k, v and o allow 16-byte accesses.
 template <typename T, int P, int CC, bool STATE_ONLY, bool VEC>
@@ -522,15 +523,18 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
         for (int i = 0; i < NW; ++i) u = max(u, STATE_ONLY && z == 0 ? 0u : top[z * NW + i]);
         big[z] = (float)__builtin_bit_cast(f16_t, (unsigned short)u);
       }
-      const int ep = scale_for((float)P * fabsf(s_o * w.s_kv) * big[0] * big[1], 15), ev = scale_for(fabsf(w.s_kv) * big[2], 15);
+      largest = fabsf(w.s_kv) * big[1] * big[2] * (float)n;
+      // a state near fp32's end takes the exponents down, so that X 2^ev and the units of X's product stay finite: for |X| up to
+      // 2^e the split values lose what lies below 2^(e - 150) and the weights what lies below 2^(e - 165)
       const int ex = scale_for(bound, 14);
+      const int ep = min(scale_for((float)P * fabsf(s_o * w.s_kv) * big[0] * big[1], 15), 126 + ex);
+      const int ev = min(scale_for(fabsf(w.s_kv) * big[2], 15), 126 - __builtin_amdgcn_frexp_expf(fminf(bound + largest, 3e38f)));
       unit_p = pow2(ep);                // weights
       unit_x = pow2(ex - E);            // X as an operand
       back = pow2(ep - ex);             // its product, in the weights' units
       unit_v = pow2(ev);                // values on their way into X
       carry = pow2(ev - E);
       E = ev;
-      largest = fabsf(w.s_kv) * big[1] * big[2] * (float)n;
     }
     f32x4 O[STATE_ONLY ? 1 : NI];
     if (!STATE_ONLY) {
@@ -585,7 +589,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
     // ---- X = lam^n X + K^T V'
     x8<T> v[C / 32];
     const float f = pw[n - shift] * carry;
-    if constexpr (F16) bound = bound * pw[n - shift] + largest;
+    if constexpr (F16) bound = fminf(bound * pw[n - shift] + largest, 3e38f);
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp)
 #pragma unroll

@@ -423,3 +423,38 @@ def test_layouts_of_every_type(B, T, D, dtype):
         a = na.decay_attention_bwd(k, q, k, v, decay, state)
         b = na.decay_attention_bwd(packed[1], *packed, decay, state)
         assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("e,v", [(64, 0), (70, -14), (75, 0), (90, -10), (110, 0), (118, -14), (123, 5)])
+@pytest.mark.parametrize("T", [130, 900])
+def test_states_up_to_the_end_of_fp32(T, e, v, dtype):
+    """States and their gradients of 2^e beside ordinary and small tokens: what fp32 can hold stays finite, whatever units the
+    fp16 kernel carries the state in.  Results beyond their type's range are left out; e = 123 leaves room for four sigma."""
+    c = make(1, T, 3, 32, 24, dtype, e + T)
+    c["log_decay"] = torch.tensor([-3.0, -0.4, 0.0], device=DEV)
+    c["v"] = (c["v"].double() * 2.0 ** v).to(dtype)
+    c["do"] = (c["do"].double() * 2.0 ** v).to(dtype)
+    c["state"], c["d_state"] = (c[n].clamp(-4, 4) * 2.0 ** e for n in ("state", "d_state"))
+    got = run_all(c)
+    want, mag = recurrence(c, 32 ** -0.5), recurrence(c, 32 ** -0.5, True)
+    top = torch.finfo(dtype).max
+    for name, g in got.items():
+        if name in ("o", "dq", "dk", "dv"):
+            # a product of 16-bit rounded weights and states can leave the type's range where its magnitude sum does
+            fits = mag[name] < 0.9 * top
+            if dtype != torch.float16:
+                # the product of a row with the state before its chunk of up to 64 tokens is formed in fp32 without its scale and
+                # decay, and has to fit itself: elements of at most 4 2^e, decayed up to that chunk, plus what the tokens add
+                row = c[{"o": "q", "dq": "do", "dk": "v", "dv": "k"}[name]].double().abs().sum(-1, keepdim=True)
+                t = torch.arange(T, device=DEV) if name in ("o", "dq") else torch.arange(T, device=DEV).flip(0)
+                lam = torch.exp(c["log_decay"].double().view(1, 3) * (t - 64).clamp_min(0).view(T, 1)).view(1, T, 3, 1)
+                fits &= row * (4 * 2.0 ** e * lam + 2.0 ** 40) < 0.9 * torch.finfo(torch.float32).max
+        else:
+            fits = torch.ones_like(g, dtype=torch.bool)
+            assert torch.isfinite(g).all(), name
+        # a decay over d tokens is 2^(g2 d), g2 = g log2(e): log2(e), g2 and the product are rounded, 3 U of an exponent of |g| d
+        # (in units of e), so 3 U |g| d of the power.  With states this large a power counts that would vanish otherwise
+        g3 = 3 * c["log_decay"].double().abs() * T * U
+        t = tolerance(name, want[name], mag[name], dtype, T, 32, 24) + mag[name] * (g3.view(3, 1) if g.shape[1] == T else g3.view(3, 1, 1))
+        assert fits.any() and ((g.double() - want[name]).abs() <= t)[fits].all(), (name, ((g.double() - want[name]).abs() / t)[fits].max())
