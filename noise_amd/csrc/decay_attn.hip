@@ -63,6 +63,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t chunk_rows(const void* first, 
 // A byte offset into such a buffer; one before its start, or of a column that does not exist, lands far behind its end.
 __device__ __forceinline__ int chunk_offset(int off, bool exists) { return (int)min((unsigned)(exists ? off : -1), 0x80000000u); }
 
+// A v that is not finite may reach no earlier token: its weight there is zero, but zero times it is not.  Such rows are rare, so
+// they cost the walk a test as they come in, and where a chunk holds one behind its first token it ends before it.  The first
+// of them goes through LDS (`cut`, one per chunk in flight); CUT_NONE: there is none.
+constexpr int CUT_NONE = 1 << 30;
+
 // fp32 arithmetic throughout (v_mfma_f32_16x16x4_f32).  P: dk and dv padded to 16, 32, 64 or 128; P / 16 waves up to four,
 // each owning 16 NT of the P state columns.  The contraction index of an MFMA may be permuted as long as both operands agree:
 // lane quarter q takes elements 4q..4q+3 of a 16-wide block over four consecutive instructions, so row-major operands are
@@ -81,6 +86,7 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, 2) void walk_f32_kernel(Walk
   __shared__ float pw[DA_C + 1];                             // lam^i
   __shared__ float pv[2 * DA_C];                             // s_kv lam^{31-i}; a chunk of n tokens starts at 32 - n
   __shared__ float pp[DA_C + 16];                            // [15 + i - j]: s_o s_kv lam^{i-j}
+  __shared__ int cut[2];
   const int tid = threadIdx.x, wave = NW == 1 ? 0 : tid >> 6, lane = tid & 63, q = lane >> 4, l16 = lane & 15;
   const int bh = blockIdx.x % (w.B * w.H), seg = blockIdx.x / (w.B * w.H);
   const int b = bh / w.H, h = bh % w.H;
@@ -153,24 +159,50 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, 2) void walk_f32_kernel(Walk
     rows4(kb, sk_t, dk, c0, rk);
     rows4(vb, sv_t, dv, c0, rv);
   };
+  // returns the first row behind the chunk's first whose v is not finite, among this thread's
   auto put = [&]() {
+    int bad = CUT_NONE;
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
       const int at = (i0 + s * RS) * LD + cc;
       if constexpr (!STATE_ONLY) *(f32x4*)(sa + at) = ra[s];
       *(f32x4*)(sk + at) = rk[s];
       *(f32x4*)(sv + at) = rv[s];
+      if constexpr (!STATE_ONLY) {
+        float z = 0.f;                                      // stays zero over finite values
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z = __builtin_fmaf(rv[s][e], 0.f, z);
+        const int row = i0 + s * RS;
+        bad = z != 0.f && row > 0 ? min(bad, row) : bad;
+      }
     }
+    return bad;
   };
   if (p0 < p1) {
+    if (!STATE_ONLY && tid < 2) cut[tid] = CUT_NONE;
     fetch(p0);
-    put();
+    const int bad = put();
+    if constexpr (!STATE_ONLY) {
+      __syncthreads();
+      if (bad < CUT_NONE) atomicMin(&cut[0], bad);
+    }
   }
-  for (int c0 = p0; c0 < p1; c0 += DA_C) {
-    const int n = min(DA_C, p1 - c0);                       // tokens in this chunk
+  int turn = 0;
+  for (int c0 = p0, n; c0 < p1; c0 += n, turn ^= 1) {
+    n = min(DA_C, p1 - c0);                                 // tokens in this chunk
     const int shift = w.shift && c0 == 0 ? 1 : 0;
     __syncthreads();
+    const int first_bad = STATE_ONLY ? CUT_NONE : cut[turn];
     fetch(c0 + DA_C);                                       // behind the last chunk: zeros, without an access
+    if constexpr (!STATE_ONLY) {
+      if (__builtin_amdgcn_readfirstlane(first_bad) < CUT_NONE) {
+        n = __builtin_amdgcn_readfirstlane(first_bad);
+        for (int i = n * LD + tid; i < DA_C * LD; i += NTHR) sk[i] = sv[i] = 0.f;
+        fetch(c0 + n);
+        __syncthreads();
+        if (tid == 0) cut[turn] = CUT_NONE;                 // read by all; next written behind the next barrier
+      }
+    }
     f32x4 O[2][NT];
     if (!STATE_ONLY) {
       // ---- weights lam^{i-j} (a_i . k_j), transposed: a lane holds four neighbouring j of one i.  One 16 x 16 tile per wave and
@@ -258,7 +290,7 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, 2) void walk_f32_kernel(Walk
     }
     // the next tiles go in before this chunk's rows go out: waiting for loads that are older than a store is not waiting for the
     // store (memory operations are counted in order)
-    put();
+    const int bad = put();
     if (!STATE_ONLY) {
       const auto rs = chunk_rows(ob + (reverse ? len - c0 - n : c0) * (long)so_t, n, so_t, dv, 4);
 #pragma unroll
@@ -276,6 +308,7 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, 2) void walk_f32_kernel(Walk
           }
         }
       }
+      if (bad < CUT_NONE) atomicMin(&cut[turn ^ 1], bad);
     }
   }
   // ---- state behind the segment
@@ -379,7 +412,8 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
   __shared__ float pw[C + 1];                             // lam^i
   __shared__ float pv[2 * C];                             // s_kv lam^{63-i}; a chunk of n tokens starts at 64 - n
   __shared__ float pp[C + 16];                            // [15 + i - j]: s_o s_kv lam^{i-j}
-  __shared__ unsigned top[F16 ? 3 * NW : 1];                 // largest a, k, v of the waves' pieces, as bits
+  __shared__ unsigned top[F16 ? 3 * NW : 1];                 // largest finite a, k, v of the waves' pieces, as bits
+  __shared__ int cut[2];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, q = lane >> 4, l16 = lane & 15;
   const int bh = blockIdx.x % (w.B * w.H), seg = blockIdx.x / (w.B * w.H);
   const int b = bh / w.H, h = bh % w.H;
@@ -439,7 +473,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) bound = fmaxf(bound, fabsf(X[kp][s][r]));
+        for (int r = 0; r < 4; ++r) bound = fmaxf(bound, fabsf(X[kp][s][r]) < INFINITY ? fabsf(X[kp][s][r]) : 0.f);
     bound = wave_reduce_max(bound);
   }
 
@@ -475,7 +509,10 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
     rows8(kb, sk_t, dk, w.vk, c0, rk);
     rows8(vb, sv_t, dv, w.vv, c0, rv);
   };
+  // returns the first row behind the chunk's first whose v is not finite, among this thread's
   auto put = [&]() {
+    int bad = CUT_NONE;
+    u16x2 m[3] = {};                                        // largest a, k, v
 #pragma unroll
     for (int s = 0; s < SLOTS; ++s) {
       const int at = (i0 + s * RS) * LD + cc;
@@ -484,35 +521,64 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
       *(uint2*)kd = make_uint2(rk[s][0], rk[s][1]);
       *(uint2*)(kd + 16) = make_uint2(rk[s][2], rk[s][3]);
       *(u32x4*)(sv + at) = rv[s];
+      u16x2 mv = {};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (F16 && !STATE_ONLY) m[0] = abs_max16(m[0], ra[s][e]);
+        if constexpr (F16) m[1] = abs_max16(m[1], rk[s][e]);
+        if constexpr (F16 || !STATE_ONLY) mv = abs_max16(mv, rv[s][e]);
+      }
+      if constexpr (F16) m[2] = __builtin_elementwise_max(m[2], mv);
+      if constexpr (!STATE_ONLY) {
+        const int row = i0 + s * RS;
+        bad = max(mv[0], mv[1]) >= (F16 ? 0x7c00 : 0x7f80) && row > 0 ? min(bad, row) : bad;
+      }
     }
     if constexpr (F16) {
-      u16x2 m[3] = {};
-#pragma unroll
-      for (int s = 0; s < SLOTS; ++s)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (!STATE_ONLY) m[0] = abs_max16(m[0], ra[s][e]);
-          m[1] = abs_max16(m[1], rk[s][e]);
-          m[2] = abs_max16(m[2], rv[s][e]);
-        }
 #pragma unroll
       for (int z = STATE_ONLY ? 1 : 0; z < 3; ++z) {
         unsigned u = max(m[z][0], m[z][1]);
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) u = max(u, (unsigned)__shfl_xor((int)u, o, 64));
+        if (u >= 0x7c00) {                                  // (the whole wave) a value that is not finite says nothing about the others
+          u = 0;
+          for (int s = 0; s < SLOTS; ++s)
+            for (int e = 0; e < 8; ++e) {
+              const unsigned x = (z == 0 ? ra[STATE_ONLY ? 0 : s] : z == 1 ? rk[s] : rv[s])[e >> 1] >> (e & 1) * 16 & 0x7fff;
+              u = max(u, x < 0x7c00 ? x : 0u);
+            }
+          for (int o = 32; o > 0; o >>= 1) u = max(u, (unsigned)__shfl_xor((int)u, o, 64));
+        }
         if (lane == 0) top[z * NW + wave] = u;
       }
     }
+    return bad;
   };
   if (p0 < p1) {
+    if (!STATE_ONLY && tid < 2) cut[tid] = CUT_NONE;
     fetch(p0);
-    put();
+    const int bad = put();
+    if constexpr (!STATE_ONLY) {
+      __syncthreads();
+      if (bad < CUT_NONE) atomicMin(&cut[0], bad);
+    }
   }
-  for (int c0 = p0; c0 < p1; c0 += C) {
-    const int n = min(C, p1 - c0);                       // tokens in this chunk
+  int turn = 0;
+  for (int c0 = p0, n; c0 < p1; c0 += n, turn ^= 1) {
+    n = min(C, p1 - c0);                                 // tokens in this chunk
     const int shift = w.shift && c0 == 0 ? 1 : 0;
     __syncthreads();
+    const int first_bad = STATE_ONLY ? CUT_NONE : cut[turn];
     if (P < 128 || STATE_ONLY || c0 + C < p1) fetch(c0 + C);   // behind the last chunk: zeros, without an access
+    if constexpr (!STATE_ONLY) {
+      if (__builtin_amdgcn_readfirstlane(first_bad) < CUT_NONE) {
+        n = __builtin_amdgcn_readfirstlane(first_bad);
+        for (int i = n * LD + tid; i < C * LD; i += NTHR) sk[i] = sv[i] = (T)0.f;
+        fetch(c0 + n);
+        __syncthreads();
+        if (tid == 0) cut[turn] = CUT_NONE;                 // read by all; next written behind the next barrier
+      }
+    }
     float unit_p = 1.f, unit_x = 1.f, back = 1.f, unit_v = 1.f, carry = 1.f, largest = 0.f;
     if constexpr (F16) {
       float big[3];
@@ -638,7 +704,8 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
     }
     // the next tiles go in before this chunk's rows go out: waiting for loads that are older than a store is not waiting for the
     // store (memory operations are counted in order).  Wide heads have no registers to hold both, and other waves to run.
-    if constexpr (P < 128) put();
+    int bad = CUT_NONE;
+    if constexpr (P < 128) bad = put();
     if (!STATE_ONLY) {
       const int col = col0 + 4 * q;
       const auto rs = chunk_rows(ob + (reverse ? len - c0 - n : c0) * (long)so_t, n, so_t, dv, 2);
@@ -659,7 +726,8 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
         }
       }
     }
-    if constexpr (P == 128) put();
+    if constexpr (P == 128) bad = put();
+    if (!STATE_ONLY && bad < CUT_NONE) atomicMin(&cut[turn ^ 1], bad);
   }
   // ---- state behind the segment
   float* dst = STATE_ONLY ? w.seg + ((size_t)bh * w.nseg + seg) * mat : seg == last_seg && w.x_end ? w.x_end + (size_t)bh * mat : nullptr;

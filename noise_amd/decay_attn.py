@@ -19,8 +19,10 @@ and behind lengths[b] are neither read nor added to the state, their rows of o a
 returned is the one behind the last real token.  `scale` defaults to Dk ** -0.5.
 
 Numbers: states are carried in fp32 accuracy whatever the tokens' type; in 16-bit types the weights inside a chunk and the
-state as it meets q are rounded to the type once each, like the output.  A token that is not finite reaches, besides all later
-ones, the other tokens of its chunk of 32 or 64.
+state as it meets q are rounded to the type once each, like the output (0.0023 from the exact result in bf16, where rounding
+the exact result alone is 0.0017).  fp16 keeps that within 2^28 of the largest value that 16 neighbouring columns of a state
+may hold by its bound, the decayed sum of max |k| max |v|.  A token that is not finite reaches what the formulas say: its
+column and later tokens, or all columns where it is one of k or q; an infinity may come out as a NaN.
 """
 import ctypes
 

@@ -458,3 +458,63 @@ def test_states_up_to_the_end_of_fp32(T, e, v, dtype):
         g3 = 3 * c["log_decay"].double().abs() * T * U
         t = tolerance(name, want[name], mag[name], dtype, T, 32, 24) + mag[name] * (g3.view(3, 1) if g.shape[1] == T else g3.view(3, 1, 1))
         assert fits.any() and ((g.double() - want[name]).abs() <= t)[fits].all(), (name, ((g.double() - want[name]).abs() / t)[fits].max())
+
+
+def poison(c, places):
+    for name, b, t, h, col, value in places:
+        c[name][b, t, h, col] = value
+    return c
+
+
+def check_poisoned(c, dtype):
+    """What the definition leaves finite is finite and as exact as ever; what it does not is not."""
+    B, T, H, dk = c["q"].shape
+    dv = c["v"].shape[-1]
+    got, want, mag = run_all(c), recurrence(c, dk ** -0.5), recurrence(c, dk ** -0.5, True)
+    for name, g in got.items():
+        ok = torch.isfinite(want[name])
+        assert torch.equal(torch.isfinite(g), ok), (name, (torch.isfinite(g) != ok).nonzero()[:4])
+        t = tolerance(name, want[name], mag[name], dtype, T, dk, dv)
+        assert ((g.double() - want[name]).abs() <= t)[ok].all(), (name, ((g.double() - want[name]).abs() / t)[ok].max())
+    return got
+
+
+NAN, INF = float("nan"), float("inf")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,T,dk,dv", [(2, 7, 10, 10), (2, 150, 16, 16), (2, 130, 33, 24), (2, 200, 64, 64), (1, 1100, 64, 40), (2, 140, 128, 128),
+                                       (1, 900, 128, 100)])
+@pytest.mark.parametrize("name", ["q", "k", "v", "do"])
+def test_a_token_that_is_not_finite(name, B, T, dk, dv, dtype):
+    """One, two neighbouring, and several values of a tensor that are not finite, at the ends of chunks and inside them: neither a
+    token before it (behind it in the gradients that run backwards) nor another column feels them."""
+    n = dv if name in ("v", "do") else dk
+    for i, places in enumerate(([(T // 2, 3, NAN)], [(T - 1, 0, INF), (0, n - 1, -INF)], [(T // 3, 2, INF), (T // 3 + 1, 1, NAN), (T // 3 + 2, n - 2, INF)],
+                                [(t, (5 * t) % n, -INF) for t in (1, 31, 32, 63, 64, 65, 96, 127, 128) if t < T])):
+        c = make(B, T, 2, dk, dv, dtype, 100 * i + T + dk)
+        c["log_decay"] = torch.tensor([-0.05, 0.0], device=DEV)
+        check_poisoned(poison(c, [(name, B - 1, t, 1, col, x) for t, col, x in places]), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_poison_everywhere_and_nowhere_else(dtype):
+    """Tokens of every tensor and elements of the states at once, a clip whose tokens are all poisoned in one column, padding, and
+    layouts without 16-byte rows; clips and heads beside them keep the very bits they have without."""
+    c = make(4, 260, 3, 40, 40, dtype, 6, packed=True, ragged=True)
+    c["lengths"][:] = torch.tensor([260, 100, 177, 0])
+    c["log_decay"] = torch.tensor([-0.1, 0.0, -1.0], device=DEV)
+    clean = run_all(c)
+    poison(c, [("v", 0, t, 1, 7, NAN) for t in range(260)] + [("k", 2, 40, 0, 3, INF), ("q", 2, 50, 2, 0, NAN), ("do", 2, 60, 2, 5, INF),
+                                                             ("v", 2, 33, 1, 39, -INF), ("v", 2, 34, 1, 38, INF), ("v", 2, 176, 1, 0, NAN),
+                                                             ("state", 1, 0, 2, 4, INF), ("d_state", 1, 1, 3, 9, NAN)])
+    pad = torch.arange(260, device=DEV)[None, :] >= c["lengths"][:, None]
+    for n in ("q", "k", "v", "do"):
+        c[n][pad] = NAN
+    got = check_poisoned(c, dtype)
+    touched = torch.zeros(4, 3, dtype=torch.bool)
+    for b, h in ((0, 1), (2, 0), (2, 2), (2, 1), (1, 0), (1, 1)):
+        touched[b, h] = True
+    for n, g in got.items():
+        heads = (lambda t: t.transpose(1, 2)) if n in ("o", "dq", "dk", "dv") else (lambda t: t)
+        assert torch.equal(heads(g)[~touched.to(DEV)], heads(clean[n])[~touched.to(DEV)]), n
