@@ -366,21 +366,21 @@ constexpr long LN_LAUNCH_ROWS = 1L << 23;
 // 109, 524288 x 128 fp32 - / 93 / 97 / 97.
 constexpr int LN_FWD_PER = 2, LN_FWD_FULL = 2048;
 
-// M(vec, lanes, nv, nt) for the chosen shape; single values are never stored past the caches (rows narrower than a line)
-#define LN_SHAPES(M, V, NT)                                                 \
+// M(vec, lanes, nv, nt) for the chosen shape; rows of 129 to 256 pieces take L lanes with N pieces each.  Only whole pieces are
+// stored past the caches; single values go through them and are merged into lines there.
+#define LN_SHAPES(M, V, NT, L, N)                                           \
   if (g.lanes == 16) M(V, 16, 1, NT)                                        \
   else if (g.lanes == 32) M(V, 32, 1, NT)                                   \
   else if (g.lanes == 64 && g.nv == 1) M(V, 64, 1, NT)                      \
   else if (g.lanes == 64 && g.nv == 2) M(V, 64, 2, NT)                      \
-  else if (g.lanes == 64) M(V, 64, 4, NT)                                   \
-  else if (g.nv == 1) M(V, 256, 1, NT)                                      \
+  else if (g.lanes == L && g.nv == N) M(V, L, N, NT)                        \
   else if (g.nv == 2) M(V, 256, 2, NT)                                      \
   else if (g.nv == 4) M(V, 256, 4, NT)                                      \
   else M(V, 256, 8, NT)
-#define LN_PICK(M)                                       \
-  if (g.vec == V && nt) { LN_SHAPES(M, V, true) }        \
-  else if (g.vec == V) { LN_SHAPES(M, V, false) }        \
-  else { LN_SHAPES(M, 1, false) }
+#define LN_PICK(M, L, N)                                       \
+  if (g.vec == V && nt) { LN_SHAPES(M, V, true, L, N) }        \
+  else if (g.vec == V) { LN_SHAPES(M, V, false, L, N) }        \
+  else { LN_SHAPES(M, 1, false, L, N) }
 
 template <typename T, typename W>
 void ln_fwd_rows(const LnGeom& g, const T* x, long ldx, const W* w, const W* b, float eps, T* y, float* mean, float* rstd,
@@ -394,7 +394,7 @@ void ln_fwd_rows(const LnGeom& g, const T* x, long ldx, const W* w, const W* b, 
   const int per = groups >= (long)LN_FWD_FULL * LN_FWD_PER ? LN_FWD_PER : 1;
   const dim3 grid((unsigned)((groups + per - 1) / per));
 #define LN_FWD(VV, L, N, NT) hipLaunchKernelGGL((ln_fwd_kernel<T, W, VV, L, N, NT>), grid, dim3(256), 0, st, x, ldx, w, b, eps, y, mean, rstd, rows, D, per);
-  LN_PICK(LN_FWD)
+  LN_PICK(LN_FWD, 64, 4)
 #undef LN_FWD
 }
 
@@ -437,7 +437,7 @@ void ln_bwd(const void* dy, long lddy, const void* x, long ldx, const float* mea
     nslab = noise_grid(rows, 256 / g.lanes, g.lanes < 256 ? LN_BWD_GRID / 2 : g.nv == 1 ? LN_BWD_GRID : LN_BWD_GRID / 4);
     const dim3 grid(nslab);
 #define LN_BWD(VV, L, N, NT) hipLaunchKernelGGL((ln_bwd_kernel<T, W, VV, L, N, NT>), grid, dim3(256), 0, st, gp, lddy, xp, ldx, mean, rstd, wp, dp, sl, rows, D);
-    LN_PICK(LN_BWD)
+    LN_PICK(LN_BWD, 256, 1)
 #undef LN_BWD
   }
   if (sl) {
