@@ -73,6 +73,7 @@ class MultiTensorAdamW:
     every offset a multiple of 256, and scale [offsets[i] / 256 ...] of the scale buffers.
     """
     BLOCK = 256
+    MOST = 1 << 33      # values of one tensor: what one launch covers
 
     def __init__(self, params, lr=1e-4, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32):
         self.params = list(params)
@@ -92,6 +93,8 @@ class MultiTensorAdamW:
                 raise TypeError(f"parameter {i} is {p.dtype}: float32, bfloat16 or float16 expected")
             if not p.is_contiguous():
                 raise ValueError(f"parameter {i} of shape {tuple(p.shape)} is not contiguous")
+            if p.numel() > self.MOST:
+                raise ValueError(f"parameter {i} has {p.numel()} values: at most {self.MOST} are supported")
         self._apart(self.params)
         self.lr, self.betas, self.eps, self.weight_decay = hyper
         self.state_bits = state_bits
@@ -131,7 +134,7 @@ class MultiTensorAdamW:
     def step(self, grad_scale=1.0, grads=None):
         """One update from `grads` (one tensor or None per parameter), the parameters' own `.grad` when omitted.
         `grad_scale` multiplies every gradient (1 / world size of a summed data-parallel gradient)."""
-        params, n = self.params, len(self.params)
+        params, n, grad_scale = self.params, len(self.params), float(grad_scale)
         grads = list(map(attrgetter("grad"), params)) if grads is None else list(grads)
         if len(grads) != n:
             raise ValueError(f"{len(grads)} gradients for {n} parameters")

@@ -384,3 +384,24 @@ def test_step_output_over_other_arguments():
     for strides in ((5, D, 7, D, 9, D), (0, D) * 3):      # one stream: its stride says nothing
         with pytest.raises(RuntimeError, match="no ROCm-capable device"):
             step(q, strides=strides, B=1)
+
+
+def test_a_step_that_cannot_run_leaves_the_step_counts(on_cpu):
+    """A tensor beyond one launch is refused at construction, and a grad_scale that is no number before the counts advance; a
+    number of another kind counts as one."""
+    import numpy as np
+    import noise_amd as na
+    big = lambda n: torch.nn.Parameter(torch.empty(n, device="meta", dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="at most"):
+        na.MultiTensorAdamW([big(8), big((1 << 33) + 1)])
+    na.MultiTensorAdamW([big(1 << 33)], state_bits=8)
+    p, g = torch.nn.Parameter(torch.zeros(4)), torch.ones(4)
+    opt = na.MultiTensorAdamW([p])
+    for bad in (None, "x", torch.ones(2)):
+        with pytest.raises((TypeError, ValueError, RuntimeError)):
+            opt.step(grad_scale=bad, grads=[g])
+        assert not on_cpu
+    for scale in (torch.tensor(0.5), np.float32(0.5), 0.5):
+        opt.step(grad_scale=scale, grads=[g])
+        name, args = on_cpu[-1]
+        assert name == "noise_adamw_multi" and type(args[-2]) is float and args[-2] == 0.5
