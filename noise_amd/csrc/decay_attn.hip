@@ -410,7 +410,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
   __shared__ __attribute__((aligned(16))) T sk[C * LD], sv[C * LD];
   __shared__ __attribute__((aligned(16))) T sp[STATE_ONLY ? 8 : C * LDP];
   __shared__ float pw[C + 1];                             // lam^i
-  __shared__ float pv[2 * C];                             // s_kv lam^{63-i}; a chunk of n tokens starts at 64 - n
+  __shared__ float pv[2 * C];                             // s_kv lam^{C-1-i}; a chunk of n tokens starts at C - n
   __shared__ float pp[C + 16];                            // [15 + i - j]: s_o s_kv lam^{i-j}
   __shared__ unsigned top[F16 ? 3 * NW : 1];                 // largest finite a, k, v of the waves' pieces, as bits
   __shared__ int cut[2];
@@ -876,10 +876,12 @@ template <typename T>
 void walk_launch_16(const WalkSet& set, int n, int sums, hipStream_t st) {
   const int d = set.w[0].dk > set.w[0].dv ? set.w[0].dk : set.w[0].dv;
   const bool vec = walk_vec(set, n);
-  // tokens per chunk: 32 where 64 would spill registers (heads of 128: 273 -> 251 us for 32 clips of 2048 tokens, 16 heads) or
-  // cost a workgroup per CU (heads of 64 in bf16: 139 -> 126 us for 64 clips of 2048 tokens, 8 heads; in fp16 150 -> 163; heads of
-  // 16 in bf16, 64 clips of 1001: forward 44 -> 39 us, backward 109 -> 97, one clip of 60001 with 16 heads of 32: 283 -> 331); a pass that keeps only the state
-  // has the registers for 64 (60001 tokens, 16 heads of 128: 149 -> 134 us)
+  // tokens per chunk: 32 for heads of 128, where 64 spill registers (273 -> 251 us for 32 clips of 2048 tokens, 16 heads; at 32 the
+  // kernels for rows of 16-byte pieces spill none, those for single values 7 registers in bf16 and 28 in fp16), and for bf16
+  // heads of up to 64, where 64 cost a workgroup per CU: heads of 64, 64 clips of 2048 tokens, 8 heads 139 -> 126 us (fp16: 150 ->
+  // 163); heads of 16, 64 clips of 1001 forward 44 -> 39 us, backward 109 -> 97.  One long clip, which has few workgroups
+  // anyway, loses by it: 60001 tokens with 16 heads of 32 283 -> 331 us backward.  A pass that keeps only the state has the
+  // registers for 64 (60001 tokens, 16 heads of 128: 149 -> 134 us)
   constexpr int C64 = __is_same(T, bf16_t) ? 32 : 64;
   walk_passes(set, n, sums, st, [&](dim3 grid, auto only) {
     constexpr bool ONLY = decltype(only)::value;

@@ -334,8 +334,9 @@ struct LnGeom {
 };
 
 // The narrowest group of lanes that holds the row, a wave with at most `most` pieces per lane (forward 4; backward 2, since each
-// piece brings two gradient sums along: 65536 rows of 2048 bf16 values take 179 us with 64 lanes x 4 and 156 with 256 x 1).  `vec` is the 16-byte piece when every row of every tensor starts on a
-// 16-byte boundary and the width is a whole number of pieces, else single values.
+// piece brings two gradient sums along: 65536 rows of 2048 bf16 values take 179 us with 64 lanes x 4 and 156 with 256 x 1).
+// `vec` is the 16-byte piece when every row of every tensor starts on a 16-byte boundary and the width is a whole number of
+// pieces, else single values, whatever the width.
 LnGeom ln_geom(int D, int vec, int most) {
   static const int shapes[][2] = {{16, 1}, {32, 1}, {64, 1}, {64, 2}, {64, 4}, {256, 1}, {256, 2}, {256, 4}, {256, 8}};
   for (auto& s : shapes)
