@@ -10,9 +10,11 @@
 //
 // 8-bit states: m and r = sqrt(v) as e4m3 values with one fp32 scale = max|.| / 448 per 256 consecutive values of a tensor,
 // i.e. one wave's four values per lane.  r rather than v: its range within a block (2^18 : 1) is then v's 2^36 : 1.  A
-// positive r never becomes zero (it would leave m / eps).  The new moments are formed and rounded in 64 bits: 8-bit values
-// then depend on the inputs alone and not on the order of fp32 operations next to a rounding border.  A block with a
-// non-finite moment gets a NaN scale, which the next step shows in its parameters.
+// positive r never becomes zero (it would leave m / eps).  The new moments are formed and rounded in 64 bits, by the rule's own
+// operations, each rounded once: m = RN(RN(b1 m) + RN((1 - b1) g)), the root and both divisions to the nearest double.  Sums of
+// short numbers land on the border between two codes, or a scale halfway between two floats, by far more often than by chance
+// (b1 = 0.9: one scale in 600 of a model's list), and then an ulp of a double decides the code.  A block with a non-finite
+// moment gets a NaN scale, which the next step shows in its parameters.
 #include "token.h"
 
 namespace {
@@ -150,34 +152,44 @@ __device__ __forceinline__ unsigned wave_max_u32(unsigned v) {
   return max(max(a, b), max(c, d));
 }
 
-// A double as the float that rounds to the same 8-bit value: cut off, with the lowest bit set where something was lost, so
-// that the second rounding sees which side of a border the value lies on.
-__device__ __forceinline__ float to_odd(double x) {
-  const unsigned long long b = __double_as_longlong(x);
-  unsigned lo = (unsigned)b;
-  lo = (lo & 0xe0000000u) | ((lo & 0x1fffffffu) ? 0x20000000u : 0u);
-  return (float)__longlong_as_double((long long)((b & 0xffffffff00000000ull) | lo));
-}
-
-// Four values of a 256-value block as e4m3 codes under the scale max / 448; the whole wave takes part.  The largest magnitude
-// is found on the bits of the doubles (their order is the integers', and a NaN or infinity is above all others): the high
-// words first, then, where several lanes share the highest, the low words.
-template <bool POSITIVE>
-__device__ __forceinline__ unsigned quantise4(const double (&x)[4], float& scale) {
-  double t = fabs(x[0]);
-#pragma unroll
-  for (int j = 1; j < 4; ++j) t = t >= fabs(x[j]) ? t : fabs(x[j]);      // a NaN among x[1..3] is taken over, one in t is lost:
-  bool nan = false;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) nan |= x[j] != x[j];                         // hence this
-  const unsigned hi = nan ? 0x7ff80000u : (unsigned)(__double_as_longlong(t) >> 32), lo = (unsigned)__double_as_longlong(t);
+// Largest magnitude of the wave's values, four per lane, found on the bits of the doubles (their order is the integers', and a NaN or
+// infinity is above all others): the high words first, then, where several lanes share the highest, the low words.
+__device__ __forceinline__ double block_top(const double (&x)[4]) {
+  const double t = __builtin_fmax(__builtin_fmax(fabs(x[0]), fabs(x[1])), __builtin_fmax(fabs(x[2]), fabs(x[3])));
+  const double sum = (x[0] + x[1]) + (x[2] + x[3]);            // a NaN is lost in the maximum, not here
+  const unsigned hi = sum != sum ? 0x7ff80000u : (unsigned)(__double_as_longlong(t) >> 32), lo = (unsigned)__double_as_longlong(t);
   const unsigned th = wave_max_u32(hi);
   const unsigned long long who = __ballot(hi == th);
   unsigned tl;
   if ((who & (who - 1)) == 0) tl = (unsigned)__builtin_amdgcn_readlane((int)lo, __builtin_ctzll(who));
   else tl = wave_max_u32(hi == th ? lo : 0u);
-  const double top = __longlong_as_double((long long)((unsigned long long)th << 32 | tl));
-  scale = (float)(top * (1.0 / 448.0));
+  return __longlong_as_double((long long)((unsigned long long)th << 32 | tl));
+}
+
+// a / b to the nearest double, with 1 / b to its last bits: the product's remainder is exact and corrects it.
+__device__ __forceinline__ double divide64(double a, double b, double inv) {
+  const double q = a * inv;
+  return __builtin_fma(__builtin_fma(-q, b, a), inv, q);
+}
+
+// sqrt of a value >= 0 in 64 bits to about 46: the hardware's reciprocal root (2^-23) and one step of Newton's method; EXACT: another
+// one, which leaves little but its own rounding.
+template <bool EXACT>
+__device__ __forceinline__ double root64(double v) {
+  const double y = __builtin_amdgcn_rsq(v + 1e-300), h = 0.5 * y;      // 1e-300: zero gives zero
+  double s = v * y;
+  s = __builtin_fma(h, __builtin_fma(-s, s, v), s);
+  return EXACT ? __builtin_fma(h, __builtin_fma(-s, s, v), s) : s;
+}
+
+// Four values of a 256-value block as e4m3 codes under the scale max / 448 (`top`: that maximum), rounded as x / scale would be.
+// What is rounded to 8 bits is a float of x / scale that is cut off, with its lowest bit set where something was lost, so that
+// the second rounding sees which side of a border the value lies on.  All borders have few bits: the 29 that the cut takes are
+// zero there.  The product x * (1 / scale) decides wherever it is further from that than it can be wrong (NEAR units of a
+// double's last place); where one of a lane's four is nearer, exact(j) and its true quotient do.
+template <bool POSITIVE, unsigned NEAR, typename Exact>
+__device__ __forceinline__ unsigned quantise4(const double (&x)[4], double top, float& scale, Exact exact) {
+  scale = (float)divide64(top, 448.0, 1.0 / 448.0);
   // 1 / scale to the last bits of a double: a float's reciprocal and two steps of Newton's method; a block whose scale is below
   // the normal floats is divided by it
   const double d = (double)scale;
@@ -185,19 +197,28 @@ __device__ __forceinline__ unsigned quantise4(const double (&x)[4], float& scale
   inv = __builtin_fma(__builtin_fma(-d, inv, 1.0), inv, inv);
   inv = __builtin_fma(__builtin_fma(-d, inv, 1.0), inv, inv);
   if (!(scale > 1e-36f && scale < 1e36f)) inv = scale > 0.f ? 1.0 / d : 0.0;
+  unsigned long long b[4];
+  unsigned away = 0xffffffffu;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    b[j] = (unsigned long long)__double_as_longlong(x[j] * inv);
+    away = min(away, ((unsigned)b[j] + NEAR) & 0x1fffffffu);
+    b[j] = (b[j] & 0xffffffffe0000000ull) | 0x20000000ull;
+  }
+  if (away <= 2 * NEAR) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const unsigned long long t = (unsigned long long)__double_as_longlong(divide64(exact(j), d, inv));
+      b[j] = (t & 0xffffffffe0000000ull) | ((t & 0x1fffffffull) ? 0x20000000ull : 0ull);
+    }
+  }
   float q[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) q[j] = __builtin_amdgcn_fmed3f(to_odd(x[j] * inv), POSITIVE && x[j] > 0.0 ? 0x1p-9f : -448.f, 448.f);
+  for (int j = 0; j < 4; ++j) q[j] = __builtin_amdgcn_fmed3f((float)__longlong_as_double((long long)b[j]), POSITIVE && x[j] > 0.0 ? 0x1p-9f : -448.f, 448.f);
   int code = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
   code = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], code, true);
-  if (th >= 0x7ff00000u) scale = __int_as_float(0x7fc00000);
+  if (!(top < INFINITY)) scale = __int_as_float(0x7fc00000);
   return (unsigned)code;
-}
-
-// sqrt of a value >= 0 in 64 bits to about 46: the hardware's reciprocal root and one step of Newton's method.
-__device__ __forceinline__ double root64(double v) {
-  const double y = __builtin_amdgcn_rsq(v + 1e-300), s = v * y;      // 1e-300: zero gives zero
-  return __builtin_fma(0.5 * y, __builtin_fma(-s, s, v), s);
 }
 
 // a / b: the hardware's reciprocal and one correction (within one unit of the last place); the division itself where b or its
@@ -227,20 +248,25 @@ __device__ __forceinline__ void adam8_unit(const AdamUnit<P, G>& t, unsigned* ms
     cm[0] = m0[0], cm[1] = m0[1], cm[2] = m1[0], cm[3] = m1[1];
     cr[0] = r0[0], cr[1] = r0[1], cr[2] = r1[0], cr[3] = r1[1];
   }
-  const double fm = c.dbeta1 * sm, fr = c.dbeta2 * (sr * sr);
-  double m[4], r[4];
+  const double fr = c.dbeta2 * (sr * sr);
+  double m[4], v[4], r[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const double gi = (double)(gv[j] * c.grad_scale);
-    m[j] = __builtin_fma((double)cm[j], fm, c.domb1 * gi);
-    r[j] = root64(__builtin_fma((double)(cr[j] * cr[j]), fr, c.domb2 * (gi * gi)));   // a code's square has 8 bits
+    m[j] = c.dbeta1 * ((double)cm[j] * sm) + c.domb1 * gi;    // the old m is exact: a code has 4 bits, a scale 24
+    v[j] = __builtin_fma((double)(cr[j] * cr[j]), fr, c.domb2 * (gi * gi));   // a few units of the last place; a code's square has 8 bits
+    r[j] = root64<false>(v[j]);
     const float denom = (float)r[j] * inv_root + c.eps;
     pv[j] = pv[j] * c.decay - t.coef.x * quotient((float)m[j], denom);
   }
   store4<FULL>(t.p, i, n, t.vec, pv);
   float nm, nr;
-  ms[q] = quantise4<false>(m, nm);
-  rs[q] = quantise4<true>(r, nr);
+  ms[q] = quantise4<false, 4>(m, block_top(m), nm, [&](int j) { return m[j]; });
+  // r is off by 2^-46 of itself: 2^6 units of its last place
+  rs[q] = quantise4<true, 512>(r, root64<true>(block_top(v)), nr, [&](int j) {
+    const double gi = (double)(gv[j] * c.grad_scale), ro = (double)cr[j] * sr;
+    return root64<true>(c.dbeta2 * (ro * ro) + c.domb2 * (gi * gi));
+  });
   if ((threadIdx.x & 63) == 0) {
     mscale[sc] = nm;
     rscale[sc] = nr;

@@ -372,3 +372,95 @@ def test_the_waveform_model_trains_with_it(bits):
             close_p(p.detach().view(-1), r, r.step(p.grad.reshape(-1), 1e-3, 0.9, 0.999, 1e-8, 1e-2), 1)
             r.p = p.detach().view(-1).double().cpu()
     assert (opt.step_count == 3).all()
+
+
+def codes_of(values):
+    """e4m3 values (exact ones) -> their bytes."""
+    c = torch.searchsorted(TABLE, values.abs().double())
+    assert torch.equal(TABLE[c], values.abs().double())
+    return (c + 128 * (values < 0)).to(torch.uint8)
+
+
+@pytest.mark.parametrize("gdtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("betas", [(0.9, 0.999), (0.5, 0.25), (0.8, 0.0)])
+def test_small_states_on_rounding_borders(betas, gdtype):
+    """First moments that are whole numbers in units of the scale, on the very border between two codes, and scales halfway between
+    two floats: sums of short numbers get there even where 1 - b1 is no short number, so the bytes are those of the rule's own
+    64-bit operations and of no others."""
+    import noise_amd as na
+    b1 = betas[0]
+    g = torch.Generator().manual_seed(8)
+    blocks = 400
+    ints = TABLE[(TABLE == TABLE.round()) & (TABLE <= 448) & (TABLE > 0)]
+    mids = (TABLE[1:] + TABLE[:-1]) / 2
+    mids = mids[(mids == mids.round()) & (mids < 448)]
+    pick = lambda t: t[torch.randint(0, len(t), (blocks, 256), generator=g)] * torch.where(torch.rand(blocks, 256, generator=g) < 0.5, -1.0, 1.0)
+    unit = 2.0 ** torch.randint(-30, -10, (blocks, 1), generator=g).double()
+    # b1 m + (1 - b1) g = y: where b1 is a multiple of 1 / 10, g = (10 y - 10 b1 m) / (10 - 10 b1) is a whole number for enough of them
+    m, y = pick(ints), pick(mids)
+    m[:, 0], y[:, 0] = 448.0, 448.0
+    need = (10 * y - round(10 * b1) * m) / round(10 - 10 * b1)
+    grad = torch.where(need == need.to(gdtype).double(), need, 0.0)
+    params, states = [torch.nn.Parameter(torch.ones(blocks * 256, device=DEV))], dict(m=codes_of(m.view(-1)), scale=unit.view(-1).float())
+    grads = [(grad * unit).view(-1).to(gdtype).to(DEV)]
+    assert torch.equal(grads[0].double().cpu().view(blocks, 256), grad * unit)
+    opt = na.MultiTensorAdamW(params, betas=betas, state_bits=8)
+    sd = opt.state_dict()
+    sd["exp_avg"], sd["exp_avg_scale"] = states["m"].view(torch.float8_e4m3fn).to(DEV), states["scale"].to(DEV)
+    r = TABLE[torch.randint(1, 127, (blocks * 256,), generator=g)]
+    sd["exp_avg_sq_root"], sd["exp_avg_sq_root_scale"] = codes_of(r).view(torch.float8_e4m3fn).to(DEV), (unit.view(-1) / 7).float().to(DEV)
+    opt.load_state_dict(sd)
+    rule = Rule(params[0], 8)
+    rule.m, rule.r = (states["m"], states["scale"]), (codes_of(r), (unit.view(-1) / 7).float())
+    on_border = 0
+    for step in range(3):
+        opt.step(grads=grads)
+        mag = rule.step(grads[0], 1e-4, *betas, 1e-8, 1e-2)
+        for key, (codes, scale) in (("exp_avg", rule.m), ("exp_avg_sq_root", rule.r)):
+            assert torch.equal(regions(opt, key + "_scale", 0), scale), (key, (regions(opt, key + "_scale", 0) != scale).sum())
+            got = regions(opt, key, 0)
+            same = (got == codes) | ((got & 127 == 0) & (codes & 127 == 0))
+            assert same.all(), (key, (~same).sum())
+        if step == 0:
+            new = b1 * value(states["m"], states["scale"], blocks * 256) + (1 - b1) * grads[0].double().cpu()
+            x = new.view(-1, 256).abs() / rule.m[1].double()[:, None]
+            on_border = torch.isin(x, mids).sum()
+    assert on_border > 500
+
+
+def test_small_state_scales_halfway_between_floats():
+    """The largest moment is 448 t with t halfway between two floats, in every block: t goes to the even one."""
+    import noise_amd as na
+    blocks = 2000
+    g = torch.Generator().manual_seed(3)
+    odd = (1 << 24) + 1 + 2 * torch.randint(0, 1 << 23, (blocks,), generator=g)          # 25 bits: no float
+    old = ((odd - 1).double() * 2.0 ** -29)                                              # 24 bits
+    assert torch.equal(old.float().double(), old)
+    p = torch.nn.Parameter(torch.ones(blocks * 256, device=DEV))
+    grad = torch.zeros(blocks, 256, dtype=torch.float64)
+    grad[:, 5] = 448 * 2.0 ** -29                    # 0.5 (448 old + grad) = 448 odd 2^-30
+    codes = torch.zeros(blocks, 256, dtype=torch.uint8)
+    codes[:, 5] = 126
+    opt = na.MultiTensorAdamW([p], betas=(0.5, 0.75), state_bits=8)
+    sd = opt.state_dict()
+    sd["exp_avg"], sd["exp_avg_scale"] = codes.view(-1).view(torch.float8_e4m3fn).to(DEV), old.float().to(DEV)
+    opt.load_state_dict(sd)
+    opt.step(grads=[grad.view(-1).float().to(DEV)])
+    want = torch.where(odd % 4 == 1, odd - 1, odd + 1).double() * 2.0 ** -30              # the neighbour with an even last bit
+    assert torch.equal(opt.state["exp_avg_scale"].cpu().double(), want)
+    assert torch.equal(opt.state["exp_avg"].view(torch.uint8).cpu().view(-1, 256), codes)
+
+
+def test_first_step_of_short_gradients():
+    """From zero states the roots are sqrt(1 - b2) |g|: ratios of short gradients lie next to borders, a float's rounding away."""
+    import noise_amd as na
+    n = 256 * 4000
+    g = torch.Generator().manual_seed(5)
+    p = torch.nn.Parameter(torch.ones(n, device=DEV))
+    grad = (torch.randint(1, 256, (n,), generator=g).double() * 2.0 ** torch.randint(-3, 4, (n,), generator=g)).to(torch.bfloat16)
+    opt, rule = na.MultiTensorAdamW([p], state_bits=8), Rule(p, 8)
+    opt.step(grads=[grad.to(DEV)])
+    rule.step(grad, 1e-4, 0.9, 0.999, 1e-8, 1e-2)
+    for key, (codes, scale) in (("exp_avg", rule.m), ("exp_avg_sq_root", rule.r)):
+        assert torch.equal(regions(opt, key + "_scale", 0), scale), key
+        assert torch.equal(regions(opt, key, 0), codes), (key, (regions(opt, key, 0) != codes).sum())
