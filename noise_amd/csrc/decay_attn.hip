@@ -328,7 +328,11 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, 2) void walk_f32_kernel(Walk
 
 // 16-bit tokens on the 16-bit matrix cores (v_mfma_f32_16x16x32_bf16 / _f16), 32 or 64 tokens per chunk, P / 16 waves that own 16
 // state columns each.  What is rounded to 16 bits on its way into a product, and what is not:
-//   * the weights lam^{i-j} (a_i . k_j) and the state as it meets a_i: once each, like the output they lead to;
+//   * the weights lam^{i-j} (a_i . k_j) and the state as it meets a_i go in as two terms of the type each (2^-15 in bf16, 2^-22 in fp16
+//     is left over), so that the output's own rounding is the only one that counts: with one term each its error was 1.41 times that
+//     on long clips and up to 2.3 times on single tokens.  The weights' second term costs nothing; the state's: heads of 64, 64 clips
+//     of 1001 tokens, 8 heads 70 -> 69 us; heads of 128 by instruction issue, 8 clips of 4096, 16 heads 205 -> 216 us forward,
+//     397 -> 465 backward;
 //   * lam^{n-1-j} v_j on its way into the state is split into three terms of the type (24 bits), since the state is fp32,
 //     carried over any number of chunks and returned: X keeps fp32 accuracy at three products per term.
 // fp16 has the fraction for that but not the range, so those three operands go in scaled by powers of two that bounds give
@@ -389,6 +393,25 @@ __device__ __forceinline__ unsigned pack16(float a, float b) {
   const x2<T> v = {(T)a, (T)b};
   return __builtin_bit_cast(unsigned, v);
 }
+// The leading term of two floats, and in their place what it leaves of them (exactly).  bf16 cuts: three terms are the whole float.
+template <typename T>
+__device__ __forceinline__ unsigned split16(float& a, float& b) {
+  if constexpr (__is_same(T, bf16_t)) {
+    const unsigned ua = __float_as_uint(a), ub = __float_as_uint(b), c = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+    a -= __uint_as_float(ua & 0xffff0000u);
+    b -= __uint_as_float(ub & 0xffff0000u);
+    return c;
+  } else {
+    // fixed before and after they are rounded: the compiler would round them once more, each by itself, where a rest is formed, or
+    // round the product that leads to a there, and not a, and the terms would not add up
+    asm("" : "+v"(a), "+v"(b));
+    unsigned c = pack16<T>(a, b);
+    asm("" : "+v"(c));
+    a -= low16<T>(c);
+    b -= high16<T>(c);
+    return c;
+  }
+}
 __device__ __forceinline__ f32x4 mfma16(x8<bf16_t> a, x8<bf16_t> b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f32x4 mfma16(x8<f16_t> a, x8<f16_t> b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
@@ -408,7 +431,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
   constexpr int LD = P + 16, LDP = C + 8, SLOTS = C * P / 8 / NTHR;
   __shared__ __attribute__((aligned(16))) T sa[STATE_ONLY ? 8 : C * LD];
   __shared__ __attribute__((aligned(16))) T sk[C * LD], sv[C * LD];
-  __shared__ __attribute__((aligned(16))) T sp[STATE_ONLY ? 8 : C * LDP];
+  __shared__ __attribute__((aligned(16))) T sp[2][STATE_ONLY ? 8 : C * LDP];   // weights, in two terms
   __shared__ float pw[C + 1];                             // lam^i
   __shared__ float pv[2 * C];                             // s_kv lam^{C-1-i}; a chunk of n tokens starts at C - n
   __shared__ float pp[C + 16];                            // [15 + i - j]: s_o s_kv lam^{i-j}
@@ -437,7 +460,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
     // the weight tiles (0, 1) and (2, 3) lie above the diagonal but in a pair that is read: they stay zero
     for (int i = tid; i < C / 32 * 256; i += NTHR) {
       const int half = i >> 8, r = i >> 4 & 15, c = i & 15;
-      sp[(half * 32 + r) * LDP + half * 32 + 16 + c] = (T)0.f;
+      sp[0][(half * 32 + r) * LDP + half * 32 + 16 + c] = sp[1][(half * 32 + r) * LDP + half * 32 + 16 + c] = (T)0.f;
     }
   }
   const T* ab = (const T*)w.a + (size_t)b * w.sa.b + (size_t)h * w.sa.h;
@@ -602,6 +625,7 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
       carry = pow2(ev - E);
       E = ev;
     }
+    const float decay = pw[n - shift] * carry;
     f32x4 O[STATE_ONLY ? 1 : NI];
     if (!STATE_ONLY) {
       // ---- weights, transposed tile by tile (rows j, columns i) so that a lane holds four neighbouring j of one i: the
@@ -628,38 +652,44 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
         asm("" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]));
         const int last = it == jt ? l16 - 4 * q : 4;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[r] = r <= last ? acc[r] * (F16 ? unit_p * f[r] : f[r]) : 0.f;
-        *(uint2*)(sp + i * LDP + j) = make_uint2(pack16<T>(acc[0], acc[1]), pack16<T>(acc[2], acc[3]));
+        for (int r = 0; r < 4; ++r) f[r] = r <= last ? acc[r] * (F16 ? unit_p * f[r] : f[r]) : 0.f;
+        *(uint2*)(sp[0] + i * LDP + j) = make_uint2(split16<T>(f[0], f[1]), split16<T>(f[2], f[3]));
+        *(uint2*)(sp[1] + i * LDP + j) = make_uint2(pack16<T>(f[0], f[1]), pack16<T>(f[2], f[3]));
       }
-      // ---- what the state contributes, transposed: rows are the wave's columns, columns the tokens
+      // ---- what the state contributes, transposed: rows are the wave's columns, columns the tokens.  X goes on decayed; its old
+      // registers are split where they lie
 #pragma unroll
       for (int it = 0; it < NI; ++it) O[it] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kp = 0; kp < KP; ++kp) {
-        u32x4 u;
+        u32x4 high, low;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x0 = X[kp][e >> 1][2 * (e & 1)], x1 = X[kp][e >> 1][2 * (e & 1) + 1];
-          u[e] = F16 ? pack16<T>(x0 * unit_x, x1 * unit_x) : pack16<T>(x0, x1);
+          float x0 = X[kp][e >> 1][2 * (e & 1)], x1 = X[kp][e >> 1][2 * (e & 1) + 1];
+          if constexpr (F16) x0 *= unit_x, x1 *= unit_x;
+          high[e] = split16<T>(x0, x1);
+          low[e] = pack16<T>(x0, x1);
         }
-        const x8<T> x = __builtin_bit_cast(x8<T>, u);
+        // (all of one term, then all of the other: a product waits for the one before it that adds to the same tile)
+        x8<T> y[NI];
 #pragma unroll
         for (int it = 0; it < NI; ++it) {
-          const x8<T> y = *(const x8<T>*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
-          O[it] = mfma16(x, y, O[it]);
+          y[it] = *(const x8<T>*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
+          O[it] = mfma16(__builtin_bit_cast(x8<T>, low), y[it], O[it]);
         }
+#pragma unroll
+        for (int it = 0; it < NI; ++it) O[it] = mfma16(__builtin_bit_cast(x8<T>, high), y[it], O[it]);
       }
 #pragma unroll
       for (int it = 0; it < NI; ++it) O[it] *= s_o * pw[it * 16 + l16 + 1 - shift] * back;
     }
     // ---- X = lam^n X + K^T V'
     x8<T> v[C / 32];
-    const float f = pw[n - shift] * carry;
     if constexpr (F16) bound = fminf(bound * pw[n - shift] + largest, 3e38f);
 #pragma unroll
     for (int kp = 0; kp < KP; ++kp)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) X[kp][s] *= f;
+      for (int s = 0; s < 2; ++s) X[kp][s] *= decay;
 #pragma unroll
     for (int jj = 0; jj < C / 32; ++jj) {
       v[jj] = read_tokens<LD, T>(sv + jj * 32 * LD + col0, q, l16);
@@ -669,16 +699,9 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
       for (int e = 0; e < 4; ++e) {
         const unsigned u = __builtin_bit_cast(u32x4, v[jj])[e];
         float y0 = low16<T>(u) * (F16 ? unit_v * f8[2 * e] : f8[2 * e]), y1 = high16<T>(u) * (F16 ? unit_v * f8[2 * e + 1] : f8[2 * e + 1]);
-        // the compiler may round the exact product, not y, to fp16 in one of the two places that read the first term, and the
-        // terms would then not add up: y is fixed before it is split
-        if constexpr (F16) asm("" : "+v"(y0), "+v"(y1));
 #pragma unroll
-        for (int z = 0; z < 3; ++z) {
-          const unsigned c = pack16<T>(y0, y1);
-          t[z][e] = c;
-          y0 -= low16<T>(c);
-          y1 -= high16<T>(c);
-        }
+        for (int z = 0; z < 2; ++z) t[z][e] = split16<T>(y0, y1);
+        t[2][e] = pack16<T>(y0, y1);
       }
 #pragma unroll
       for (int kp = 0; kp < KP; ++kp)
@@ -697,10 +720,12 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
 #pragma unroll
       for (int jj = 0; jj < C / 32; ++jj)
 #pragma unroll
-        for (int it = 2 * jj; it < NI; ++it) {
-          const x8<T> y = *(const x8<T>*)(sp + (it * 16 + l16) * LDP + jj * 32 + 8 * q);
-          O[it] = mfma16(v[jj], y, O[it]);
-        }
+        for (int z = 1; z >= 0; --z)
+#pragma unroll
+          for (int it = 2 * jj; it < NI; ++it) {
+            const x8<T> y = *(const x8<T>*)(sp[z] + (it * 16 + l16) * LDP + jj * 32 + 8 * q);
+            O[it] = mfma16(v[jj], y, O[it]);
+          }
     }
     // the next tiles go in before this chunk's rows go out: waiting for loads that are older than a store is not waiting for the
     // store (memory operations are counted in order).  Wide heads have no registers to hold both, and other waves to run.
@@ -877,9 +902,10 @@ void walk_launch_16(const WalkSet& set, int n, int sums, hipStream_t st) {
   const int d = set.w[0].dk > set.w[0].dv ? set.w[0].dk : set.w[0].dv;
   const bool vec = walk_vec(set, n);
   // tokens per chunk: 32 for heads of 128, where 64 spill registers (273 -> 251 us for 32 clips of 2048 tokens, 16 heads; at 32 the
-  // kernels for rows of 16-byte pieces spill none, those for single values 7 registers in bf16 and 28 in fp16), and for bf16
+  // kernels for rows of 16-byte pieces spill none, those for single values some), and for bf16
   // heads of up to 64, where 64 cost a workgroup per CU: heads of 64, 64 clips of 2048 tokens, 8 heads 139 -> 126 us (fp16: 150 ->
-  // 163); heads of 16, 64 clips of 1001 forward 44 -> 39 us, backward 109 -> 97.  One long clip, which has few workgroups
+  // 163); heads of 16, 64 clips of 1001 forward 44 -> 39 us, backward 109 -> 97 (fp16: 66 -> 72 and 133 -> 109, so by
+  // direction there).  One long clip, which has few workgroups
   // anyway, loses by it: 60001 tokens with 16 heads of 32 283 -> 331 us backward.  A pass that keeps only the state has the
   // registers for 64 (60001 tokens, 16 heads of 128: 149 -> 134 us)
   constexpr int C64 = __is_same(T, bf16_t) ? 32 : 64;
@@ -890,7 +916,8 @@ void walk_launch_16(const WalkSet& set, int n, int sums, hipStream_t st) {
     if (vec) hipLaunchKernelGGL((walk_16_kernel<T, P, C, ONLY, true>), grid, dim3(P * 4), 0, st, set); \
     else hipLaunchKernelGGL((walk_16_kernel<T, P, C, ONLY, false>), grid, dim3(P * 4), 0, st, set);    \
   } while (0)
-    if (d <= 32) GO(32, C64);
+    if (d <= 32 && n > 1) GO(32, 32);
+    else if (d <= 32) GO(32, C64);
     else if (d <= 64) GO(64, C64);
     else GO(128, (ONLY ? 64 : 32));
 #undef GO

@@ -18,10 +18,10 @@ packed projection are read in place; a last axis without unit stride is copied f
 and behind lengths[b] are neither read nor added to the state, their rows of o and of the gradients are zero, and the state
 returned is the one behind the last real token.  `scale` defaults to Dk ** -0.5.
 
-Numbers: states are carried in fp32 accuracy whatever the tokens' type; in 16-bit types the weights inside a chunk and the
-state as it meets q are rounded to the type once each, like the output (0.0023 from the exact result in bf16, where rounding
-the exact result alone is 0.0017).  fp16 keeps that within 2^28 of the largest value that 16 neighbouring columns of a state
-may hold by its bound, the decayed sum of max |k| max |v|.  A token that is not finite reaches what the formulas say: its
+Numbers: states are carried in fp32 accuracy whatever the tokens' type, and in 16-bit types o, dq, dk and dv are rounded to the type
+once: the weights inside a chunk and the state as it meets q enter the products with at least 15 bits of fraction.  In fp16 that
+holds within 2^18 of the largest value that 16 neighbouring columns of a state may hold by its bound, the decayed sum of
+max |k| max |v|, and one bit less for each factor of two beyond.  A token that is not finite reaches what the formulas say: its
 column and later tokens, or all columns where it is one of k or q; an infinity may come out as a NaN.
 """
 import ctypes

@@ -518,3 +518,23 @@ def test_poison_everywhere_and_nowhere_else(dtype):
     for n, g in got.items():
         heads = (lambda t: t.transpose(1, 2)) if n in ("o", "dq", "dk", "dv") else (lambda t: t)
         assert torch.equal(heads(g)[~touched.to(DEV)], heads(clean[n])[~touched.to(DEV)]), n
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,T,H,dk,dv", [(1, 1, 1, 8, 8), (1, 3, 2, 8, 8), (2, 5, 2, 128, 128), (4, 20, 4, 16, 16), (3, 33, 3, 10, 10), (2, 100, 2, 33, 64),
+                                         (2, 300, 4, 64, 64), (2, 300, 3, 128, 100), (1, 1500, 2, 128, 128), (1, 2000, 2, 24, 24)])
+def test_16_bit_results_are_rounded_once(B, T, H, dk, dv, dtype):
+    """Two terms of a 16-bit type leave 2^-15 (bf16: the first is cut, 2^-7 of the value, the second rounded, 2^-8 of that) or 2^-22 (fp16:
+    2^-11 twice) of each weight and of each state element as it enters a product; a term of a result passes through one of them.
+    fp16 is scaled to 2^14 by a bound, below 2^-14 its steps are 2^-24: 2^-39 of a bound that is far less than 2^16 times the
+    magnitudes that are added up here.  Beside that the fp32 roundings as ever, and one rounding of the result."""
+    c = make(B, T, H, dk, dv, dtype, B + 7 * T + dk)
+    c["log_decay"] = torch.tensor([-0.125, -4e-4, -0.01, 0.0][:H], device=DEV)
+    got, scale = run_all(c), dk ** -0.5
+    want, mag = recurrence(c, scale), recurrence(c, scale, True)
+    left = 2.0 ** -15 if dtype == torch.bfloat16 else 2.0 ** -22 + 2.0 ** -23
+    n = (T + max(dk, dv)) + 16 + 2 * (T // 32 + 1)
+    for name in ("o", "dq", "dk", "dv"):
+        t = (n * U + 1.01 * left) * mag[name] + half(dtype) * want[name].abs() * 1.01 + tiny(dtype) + 1e-30
+        d = (got[name].double() - want[name]).abs()
+        assert (d <= t).all(), (name, (d / t).max().item())
