@@ -330,9 +330,10 @@ __global__ __launch_bounds__(P >= 64 ? 256 : P * 4, 2) void walk_f32_kernel(Walk
 // state columns each.  What is rounded to 16 bits on its way into a product, and what is not:
 //   * the weights lam^{i-j} (a_i . k_j) and the state as it meets a_i go in as two terms of the type each (2^-15 in bf16, 2^-22 in fp16
 //     is left over), so that the output's own rounding is the only one that counts: with one term each its error was 1.41 times that
-//     on long clips and up to 2.3 times on single tokens.  The weights' second term costs nothing; the state's: heads of 64, 64 clips
-//     of 1001 tokens, 8 heads 70 -> 69 us; heads of 128 by instruction issue, 8 clips of 4096, 16 heads 205 -> 216 us forward,
-//     397 -> 465 backward;
+//     on long clips and up to 2.3 times on single tokens.  The weights' second term costs nothing; the state's, in us before and
+//     after: heads of 64, 64 clips of 1001 tokens, 8 heads 70 and 70, one workgroup per CU (256 pairs of 2048 tokens) 80 and 87; heads
+//     of 128, 192 pairs 129 and 132, where instruction issue bounds them (8 clips of 4096, 16 heads) 207 and 217 forward, 398 and
+//     463 backward;
 //   * lam^{n-1-j} v_j on its way into the state is split into three terms of the type (24 bits), since the state is fp32,
 //     carried over any number of chunks and returned: X keeps fp32 accuracy at three products per term.
 // fp16 has the fraction for that but not the range, so those three operands go in scaled by powers of two that bounds give
@@ -660,25 +661,40 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
       // registers are split where they lie
 #pragma unroll
       for (int it = 0; it < NI; ++it) O[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+      // All of the first terms, then the second ones, which are formed while the products run; in wide heads they add to tiles of
+      // their own, so that the two do not wait for each other
+      constexpr bool APART = P == 128;
+      u32x4 low[KP];
+      x8<T> y[KP][NI];
+      f32x4 R[NI];
+#pragma unroll
+      for (int it = 0; it < NI; ++it) R[it] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kp = 0; kp < KP; ++kp) {
-        u32x4 high, low;
+        u32x4 high;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float x0 = X[kp][e >> 1][2 * (e & 1)], x1 = X[kp][e >> 1][2 * (e & 1) + 1];
           if constexpr (F16) x0 *= unit_x, x1 *= unit_x;
           high[e] = split16<T>(x0, x1);
-          low[e] = pack16<T>(x0, x1);
+          low[kp][e] = pack16<T>(x0, x1);
         }
-        // (all of one term, then all of the other: a product waits for the one before it that adds to the same tile)
-        x8<T> y[NI];
 #pragma unroll
         for (int it = 0; it < NI; ++it) {
-          y[it] = *(const x8<T>*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
-          O[it] = mfma16(__builtin_bit_cast(x8<T>, low), y[it], O[it]);
+          y[kp][it] = *(const x8<T>*)(sa + (it * 16 + l16) * LD + kp * 32 + 8 * q);
+          O[it] = mfma16(__builtin_bit_cast(x8<T>, high), y[kp][it], O[it]);
         }
+      }
 #pragma unroll
-        for (int it = 0; it < NI; ++it) O[it] = mfma16(__builtin_bit_cast(x8<T>, high), y[it], O[it]);
+      for (int kp = 0; kp < KP; ++kp)
+#pragma unroll
+        for (int it = 0; it < NI; ++it) {
+          f32x4& to = APART ? R[it] : O[it];
+          to = mfma16(__builtin_bit_cast(x8<T>, low[kp]), y[kp][it], to);
+        }
+      if constexpr (APART) {
+#pragma unroll
+        for (int it = 0; it < NI; ++it) O[it] += R[it];
       }
 #pragma unroll
       for (int it = 0; it < NI; ++it) O[it] *= s_o * pw[it * 16 + l16 + 1 - shift] * back;
