@@ -951,11 +951,13 @@ int walk_launch(const WalkSet& set, int n, int sums, int dtype, hipStream_t st) 
 // read of k and v costs more than it gives; below, the axis is cut until there are `target` workgroups.  A workgroup has one wave
 // per 16 columns (fp32: at most four), so narrow heads need more of them; a backward pass has three walks per pair in flight and
 // pays for segments with two sums, so it needs fewer.  Measured on 2048 tokens, us with 1 / 2 / 4 / 8 segments, forward:
-//   bf16, heads of 16: 256 pairs 54 / 62 / 62 / 69, 128 pairs 53 / 52 / 39 / 41; of 64: 256 pairs 79 / 96 / 96 / 106, 192 pairs
-//   74 / 83 / 69 / 73; of 128: 192 pairs 129 / 158 / 160 / 204, 128 pairs 126 / 116 / 107 / 130; fp16, heads of 16: 384 pairs
-//   114 / 97 / 105 / 104; fp32, heads of 128: 192 pairs 422 / 477 / 423 / 445, 128 pairs 419 / 345 / 293 / 306
-// backward: bf16, heads of 64: 128 pairs 91 / 104 / 102 / 116, 64 pairs 76 / 84 / 62 / 65; of 128: 96 pairs 183 / 220 / 208 / 250;
-//   fp32, heads of 128: 128 pairs 670 / 711 / 700 / 746, 96 pairs 668 / 699 / 577 / 576.
+//   bf16, heads of 16: 256 pairs 66 / 68 / 60 / 66, 128 pairs 66 / 62 / 43 / 39; of 64: 256 pairs 84 / 107 / 104 / 125, 192 pairs
+//   83 / 100 / 83 / 94; of 128: 192 pairs 139 / 175 / 189 / 224, 128 pairs 130 / 124 / 126 / 150; fp16, heads of 16: 384 pairs
+//   117 / 100 / 105 / 111; fp32, heads of 128: 192 pairs 433 / 483 / 431 / 461, 128 pairs 430 / 343 / 296 / 314
+// backward: bf16, heads of 64: 128 pairs 107 / 131 / 127 / 142, 64 pairs 80 / 87 / 65 / 70; of 128: 96 pairs 213 / 241 / 238 / 274;
+//   fp32, heads of 128: 128 pairs 693 / 728 / 718 / 763, 96 pairs 688 / 711 / 586 / 588.
+// Of 96 cases of 16-bit heads the rule misses the best of the four by more than 6 % in 14, by up to 18 % (fp16 heads of up to 32
+// backwards, 64 pairs: 62 us where 8 segments take 51).
 // No segment is shorter than 64 tokens or than twice the head: its state is written, scanned and read again.
 int walk_nseg(int B, int T, int H, int dk, int dv, int dtype, int backward) {
   static const int rule[3][2][4][2] = {   // {full, target} by type, direction and heads of up to 16, 32, 64, 128
