@@ -396,7 +396,7 @@ int noise_layer_norm_bwd(const void* dy, long lddy, const void* x, long ldx, con
  * (elements between clips, tokens and heads of q, k, v, o: 12 values on the HOST; unit stride on the last axis, a token stride
  * of at least the row's width and below 2^22); rows of o at and behind the length are zero.  log_decay g [H] <= 0; lengths [B]
  * or NULL (all T); state (before the first token), end (behind the last) [B][H][dk][dv] fp32 or NULL (zero; not wanted).
- * state and end must not share memory.  1 <= dk, dv <= 128.  workspace: noise_decay_attn_workspace() floats (0: may be NULL) */
+ * state and end must not share memory.  1 <= dk, dv <= 128, T <= 2^30, B H <= 2^22.  workspace: noise_decay_attn_workspace() floats (0: may be NULL) */
 long noise_decay_attn_workspace(int B, int T, int H, int dk, int dv, int dtype, int backward);
 int noise_decay_attn_fwd(const void* q, const void* k, const void* v, void* o, const long* strides, const float* log_decay,
                          const int* lengths, const float* state, float* end, float* workspace, float scale, int B, int T, int H,

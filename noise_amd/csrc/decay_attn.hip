@@ -918,12 +918,11 @@ void walk_launch_16(const WalkSet& set, int n, int sums, hipStream_t st) {
   const int d = set.w[0].dk > set.w[0].dv ? set.w[0].dk : set.w[0].dv;
   const bool vec = walk_vec(set, n);
   // tokens per chunk: 32 for heads of 128, where 64 spill registers (273 -> 251 us for 32 clips of 2048 tokens, 16 heads; at 32 the
-  // kernels for rows of 16-byte pieces spill none, those for single values some), and for bf16
+  // kernels for rows of 16-byte pieces still spill 3 in bf16 and 7 in fp16, those for single values 36 and 55), and for bf16
   // heads of up to 64, where 64 cost a workgroup per CU: heads of 64, 64 clips of 2048 tokens, 8 heads 139 -> 126 us (fp16: 150 ->
-  // 163); heads of 16, 64 clips of 1001 forward 44 -> 39 us, backward 109 -> 97 (fp16: 66 -> 72 and 133 -> 109, so by
-  // direction there).  One long clip, which has few workgroups
-  // anyway, loses by it: 60001 tokens with 16 heads of 32 283 -> 331 us backward.  A pass that keeps only the state has the
-  // registers for 64 (60001 tokens, 16 heads of 128: 149 -> 134 us)
+  // 163); heads of 16, 64 clips of 1001 forward 44 -> 39 us, backward 109 -> 97 (fp16: 66 -> 72 and 133 -> 109, so by direction
+  // there).  One long clip, which has few workgroups anyway, loses by it: 60001 tokens with 16 heads of 32 283 -> 331 us
+  // backward.  A pass that keeps only the state has the registers for 64 (60001 tokens, 16 heads of 128: 149 -> 134 us)
   constexpr int C64 = __is_same(T, bf16_t) ? 32 : 64;
   walk_passes(set, n, sums, st, [&](dim3 grid, auto only) {
     constexpr bool ONLY = decltype(only)::value;
