@@ -662,9 +662,9 @@ __global__ __launch_bounds__(P * 4, P == 128 ? 4 : 3) void walk_16_kernel(WalkSe
 #pragma unroll
       for (int it = 0; it < NI; ++it) O[it] = f32x4{0.f, 0.f, 0.f, 0.f};
       // All of the first terms, then the second ones, which are formed while the products run; in wide heads they add to tiles of
-      // their own, so that the two do not wait for each other, and where registers are short (LEAN: fp16, single values) each pair
-      // of terms is used up at once (fp16, 8 clips of 2048 tokens, 16 heads of 100: 348 -> 297 us)
-      constexpr bool LEAN = P == 128 && (F16 || !VEC), APART = P == 128 && !LEAN;
+      // their own, so that the two do not wait for each other (bf16), and where registers are short (LEAN: fp16, single values) each
+      // pair of terms is used up at once (fp16, 8 clips of 2048 tokens, 16 heads of 100: 348 -> 297 us)
+      constexpr bool LEAN = P == 128 && (F16 || !VEC), APART = P == 128 && !F16;   // APART: the same sums whatever VEC is
       u32x4 low[KP];
       x8<T> y[KP][NI];
       f32x4 R[NI];
@@ -924,7 +924,7 @@ void walk_launch_16(const WalkSet& set, int n, int sums, hipStream_t st) {
   const int d = set.w[0].dk > set.w[0].dv ? set.w[0].dk : set.w[0].dv;
   const bool vec = walk_vec(set, n);
   // tokens per chunk: 32 for heads of 128, where 64 spill registers (273 -> 251 us for 32 clips of 2048 tokens, 16 heads; at 32 the
-  // kernels for rows of 16-byte pieces spill 3 in bf16 and none in fp16, those for single values 7 and 30), and for bf16
+  // kernels for rows of 16-byte pieces spill 3 in bf16 and none in fp16, those for single values 11 and 30), and for bf16
   // heads of up to 64, where 64 cost a workgroup per CU: heads of 64, 64 clips of 2048 tokens, 8 heads 139 -> 126 us (fp16: 150 ->
   // 163); heads of 16, 64 clips of 1001 forward 44 -> 39 us, backward 109 -> 97 (fp16: 66 -> 72 and 133 -> 109, so by direction
   // there).  One long clip, which has few workgroups anyway, loses by it: 60001 tokens with 16 heads of 32 283 -> 331 us
